@@ -83,6 +83,14 @@ SIGNATURES = {
     "b200_gemm_splitk": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p] + [c_int64] * 12 + [c_double, c_double, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
     "b200_gemm_f32_scratch_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
     "b200_gemm_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p] + [c_int64] * 12 + [c_double, c_double, c_void_p, c_int64, c_void_p, c_void_p]),
+    "b200_gated_linear_scratch_bytes": (c_int64, [c_void_p] * 2 + [c_int64] * 7),
+    "b200_gated_linear": (c_int, [c_void_p] * 4 + [c_int64] * 7 + [c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
+    "b200_gate": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "b200_gate_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "b200_dropout": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_double, c_void_p, c_int64, c_int, c_void_p]),
+    "b200_quantize_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]),
+    "b200_mm_int8_scratch_bytes": (c_int64, [c_void_p] * 2 + [c_int64] * 7),
+    "b200_mm_int8": (c_int, [c_void_p] * 6 + [c_int64] * 7 + [c_int, c_void_p, c_int64, c_void_p, c_void_p]),
     "b200_allclose": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_double, c_double, c_void_p, c_int, c_void_p]),
     "b200_l2_flush": (c_int, [c_void_p, c_int64, c_void_p]),
 }

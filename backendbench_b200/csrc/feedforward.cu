@@ -1,0 +1,347 @@
+// What stands around the products of a feed-forward block: the gate of a projection pair and its gradient, dropout
+// whose mask is drawn from a counter, and the quantisation of rows to 8 bits. All are one pass over their data.
+#include "b200_common.cuh"
+#include "gate_act.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr int kFfThreads = 256;
+
+// ------------------------------------------------------------------ the gate
+// h = act(g) * u of projections P = [g | u] (M x 2 N). fp32 products come in two steps (their sums are
+// put together from six plane products over several launches), so the gate has a kernel of its own there.
+// VEC elements to a thread: 16 bytes of each operand where rows are on the grid, else one.
+template <typename T, typename ACT, int VEC>
+__global__ void __launch_bounds__(kFfThreads) gate_forward(const T* p, T* __restrict__ h, int64_t M, int64_t N) {
+  const int64_t per_row = N / VEC, total = M * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kFfThreads) {
+    const int64_t m = total <= 0xffffffffll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(per_row) : i / per_row;
+    const T* row = p + i * VEC + m * N;  // m rows of 2 N, not N, lie before
+    float g[VEC], u[VEC];
+    if constexpr (VEC > 1) {
+      widen<T>(ld_stream(row), g);
+      widen<T>(ld_stream(row + N), u);
+    } else {
+      g[0] = to_f32(row[0]);
+      u[0] = to_f32(row[N]);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) g[e] = ACT::template f<sizeof(T) == 2>(g[e]) * u[e];
+    if constexpr (VEC > 1) *reinterpret_cast<uint4*>(h + i * VEC) = narrow<T>(g);
+    else h[i] = from_f32<T>(g[0]);
+  }
+}
+
+// dP = [dh * u * act'(g) | dh * act(g)]
+template <typename T, typename ACT, int VEC>
+__global__ void __launch_bounds__(kFfThreads) gate_backward(const T* dh, const T* p, T* __restrict__ dp, int64_t M, int64_t N) {
+  const int64_t per_row = N / VEC, total = M * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kFfThreads) {
+    const int64_t m = total <= 0xffffffffll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(per_row) : i / per_row;
+    const int64_t at = i * VEC + m * N;
+    float d[VEC], g[VEC], u[VEC];
+    if constexpr (VEC > 1) {
+      const uint4 rd = ld_stream(dh + i * VEC), rg = ld_stream(p + at), ru = ld_stream(p + at + N);
+      widen<T>(rd, d);
+      widen<T>(rg, g);
+      widen<T>(ru, u);
+    } else {
+      d[0] = to_f32(dh[i]);
+      g[0] = to_f32(p[at]);
+      u[0] = to_f32(p[at + N]);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float a, s;
+      ACT::template both<sizeof(T) == 2>(g[e], a, s);
+      g[e] = d[e] * u[e] * s;
+      u[e] = d[e] * a;
+    }
+    if constexpr (VEC > 1) {  // (both products read it next: not streamed past L2)
+      *reinterpret_cast<uint4*>(dp + at) = narrow<T>(g);
+      *reinterpret_cast<uint4*>(dp + at + N) = narrow<T>(u);
+    } else {
+      dp[at] = from_f32<T>(g[0]);
+      dp[at + N] = from_f32<T>(u[0]);
+    }
+  }
+}
+
+inline int ff_grid(int64_t items) {
+  const int64_t b = (items + kFfThreads - 1) / kFfThreads, most = kNumSMs * 16LL;
+  return static_cast<int>(b < most ? b : most);
+}
+
+template <typename T> int launch_gate(const void* dh, const void* p, void* out, int64_t M, int64_t N, int act, cudaStream_t st) {
+  constexpr int kVec = 16 / sizeof(T);
+  const bool vec = N % kVec == 0 && aligned16(p) && aligned16(out) && (!dh || aligned16(dh));
+  const int grid = ff_grid(M * N / (vec ? kVec : 1));
+  const T *tp = static_cast<const T*>(p), *td = static_cast<const T*>(dh);
+  T* to = static_cast<T*>(out);
+  gate_act_each(act, [&](auto a) {
+    using A = decltype(a);
+    if (dh) {
+      if (vec) gate_backward<T, A, kVec><<<grid, kFfThreads, 0, st>>>(td, tp, to, M, N);
+      else gate_backward<T, A, 1><<<grid, kFfThreads, 0, st>>>(td, tp, to, M, N);
+    } else {
+      if (vec) gate_forward<T, A, kVec><<<grid, kFfThreads, 0, st>>>(tp, to, M, N);
+      else gate_forward<T, A, 1><<<grid, kFfThreads, 0, st>>>(tp, to, M, N);
+    }
+  });
+  return check_launch();
+}
+
+int gate(const void* dh, const void* p, void* out, int64_t M, int64_t N, int act, int dtype, cudaStream_t st) {
+  switch (dtype) {
+    case B200_F32: return launch_gate<float>(dh, p, out, M, N, act, st);
+    case B200_BF16: return launch_gate<__nv_bfloat16>(dh, p, out, M, N, act, st);
+    default: return launch_gate<__half>(dh, p, out, M, N, act, st);
+  }
+}
+
+// ------------------------------------------------------------------ dropout
+// y_i = residual_i + (word_i >= threshold ? x_i * scale : 0), word_i = word i % 4 of Philox-4x32 with ten rounds
+// (J. Salmon, M. Moraes, R. Dror, D. Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011) for the 128-bit counter
+// (offset + i / 4, subsequence) under the 64-bit key `seed`. Nothing but the counter goes into an element's
+// word, so the backward pass draws the same mask again instead of reading one, whatever the launch shape.
+// What is dropped is not multiplied: an infinity or a NaN in a dropped place leaves nothing.
+struct PhiloxKeys {
+  uint32_t k[20];
+  __device__ __forceinline__ explicit PhiloxKeys(uint64_t seed) {
+    uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+      k[2 * r] = k0;
+      k[2 * r + 1] = k1;
+      k0 += 0x9E3779B9u;
+      k1 += 0xBB67AE85u;
+    }
+  }
+};
+__device__ __forceinline__ void philox(const PhiloxKeys& key, uint64_t count, uint64_t subsequence, uint32_t* w) {
+  uint32_t a = static_cast<uint32_t>(count), b = static_cast<uint32_t>(count >> 32), c = static_cast<uint32_t>(subsequence), d = static_cast<uint32_t>(subsequence >> 32);
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t p = static_cast<uint64_t>(a) * 0xD2511F53u, q = static_cast<uint64_t>(c) * 0xCD9E8D57u;
+    a = static_cast<uint32_t>(q >> 32) ^ b ^ key.k[2 * r];
+    c = static_cast<uint32_t>(p >> 32) ^ d ^ key.k[2 * r + 1];
+    b = static_cast<uint32_t>(q);
+    d = static_cast<uint32_t>(p);
+  }
+  w[0] = a;
+  w[1] = b;
+  w[2] = c;
+  w[3] = d;
+}
+
+struct DropoutArgs {
+  int64_t n;
+  uint64_t subsequence;
+  const int64_t* state;  // seed, offset
+  uint32_t threshold;
+  int mode;              // 0: nothing is dropped, 1: by the words, 2: everything
+  float scale;
+};
+
+// VEC = 16 bytes of elements (one or two counters) or four elements (unaligned: one counter)
+template <typename T, bool VECTOR>
+__global__ void __launch_bounds__(kFfThreads) dropout_kernel(const T* x, const T* residual, T* __restrict__ y, DropoutArgs A) {
+  constexpr int kPer = VECTOR ? 16 / static_cast<int>(sizeof(T)) : 4;
+  const PhiloxKeys key(static_cast<uint64_t>(A.state[0]));
+  const uint64_t offset = static_cast<uint64_t>(A.state[1]);
+  const int64_t groups = (A.n + kPer - 1) / kPer;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x; i < groups; i += static_cast<int64_t>(gridDim.x) * kFfThreads) {
+    const int64_t at = i * kPer;
+    const int left = A.n - at < kPer ? static_cast<int>(A.n - at) : kPer;
+    float v[kPer], r[kPer];
+    uint4 rx, rr;
+    const bool whole = VECTOR && left == kPer;
+    if (whole) {
+      rx = ld_stream(x + at);
+      if (residual) rr = ld_stream(residual + at);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        v[e] = e < left ? to_f32(x[at + e]) : 0.f;
+        r[e] = residual && e < left ? to_f32(residual[at + e]) : 0.f;
+      }
+    }
+    uint32_t w[kPer];
+    if (A.mode == 1) {
+#pragma unroll
+      for (int c = 0; c < kPer / 4; ++c) philox(key, offset + static_cast<uint64_t>(i) * (kPer / 4) + c, A.subsequence, w + 4 * c);
+    }
+    if (whole) {
+      widen<T>(rx, v);
+      if (residual) widen<T>(rr, r);
+    }
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const bool keep = A.mode == 0 || (A.mode == 1 && w[e] >= A.threshold);
+      v[e] = keep ? v[e] * A.scale : 0.f;
+      if (residual) v[e] += r[e];
+    }
+    if (whole) {
+      st_stream(y + at, narrow<T>(v));
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        if (e < left) y[at + e] = from_f32<T>(v[e]);
+    }
+  }
+}
+
+template <typename T> int launch_dropout(const void* x, const void* residual, void* y, const DropoutArgs& A, cudaStream_t st) {
+  const bool vec = aligned16(x) && aligned16(y) && (!residual || aligned16(residual));
+  const int64_t per = vec ? 16 / static_cast<int>(sizeof(T)) : 4;
+  const int grid = ff_grid((A.n + per - 1) / per);
+  const T *tx = static_cast<const T*>(x), *tr = static_cast<const T*>(residual);
+  if (vec) dropout_kernel<T, true><<<grid, kFfThreads, 0, st>>>(tx, tr, static_cast<T*>(y), A);
+  else dropout_kernel<T, false><<<grid, kFfThreads, 0, st>>>(tx, tr, static_cast<T*>(y), A);
+  return check_launch();
+}
+
+// ------------------------------------------------------------------ rows to 8 bits
+// scale = max|x| / 127, q = x * (127 / max|x|) rounded to even; a row of zeros (or of values below 2^-118, whose
+// reciprocal scale would overflow) has scale 0 and zeros, a row with an infinity or a NaN has that as its scale and zeros.
+// NV vectors of 16 bytes to a thread: the row is read once and stays in registers. NV = 0: any length
+// and alignment, read twice.
+constexpr float kLeastMax = 3.0092655e-36f;  // 2^-118
+
+__device__ __forceinline__ float abs_max_nan(float m, float v) {  // a NaN stays
+  const float a = fabsf(v);
+  return a > m || a != a ? a : m;
+}
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* x, int8_t* __restrict__ q, float* __restrict__ scale, int64_t cols, int64_t pitch) {
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  __shared__ float part[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  next_grid_may_start();  // (the product's CTAs set themselves up meanwhile)
+  const T* row = x + blockIdx.x * pitch;
+  int8_t* qrow = q + blockIdx.x * cols;
+  float m = 0.f;
+  uint4 raw[NV ? NV : 1];
+  if constexpr (NV) {
+    const int64_t vecs = cols / kPer;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int64_t j = tid + static_cast<int64_t>(k) * blockDim.x;
+      raw[k] = j < vecs ? ld_stream(row + j * kPer) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float v[kPer];
+      widen<T>(raw[k], v);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) m = abs_max_nan(m, v[e]);
+    }
+  } else {
+    for (int64_t j = tid; j < cols; j += blockDim.x) m = abs_max_nan(m, to_f32(row[j]));
+  }
+  auto all = [&](float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = abs_max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  };
+  m = all(m);
+  if (lane == 0) part[warp] = m;
+  __syncthreads();
+  m = all(lane < static_cast<int>((blockDim.x + 31) >> 5) ? part[lane] : 0.f);
+  const bool some = m >= kLeastMax && m <= 3.402823466e38f;
+  const float inv = some ? __fdiv_rn(127.f, m) : 0.f;
+  if (tid == 0) scale[blockIdx.x] = m < kLeastMax ? 0.f : __fdiv_rn(m, 127.f);
+  auto one = [&](float v) { return some ? __float2int_rn(v * inv) : 0; };
+  if constexpr (NV) {
+    const int64_t vecs = cols / kPer;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int64_t j = tid + static_cast<int64_t>(k) * blockDim.x;
+      if (j >= vecs) break;
+      float v[kPer];
+      widen<T>(raw[k], v);
+      uint32_t w[kPer / 4];
+#pragma unroll
+      for (int e = 0; e < kPer / 4; ++e)
+        w[e] = (one(v[4 * e]) & 0xff) | (one(v[4 * e + 1]) & 0xff) << 8 | (one(v[4 * e + 2]) & 0xff) << 16 | static_cast<uint32_t>(one(v[4 * e + 3])) << 24;
+      if constexpr (kPer == 8) *reinterpret_cast<uint2*>(qrow + j * 8) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(qrow + j * 4) = w[0];
+    }
+  } else {
+    for (int64_t j = tid; j < cols; j += blockDim.x) qrow[j] = static_cast<int8_t>(one(to_f32(row[j])));
+  }
+}
+
+template <typename T> void launch_quantize(const void* x, void* q, void* scale, int64_t rows, int64_t cols, int64_t pitch, cudaStream_t st) {
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  const T* tx = static_cast<const T*>(x);
+  int8_t* tq = static_cast<int8_t*>(q);
+  float* ts = static_cast<float*>(scale);
+  const bool vec = aligned16(x) && cols % kPer == 0 && (rows == 1 || pitch % kPer == 0) && (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
+  const int64_t vecs = cols / kPer;
+  auto threads = [](int64_t n) { return static_cast<int>(n >= 1024 ? 1024 : n <= 32 ? 32 : (n + 31) / 32 * 32); };
+  auto go = [&](auto kernel, int t) { kernel<<<static_cast<unsigned>(rows), t, 0, st>>>(tx, tq, ts, cols, pitch); };
+  if (vec && vecs <= 512) return go(quantize_rows_kernel<T, 1>, threads(vecs));
+  if (vec && vecs <= 1024) return go(quantize_rows_kernel<T, 2>, threads((vecs + 1) / 2));
+  if (vec && vecs <= 4096) return go(quantize_rows_kernel<T, 4>, threads((vecs + 3) / 4));
+  return go(quantize_rows_kernel<T, 0>, threads((cols + 3) / 4));
+}
+
+}  // namespace
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_gate(const void* projections, void* out, int64_t M, int64_t N, int activation, int dtype, void* stream) {
+  if (M < 0 || N < 0 || activation < 0 || activation >= B200_ACT_COUNT) return B200_EINVAL;
+  if (!is_float_dtype(dtype)) return B200_EDTYPE;
+  if (M == 0 || N == 0) return B200_OK;
+  if (!projections || !out) return B200_EINVAL;
+  return gate(nullptr, projections, out, M, N, activation, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b200_gate_backward(const void* grad, const void* projections, void* grad_projections, int64_t M, int64_t N, int activation, int dtype, void* stream) {
+  if (M < 0 || N < 0 || activation < 0 || activation >= B200_ACT_COUNT) return B200_EINVAL;
+  if (!is_float_dtype(dtype)) return B200_EDTYPE;
+  if (M == 0 || N == 0) return B200_OK;
+  if (!grad || !projections || !grad_projections) return B200_EINVAL;
+  return gate(grad, projections, grad_projections, M, N, activation, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b200_dropout(const void* x, const void* residual, void* out, int64_t n, double p, const int64_t* state, int64_t subsequence, int dtype, void* stream) {
+  if (n < 0 || !(p >= 0. && p <= 1.)) return B200_EINVAL;
+  if (!is_float_dtype(dtype)) return B200_EDTYPE;
+  if (n == 0) return B200_OK;
+  if (!x || !out || !state) return B200_EINVAL;
+  const double words = p * 4294967296.;
+  DropoutArgs A;
+  A.n = n;
+  A.subsequence = static_cast<uint64_t>(subsequence);
+  A.state = state;
+  const uint64_t threshold = static_cast<uint64_t>(nearbyint(words));
+  A.mode = threshold == 0 ? 0 : threshold > 0xffffffffull ? 2 : 1;
+  A.threshold = static_cast<uint32_t>(threshold);
+  A.scale = p < 1. ? static_cast<float>(1. / (1. - p)) : 0.f;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case B200_F32: return launch_dropout<float>(x, residual, out, A, st);
+    case B200_BF16: return launch_dropout<__nv_bfloat16>(x, residual, out, A, st);
+    default: return launch_dropout<__half>(x, residual, out, A, st);
+  }
+}
+
+extern "C" int b200_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t row_stride, int dtype, void* stream) {
+  if (rows < 0 || cols < 0 || rows > 0x7fffffffLL) return B200_EINVAL;
+  if (!is_float_dtype(dtype)) return B200_EDTYPE;
+  if (rows == 0) return B200_OK;
+  if (!scale || (cols && (!x || !q))) return B200_EINVAL;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == B200_F32) launch_quantize<float>(x, q, scale, rows, cols, row_stride, st);
+  else if (dtype == B200_BF16) launch_quantize<__nv_bfloat16>(x, q, scale, rows, cols, row_stride, st);
+  else launch_quantize<__half>(x, q, scale, rows, cols, row_stride, st);
+  return check_launch();
+}

@@ -1,0 +1,616 @@
+// The linear layers of a feed-forward block on the 5th-generation tensor cores:
+//
+//   gated   h[m, n] = act(g[m, n]) * u[m, n],  g = x Wg^T, u = x Wu^T   (bf16 / f16, W = [Wg; Wu], 2 N x K)
+//   int8    y[m, n] = (sum_k a[m, k] b[n, k]) * sa[m] * sb[n] + bias[n]   (int8 operands, exact 32-bit sums)
+//
+// Both read operands whose rows lie along K, in slabs of 128 bytes, and both need the whole accumulator of a tile
+// before anything is written, so they share one kernel: a TMA producer warp, a warp that issues tcgen05.mma
+// (kind::f16 or kind::i8, four steps of 32 bytes of K to a slab), two accumulators of 256 columns in tensor memory and eight
+// epilogue warps that empty one while the other fills.
+//
+// Gated: a tile of w outputs takes w rows of Wg and the same w rows of Wu as ONE B operand of 2 w rows, so that gate
+// and up land side by side in the accumulator of the same lane: x crosses into shared memory once for both,
+// and act(g) * u is formed from the fp32 sums with one rounding (training: g and u are rounded once each
+// and written beside it). A pair of CTAs (cta_group::2, 256 rows) splits it the natural way: the even CTA loads the
+// gate rows, the odd one the up rows.
+//
+// Few rows (decoding): what counts is that every SM streams its share of the weights without a pause. A tile's width is
+// any multiple of 8 (16) columns, chosen so that the tiles come out even over the SMs, and the A slab has as many
+// rows as there are; the MMA's other rows multiply whatever lies behind it and are never stored.
+#include <cuda.h>
+
+#include "b200_common.cuh"
+#include "gate_act.cuh"
+#include "tc_common.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr int kLinThreads = 320;                        // TMA warp, MMA warp, 8 epilogue warps
+constexpr int kSlabBytes = 128;                         // of K to a slab: one row of the 128-byte swizzle
+constexpr int kLinRing = 192 * 1024;
+constexpr int kLinEpiWarps = 8, kLinEpiBytes = 4096;    // staging: 32 rows x 128 bytes per epilogue warp
+constexpr int kLinMaxStages = 16;
+constexpr int kLinAccCols = 256, kLinAccs = 2;
+constexpr size_t kLinSmem = static_cast<size_t>(kLinRing) + kLinEpiWarps * kLinEpiBytes + 1024 /*align*/ + 512 /*barriers*/;
+constexpr uint64_t kLinWaitNs = 2000000000ull;
+
+enum : int { kGated = 0, kInt8 = 1 };
+
+struct LinParams {
+  int64_t M, N, K;        // outputs M x N; K in elements
+  int w;                  // output columns of a tile
+  int a_rows, b_rows;     // rows of the A box; rows of one B box
+  int b_boxes;            // boxes of B in this CTA's stage (gated on a single CTA: gate and up)
+  int k_step;             // elements of K to a slab
+  int group_m;            // row blocks per rasterisation group
+  uint32_t idesc;
+  int act;                // gated: activation
+  void* side;             // gated: the projections [M, 2 N], or NULL
+  const float* a_scale;   // int8
+  const float* b_scale;
+  const void* bias;       // int8: [N] of the output type, or NULL
+};
+
+__device__ __forceinline__ void lin_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, bool i8) {
+  if (i8) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  } else {
+    tc_mma_f16(d, a, b, idesc, accumulate);
+  }
+}
+__device__ __forceinline__ void lin_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, bool i8) {
+  if (i8) {
+    const uint32_t z = 0u;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z)
+        : "memory");
+  } else {
+    tc_mma_f16_pair(d, a, b, idesc, accumulate);
+  }
+}
+
+__device__ __forceinline__ void lin_tile(int64_t t, int64_t mt, int64_t nt, int group_m, int& mb, int& nb) {
+  const int64_t per_group = static_cast<int64_t>(group_m) * nt;
+  const int64_t g = t / per_group, in_g = t - g * per_group;
+  const int64_t left = mt - g * group_m, gm = left < group_m ? left : group_m;
+  mb = static_cast<int>(g * group_m + in_g % gm);
+  nb = static_cast<int>(in_g / gm);
+}
+
+// 32 values of a lane's row to 32 columns of `out` (row pitch `pitch`, column 0 at `col`): rounded once into the warp's
+// staging buffer (16-byte pieces swizzled so that neither side meets a bank twice), then out in 16-byte pieces of
+// eight (fp32: four) rows at a time, or element by element where rows are off the grid.
+template <typename TO>
+__device__ __forceinline__ void lin_store(const float* v, unsigned char* mine, TO* out, int64_t pitch, int nrows, int ncols, bool vec, int lane) {
+  constexpr int kRow = 32 * static_cast<int>(sizeof(TO)), kPieces = kRow / 16, kPer = 16 / static_cast<int>(sizeof(TO)), kShift = sizeof(TO) == 2 ? 1 : 0;
+  __syncwarp();  // what was there has been read out
+#pragma unroll
+  for (int j = 0; j < kPieces; ++j) *reinterpret_cast<uint4*>(mine + lane * kRow + ((j ^ ((lane >> kShift) & (kPieces - 1))) << 4)) = narrow<TO>(v + j * kPer);
+  __syncwarp();
+  if (vec) {
+    constexpr int kRowsAt = 32 / kPieces;
+    const int j = lane % kPieces, r0 = lane / kPieces;
+    if (j * kPer < ncols) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int r = r0 + i * kRowsAt;
+        if (r < nrows) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * pitch + j * kPer) = *reinterpret_cast<const uint4*>(mine + r * kRow + ((j ^ ((r >> kShift) & (kPieces - 1))) << 4));
+      }
+    }
+  } else if (lane < ncols) {
+    const int j = lane / kPer, e = lane % kPer;
+    for (int r = 0; r < nrows; ++r) out[static_cast<int64_t>(r) * pitch + lane] = *(reinterpret_cast<const TO*>(mine + r * kRow + ((j ^ ((r >> kShift) & (kPieces - 1))) << 4)) + e);
+  }
+}
+
+template <int MODE, typename TO, bool kPair>
+__global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, TO* __restrict__ out, LinParams p, uint32_t* __restrict__ status) {
+  constexpr bool kI8 = MODE == kInt8;
+  constexpr int kTileM = kPair ? 256 : 128;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  unsigned char* epi_stage = smem + kLinRing;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kLinRing + kLinEpiWarps * kLinEpiBytes);
+  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(bars + 2 * kLinMaxStages + 2 * kLinAccs);
+  volatile uint32_t* abort_flag = tmem_base_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t smem_base = smem_u32(smem), bar_base = smem_u32(bars);
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (kLinMaxStages + s); };
+  auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * kLinMaxStages + a); };
+  auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * kLinMaxStages + kLinAccs + a); };
+  const uint32_t a_bytes = static_cast<uint32_t>(p.a_rows) * kSlabBytes, b_bytes = static_cast<uint32_t>(p.b_rows) * kSlabBytes;
+  const uint32_t stage_bytes = a_bytes + static_cast<uint32_t>(p.b_boxes) * b_bytes;
+  const int fit = kLinRing / static_cast<int>(stage_bytes), stages = fit < kLinMaxStages ? fit : kLinMaxStages;
+  const uint32_t cta_rank = kPair ? cluster_ctarank() : 0u;
+
+  if (threadIdx.x == 64) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_a)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_b)) : "memory");
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < kLinAccs; ++a) {
+      mbar_init(tfull_bar(a), 1);
+      mbar_init(tempty_bar(a), kPair ? 16 : 8);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    if (kPair) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)), "r"(kLinAccs * kLinAccCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)), "r"(kLinAccs * kLinAccCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (kPair) cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_base_slot;
+  after_grids_before();
+  const float *a_scale = waited(p.a_scale), *b_scale = waited(p.b_scale);
+  const TO* bias = waited(static_cast<const TO*>(p.bias));
+
+  const int64_t mt = (p.M + kTileM - 1) / kTileM, nt = (p.N + p.w - 1) / p.w, tiles = mt * nt;
+  const int64_t tile_first = kPair ? (blockIdx.x >> 1) : blockIdx.x, tile_step = kPair ? (gridDim.x >> 1) : gridDim.x;
+  const int slabs = static_cast<int>((p.K + p.k_step - 1) / p.k_step);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int64_t t = tile_first; t < tiles && ok; t += tile_step) {
+        int mb, nb;
+        lin_tile(t, mt, nt, p.group_m, mb, nb);
+        const int m0 = mb * kTileM + static_cast<int>(cta_rank) * 128;
+        // gated: the gate rows n0.., then the up rows N + n0..; a pair has a box of B to each CTA
+        int n0 = nb * p.w, n1 = n0 + static_cast<int>(p.N);
+        if (kPair && cta_rank == 1u) n0 = kI8 ? n0 + p.b_rows : n1;
+        for (int kb = 0; kb < slabs; ++kb) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, kLinWaitNs)) { ok = false; break; }
+          const uint32_t a_dst = smem_base + stage * stage_bytes, b_dst = a_dst + a_bytes;
+          const int k = kb * p.k_step;
+          if (kPair) {
+            const uint32_t fbar = map_to_cta(full_bar(stage), 0u);
+            if (cta_rank == 0u) mbar_expect_tx(full_bar(stage), 2 * stage_bytes);
+            tma_load_3d_pair(a_dst, &map_a, fbar, k, m0, 0);
+            tma_load_3d_pair(b_dst, &map_b, fbar, k, n0, 0);
+          } else {
+            mbar_expect_tx(full_bar(stage), stage_bytes);
+            tma_load_3d(b_dst, &map_b, full_bar(stage), k, n0, 0);
+            if (!kI8) tma_load_3d(b_dst + b_bytes, &map_b, full_bar(stage), k, n1, 0);
+            tma_load_3d(a_dst, &map_a, full_bar(stage), k, m0, 0);
+          }
+          if (++stage == stages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (kPair && ok) {
+        // the even CTA's commits arrive here from afar: none may land after this CTA's shared memory is gone
+        for (int i = 0; i < stages && ok; ++i) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, kLinWaitNs)) ok = false;
+          if (++stage == stages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        if (status) atomicOr(status, B200_DEV_WAIT_TIMEOUT);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (the whole warp walks, one lane issues)
+    if (cta_rank == 0u) {
+      const uint32_t empty0 = kPair ? map_to_cta(empty_bar(0), 0u) : 0u, empty1 = kPair ? map_to_cta(empty_bar(0), 1u) : 0u;
+      auto warp_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, kLinWaitNs)) != 0; };
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int64_t t = tile_first; t < tiles && ok; t += tile_step) {
+        if (!warp_wait(tempty_bar(acc), acc_phase ^ 1u)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kLinAccCols);
+        for (int kb = 0; kb < slabs; ++kb) {
+          if (!warp_wait(full_bar(stage), phase)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a_addr = smem_base + stage * stage_bytes, b_addr = a_addr + a_bytes;
+          uint64_t da[4], db[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            da[k] = smem_desc(a_addr + k * 32u, 16u, 1024u);
+            db[k] = smem_desc(b_addr + k * 32u, 16u, 1024u);
+          }
+          const uint32_t e0 = kPair ? empty0 + 8u * stage : empty_bar(stage), e1 = empty1 + 8u * stage;
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (kPair) lin_mma_pair(d_tmem, da[k], db[k], p.idesc, (kb | k) != 0 ? 1u : 0u, kI8);
+              else lin_mma(d_tmem, da[k], db[k], p.idesc, (kb | k) != 0 ? 1u : 0u, kI8);
+            }
+            if (kPair) {
+              tc_commit_pair(e0);
+              tc_commit_pair(e1);
+            } else {
+              tc_commit(e0);
+            }
+          }
+          __syncwarp();
+          if (++stage == stages) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        if (elect_one()) {
+          if (kPair) {
+            tc_commit_pair(map_to_cta(tfull_bar(acc), 0u));
+            tc_commit_pair(map_to_cta(tfull_bar(acc), 1u));
+          } else {
+            tc_commit(tfull_bar(acc));
+          }
+        }
+        __syncwarp();
+        if (++acc == kLinAccs) { acc = 0; acc_phase ^= 1u; }
+      }
+      if (!ok && lane == 0) {
+        *abort_flag = 1;
+        if (status) atomicOr(status, B200_DEV_WAIT_TIMEOUT);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue: 32 columns at a time, two warps to a lane quarter
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    unsigned char* mine = epi_stage + (warp - 2) * kLinEpiBytes;
+    constexpr int kPer = 16 / static_cast<int>(sizeof(TO)), kRegs = kI8 ? 32 : 64;
+    const bool vec = p.N % kPer == 0 && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(p.side)) & 15u) == 0;
+    const bool scales_vec = kI8 && ((reinterpret_cast<uintptr_t>(p.b_scale) | reinterpret_cast<uintptr_t>(p.bias)) & 15u) == 0;  // (a chunk starts at a multiple of 16)
+    const uint32_t tempty_target = kPair ? map_to_cta(tempty_bar(0), 0u) : 0u;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int64_t t = tile_first; t < tiles && ok; t += tile_step) {
+      int mb, nb;
+      lin_tile(t, mt, nt, p.group_m, mb, nb);
+      const int64_t mr0 = static_cast<int64_t>(mb) * kTileM + static_cast<int64_t>(cta_rank) * 128 + q * 32, n0 = static_cast<int64_t>(nb) * p.w;
+      const int wide = p.N - n0 < p.w ? static_cast<int>(p.N - n0) : p.w;  // columns of this tile that exist
+      const int nrows = p.M - mr0 < 32 ? static_cast<int>(p.M - mr0) : 32;  // <= 0: none
+      const int chunks = (wide + 31) / 32, count = (chunks + 1 - half) / 2;  // this warp takes chunks half, half + 2, ...
+      int got = 0;
+      if (lane == 0) got = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, kLinWaitNs) ? 1 : 0;
+      got = __shfl_sync(0xffffffffu, got, 0);
+      if (!got) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t t_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * kLinAccCols);
+      uint32_t r[kRegs];
+      auto fetch = [&](int i) {
+        const uint32_t col = static_cast<uint32_t>((half + 2 * i) * 32);
+        tc_ld_32x32(t_base + col, r);
+        if constexpr (!kI8) tc_ld_32x32(t_base + static_cast<uint32_t>(p.w) + col, r + 32);
+      };
+      // the chunk's values are in `v`: the next chunk is on its way while they are rounded and stored, or, behind the last,
+      // the accumulator goes back to the MMA warp
+      auto next = [&](int i) {
+        if (i + 1 < count) {
+          fetch(i + 1);
+          return;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (kPair) mbar_arrive_cluster(tempty_target + 8u * acc);
+          else mbar_arrive(tempty_bar(acc));
+        }
+      };
+      if (count > 0) fetch(0);
+      else next(0);
+#pragma unroll 1
+      for (int i = 0; i < count; ++i) {
+        const int c0 = (half + 2 * i) * 32, ncols = wide - c0 < 32 ? wide - c0 : 32;
+        const int64_t n = n0 + c0;
+        float v[32];
+        tc_ld_wait();
+        if constexpr (kI8) {
+          const float sa = lane < nrows ? a_scale[mr0 + lane] : 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = static_cast<float>(static_cast<int>(r[e])) * sa;
+          next(i);
+          if (ncols == 32 && scales_vec) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const uint4 b = ld_keep_after(b_scale + n + e);
+              v[e] *= __uint_as_float(b.x);
+              v[e + 1] *= __uint_as_float(b.y);
+              v[e + 2] *= __uint_as_float(b.z);
+              v[e + 3] *= __uint_as_float(b.w);
+            }
+            if (bias) {
+#pragma unroll
+              for (int e = 0; e < 32; e += kPer) {
+                float b[kPer];
+                widen<TO>(ld_keep_after(bias + n + e), b);
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) v[e + j] += b[j];
+              }
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const bool in = e < ncols;
+              v[e] *= in ? b_scale[n + e] : 0.f;
+              if (bias) v[e] += in ? to_f32(bias[n + e]) : 0.f;
+            }
+          }
+        } else {
+          const float *g = reinterpret_cast<const float*>(r), *u = reinterpret_cast<const float*>(r + 32);
+          TO* side = static_cast<TO*>(p.side);
+          if (side && nrows > 0) {
+            lin_store<TO>(g, mine, side + mr0 * (2 * p.N) + n, 2 * p.N, nrows, ncols, vec, lane);
+            lin_store<TO>(u, mine, side + mr0 * (2 * p.N) + p.N + n, 2 * p.N, nrows, ncols, vec, lane);
+          }
+          gate_act_each(p.act, [&](auto act) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = act.fast(g[e]) * u[e];
+          });
+          next(i);
+        }
+        if (nrows > 0) lin_store<TO>(v, mine, out + mr0 * p.N + n, p.N, nrows, ncols, vec, lane);
+      }
+      if (++acc == kLinAccs) { acc = 0; acc_phase ^= 1u; }
+    }
+    if (!ok && lane == 0) {
+      *abort_flag = 1;
+      if (status) atomicOr(status, B200_DEV_WAIT_TIMEOUT);
+    }
+    __syncwarp();
+  }
+
+  // ---------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (*abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight land before the shared memory goes away
+    __syncthreads();
+  }
+  if (kPair) cluster_sync_all();
+  if (warp == 1) {
+    if (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kLinAccs * kLinAccCols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kLinAccs * kLinAccCols) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------ operands off the grid
+// A matrix [rows, K] of any strides into rows along K with a pitch that is a multiple of 16 bytes, for the copy engine.
+// 32 x 32 tiles through shared memory, read along whichever dimension is contiguous.
+template <typename E>
+__global__ void __launch_bounds__(256) pack_rows(const E* x, E* __restrict__ to, int64_t rows, int64_t K, int64_t s_r, int64_t s_k, int64_t pitch) {
+  __shared__ E tile[32][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t kt = (K + 31) / 32, tiles = ((rows + 31) / 32) * kt;
+  const bool along_k = s_k == 1 || s_r != 1;
+  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const int64_t r0 = t / kt * 32, k0 = (t % kt) * 32;
+    __syncthreads();
+    for (int i = ty; i < 32; i += 8) {
+      const int64_t r = r0 + (along_k ? i : tx), k = k0 + (along_k ? tx : i);
+      if (r < rows && k < K) tile[along_k ? i : tx][along_k ? tx : i] = x[r * s_r + k * s_k];
+    }
+    __syncthreads();
+    for (int i = ty; i < 32; i += 8)
+      if (r0 + i < rows && k0 + tx < K) to[(r0 + i) * pitch + k0 + tx] = tile[i][tx];
+  }
+}
+
+struct LinOperand {
+  const void* base;
+  int64_t rows, K, s_r, s_k;
+  int esize;
+  bool ready() const {  // as the copy engine takes it
+    return aligned16(base) && (s_k == 1 || K == 1) && (rows == 1 || (s_r >= K && s_r * esize % 16 == 0));
+  }
+  int64_t pitch() const { return (K * esize + 15) / 16 * 16 / esize; }
+  int64_t packed_bytes() const { return ready() ? 0 : (rows * pitch() * esize + 255) / 256 * 256; }
+};
+
+int pack(LinOperand& o, unsigned char*& at, cudaStream_t st, int& launches) {
+  if (o.ready()) {
+    if (o.rows == 1) o.s_r = o.pitch();  // never used
+    return B200_OK;
+  }
+  const int64_t tiles = ((o.rows + 31) / 32) * ((o.K + 31) / 32), most = kNumSMs * 8;
+  const int grid = static_cast<int>(tiles < most ? tiles : most);
+  if (o.esize == 2) pack_rows<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(o.base), reinterpret_cast<uint16_t*>(at), o.rows, o.K, o.s_r, o.s_k, o.pitch());
+  else pack_rows<uint8_t><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(o.base), at, o.rows, o.K, o.s_r, o.s_k, o.pitch());
+  const int64_t bytes = o.packed_bytes();
+  o.s_r = o.pitch();
+  o.s_k = 1;
+  o.base = at;
+  at += bytes;
+  ++launches;
+  return B200_OK;
+}
+
+bool encode_rows(CUtensorMap* map, const LinOperand& o, CUtensorMapDataType dt, int box_rows) {
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(o.K), static_cast<cuuint64_t>(o.rows), 1};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(o.s_r * o.esize), static_cast<cuuint64_t>(o.s_r * o.esize) * static_cast<cuuint64_t>(o.rows)};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(kSlabBytes / o.esize), static_cast<cuuint32_t>(box_rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return encode_fn()(map, dt, 3, const_cast<void*>(o.base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct LinPlan {
+  bool pair;
+  int w, a_rows;
+};
+// `per`: rows of B to an output column (gated 2, int8 1).
+LinPlan plan_linear(int64_t M, int64_t N, int64_t K, int per, int k_step) {
+  const int64_t slabs = (K + k_step - 1) / k_step;
+  const int most = 256 / per, grain = 16 / per;
+  if (M > 128 && N * per > 128 && slabs > 4) {
+    const int64_t mt = (M + 255) / 256;
+    auto rounds = [&](int w) { return (mt * ((N + w - 1) / w) + kNumSMs / 2 - 1) / (kNumSMs / 2); };
+    int best = most;
+    double least = static_cast<double>(rounds(most));
+    if (least <= 4.0) {
+      least *= 0.95;
+      for (const auto& c : {std::make_pair(most * 3 / 4, 0.83), std::make_pair(most / 2, 0.69)}) {
+        const double t = static_cast<double>(rounds(c.first)) * c.second;
+        if (t < least) { least = t; best = c.first; }
+      }
+    }
+    return LinPlan{true, best, 128};
+  }
+  const int a_rows = M >= 128 ? 128 : static_cast<int>((M + 7) / 8 * 8);
+  const int64_t mt = (M + 127) / 128;
+  int best = most;
+  double least = 0.;
+  for (int w = most; w >= grain; w -= grain) {
+    const int64_t tiles = mt * ((N + w - 1) / w), r = (tiles + kNumSMs - 1) / kNumSMs;
+    const double t = static_cast<double>(r) * (w * per + 0.4 * a_rows + 8);
+    if (least == 0. || t < least) { least = t; best = w; }
+  }
+  return LinPlan{false, best, a_rows};
+}
+
+template <typename Kernel, typename TO>
+int launch_linear(Kernel kernel, bool pair, int64_t tiles, cudaStream_t st, const CUtensorMap& map_a, const CUtensorMap& map_b, TO* out, const LinParams& p, uint32_t* status) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLinSmem));
+  if (e != cudaSuccess) { set_last_cuda_error(e); return B200_ELAUNCH; }
+  const int64_t slots = pair ? kNumSMs / 2 : kNumSMs;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((tiles < slots ? tiles : slots) * (pair ? 2 : 1)), 1, 1);
+  cfg.blockDim = dim3(kLinThreads, 1, 1);
+  cfg.dynamicSmemBytes = kLinSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // (see launch_after)
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pair ? 2 : 1;
+  const cudaError_t le = cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, out, p, status);
+  if (le != cudaSuccess) { set_last_cuda_error(le); return B200_ELAUNCH; }
+  return B200_OK;
+}
+
+template <int MODE>
+int run_linear(LinOperand a, LinOperand b, void* out, int64_t M, int64_t N, int64_t K, int dtype_out, bool is_bf16, LinParams& p, void* scratch, int64_t scratch_bytes, uint32_t* status, cudaStream_t st) {
+  constexpr int per = MODE == kGated ? 2 : 1;
+  if (!encode_fn()) return B200_EDRIVER;
+  const int64_t need = a.packed_bytes() + b.packed_bytes();
+  if (need && (!scratch || scratch_bytes < need + 256)) return B200_ESCRATCH;
+  unsigned char* at = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(scratch) + 255) & ~static_cast<uintptr_t>(255));
+  int launches = 1;
+  if (int rc = pack(a, at, st, launches)) return rc;
+  if (int rc = pack(b, at, st, launches)) return rc;
+  p.M = M; p.N = N; p.K = K;
+  p.k_step = kSlabBytes / a.esize;
+  const LinPlan plan = plan_linear(M, N, K, per, p.k_step);
+  p.w = plan.w;
+  p.a_rows = plan.a_rows;
+  p.b_rows = MODE == kGated ? plan.w : plan.pair ? plan.w / 2 : plan.w;
+  p.b_boxes = MODE == kGated && !plan.pair ? 2 : 1;
+  const int tile_m = plan.pair ? 256 : 128;
+  int64_t rows = (32ll << 20) / (K * a.esize) / 256 * 256;  // a group's panel of A stays in L2 while B goes by
+  rows = rows < 2048 ? 2048 : rows > 65536 ? 65536 : rows;
+  p.group_m = static_cast<int>(rows / tile_m);
+  const uint32_t fmt = MODE == kInt8 ? 1u /* signed */ : is_bf16 ? 1u : 0u, acc = MODE == kInt8 ? 2u /* s32 */ : 1u /* f32 */;
+  p.idesc = (acc << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(plan.w * per >> 3) << 17) | (static_cast<uint32_t>(tile_m >> 4) << 24);
+  const CUtensorMapDataType dt = MODE == kInt8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  alignas(64) CUtensorMap map_a, map_b;
+  if (!encode_rows(&map_a, a, dt, p.a_rows) || !encode_rows(&map_b, b, dt, p.b_rows)) return B200_EDRIVER;
+  const int64_t tiles = ((M + tile_m - 1) / tile_m) * ((N + plan.w - 1) / plan.w);
+  auto go = [&](auto* o) {
+    using TO = std::remove_pointer_t<decltype(o)>;
+    return plan.pair ? launch_linear(linear_tc<MODE, TO, true>, true, tiles, st, map_a, map_b, o, p, status) : launch_linear(linear_tc<MODE, TO, false>, false, tiles, st, map_a, map_b, o, p, status);
+  };
+  int rc;
+  if (dtype_out == B200_BF16) rc = go(static_cast<__nv_bfloat16*>(out));
+  else if (dtype_out == B200_F16) rc = go(static_cast<__half*>(out));
+  else if constexpr (MODE == kInt8) rc = go(static_cast<float*>(out));
+  else return B200_EDTYPE;
+  if (rc) return rc;
+  return check_launch(launches);
+}
+
+// y = bias, for an empty contraction
+template <typename TO> __global__ void __launch_bounds__(256) bias_rows(const TO* bias, TO* __restrict__ out, int64_t M, int64_t N) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < M * N; i += static_cast<int64_t>(gridDim.x) * 256) out[i] = bias ? bias[i % N] : from_f32<TO>(0.f);
+}
+
+constexpr int64_t kMostExtent = 0x7fffffff;
+
+}  // namespace
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int64_t b200_gated_linear_scratch_bytes(const void* x, const void* w, int64_t M, int64_t N, int64_t K, int64_t sxm, int64_t sxk, int64_t swn, int64_t swk) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  const int64_t need = LinOperand{x, M, K, sxm, sxk, 2}.packed_bytes() + LinOperand{w, 2 * N, K, swn, swk, 2}.packed_bytes();
+  return need ? need + 256 : 0;
+}
+
+extern "C" int b200_gated_linear(const void* x, const void* w, void* out, void* projections, int64_t M, int64_t N, int64_t K, int64_t sxm, int64_t sxk, int64_t swn, int64_t swk, int activation,
+                                 int dtype, void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream) {
+  if (M < 0 || N < 0 || K < 0 || activation < 0 || activation >= B200_ACT_COUNT) return B200_EINVAL;
+  if (dtype != B200_BF16 && dtype != B200_F16) return B200_EDTYPE;
+  if (M == 0 || N == 0) return B200_OK;
+  if (!out || M > kMostExtent || N > kMostExtent / 2 || K > kMostExtent) return B200_EINVAL;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (K == 0) {  // both projections are zero, and so is their product
+    cudaError_t e = cudaMemsetAsync(out, 0, static_cast<size_t>(M * N * 2), st);
+    if (e == cudaSuccess && projections) e = cudaMemsetAsync(projections, 0, static_cast<size_t>(M * N * 4), st);
+    if (e != cudaSuccess) { set_last_cuda_error(e); return B200_ELAUNCH; }
+    return B200_OK;
+  }
+  if (!x || !w) return B200_EINVAL;
+  LinParams p{};
+  p.act = activation;
+  p.side = projections;
+  return run_linear<kGated>(LinOperand{x, M, K, sxm, sxk, 2}, LinOperand{w, 2 * N, K, swn, swk, 2}, out, M, N, K, dtype, dtype == B200_BF16, p, scratch, scratch_bytes, status, st);
+}
+
+extern "C" int64_t b200_mm_int8_scratch_bytes(const void* A, const void* B, int64_t M, int64_t N, int64_t K, int64_t sAm, int64_t sAk, int64_t sBk, int64_t sBn) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  const int64_t need = LinOperand{A, M, K, sAm, sAk, 1}.packed_bytes() + LinOperand{B, N, K, sBn, sBk, 1}.packed_bytes();
+  return need ? need + 256 : 0;
+}
+
+extern "C" int b200_mm_int8(const void* A, const void* B, const float* a_scale, const float* b_scale, const void* bias, void* out, int64_t M, int64_t N, int64_t K, int64_t sAm, int64_t sAk,
+                            int64_t sBk, int64_t sBn, int dtype_out, void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream) {
+  if (M < 0 || N < 0 || K < 0 || K > B200_INT8_MAX_K) return B200_EINVAL;
+  if (!is_float_dtype(dtype_out)) return B200_EDTYPE;
+  if (M == 0 || N == 0) return B200_OK;
+  if (!out || M > kMostExtent || N > kMostExtent) return B200_EINVAL;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (K == 0) {
+    const int grid = static_cast<int>((M * N + 255) / 256 < kNumSMs * 8 ? (M * N + 255) / 256 : kNumSMs * 8);
+    if (dtype_out == B200_F32) bias_rows<<<grid, 256, 0, st>>>(static_cast<const float*>(bias), static_cast<float*>(out), M, N);
+    else if (dtype_out == B200_BF16) bias_rows<<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(bias), static_cast<__nv_bfloat16*>(out), M, N);
+    else bias_rows<<<grid, 256, 0, st>>>(static_cast<const __half*>(bias), static_cast<__half*>(out), M, N);
+    return check_launch();
+  }
+  if (!A || !B || !a_scale || !b_scale) return B200_EINVAL;
+  LinParams p{};
+  p.a_scale = a_scale;
+  p.b_scale = b_scale;
+  p.bias = bias;
+  return run_linear<kInt8>(LinOperand{A, M, K, sAm, sAk, 1}, LinOperand{B, N, K, sBn, sBk, 1}, out, M, N, K, dtype_out, false, p, scratch, scratch_bytes, status, st);
+}

@@ -10,9 +10,11 @@ the aten overload's argument list, the C-ABI-backed wrapper as its CUDA kernel, 
 instead of a function. The plugin implementations call these operators.
 
 There is still no CPU path: the CPU kernel registered here is the same wrapper, which raises
-`UnsupportedByB200` for host tensors. The operators carry no autograd formula; under the
-aten override the autograd key is aten's own (the override sits below it), and the backward
-operators of this package are registered as operators of their own.
+`UnsupportedByB200` for host tensors. The operators that mirror an aten
+overload carry no autograd formula; under the aten override the autograd key is aten's own (the
+override sits below it), and the backward operators of this package are registered as operators
+of their own. The linear layers of `feedforward.py` have no aten overload to stand under: they
+carry their own formulas (once differentiable).
 """
 
 from __future__ import annotations
@@ -21,6 +23,7 @@ import torch
 
 from . import _native
 from . import backward as _bw
+from . import feedforward as _ff
 from . import ops as _ops
 
 _aten = torch.ops.aten
@@ -89,6 +92,15 @@ for _name, (_schema, (_module, _attr), _aten_op) in OPERATORS.items():
     _library.impl(_name, _kernel_for(_module, _attr), "CUDA")
     _library.impl(_name, _kernel_for(_module, _attr), "CPU")  # raises UnsupportedByB200: there is no host path
     torch.library.register_fake(f"b200::{_name}", _fake_from(_aten_op), lib=_library)
+
+# the linear layers of a feed-forward block: operators without an aten overload, so their schemas, fake kernels and gradients are their own
+for _name, (_schema, _fake, _autograd) in _ff.OPERATORS.items():
+    _library.define(_name + _schema)
+    _library.impl(_name, _kernel_for(_ff, _name), "CUDA")
+    _library.impl(_name, _kernel_for(_ff, _name), "CPU")  # raises UnsupportedByB200
+    if _autograd is not None:
+        _library.impl(_name, _autograd, "Autograd")
+    torch.library.register_fake(f"b200::{_name}", _fake, lib=_library)
 
 
 def operator(name: str):

@@ -346,6 +346,54 @@ int b200_gemm_splitk(const void* A, const void* B, const void* bias, void* C, in
                      double alpha, double beta, int dtype, void* scratch, int64_t scratch_bytes,
                      uint32_t* status, void* stream);
 
+/* ------------------------------------------------- linear layers of a feed-forward block
+ * (no counterpart among the reference's operators; they stand beside mm / addmm) */
+
+/* Activations of a gated projection pair */
+enum { B200_ACT_SILU = 0, B200_ACT_GELU = 1, B200_ACT_GELU_TANH = 2, B200_ACT_RELU = 3, B200_ACT_SIGMOID = 4, B200_ACT_COUNT = 5 };
+
+/* out[m, n] = act(g[m, n]) * u[m, n], g = x Wg^T, u = x Wu^T, for bf16 / f16: x [M, K], w = [Wg; Wu] with
+ * 2 N rows of K (any strides; row-contiguous operands on the 16-byte grid are read as they are, others are copied
+ * into `scratch` first), out [M, N] contiguous. One tcgen05 kernel: fp32 sums, the gate on them, one
+ * rounding. `projections` (may be NULL): [M, 2 N] contiguous, takes [g | u], rounded once. A bounded
+ * wait that runs out is reported in `status` as by b200_gemm. */
+int64_t b200_gated_linear_scratch_bytes(const void* x, const void* w, int64_t M, int64_t N, int64_t K,
+                                        int64_t sxm, int64_t sxk, int64_t swn, int64_t swk);
+int b200_gated_linear(const void* x, const void* w, void* out, void* projections, int64_t M, int64_t N,
+                      int64_t K, int64_t sxm, int64_t sxk, int64_t swn, int64_t swk, int activation,
+                      int dtype, void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream);
+
+/* The gate by itself, and its gradient, for contiguous projections [M, 2 N] = [g | u]:
+ * out = act(g) * u;  grad_projections = [grad * u * act'(g) | grad * act(g)]. Every float dtype. */
+int b200_gate(const void* projections, void* out, int64_t M, int64_t N, int activation, int dtype, void* stream);
+int b200_gate_backward(const void* grad, const void* projections, void* grad_projections, int64_t M,
+                       int64_t N, int activation, int dtype, void* stream);
+
+/* out[i] = residual[i] + (word(i) >= round(p 2^32) ? x[i] / (1 - p) : 0) for n contiguous elements (residual
+ * may be NULL). word(i) is word i % 4 of Philox-4x32 with ten rounds for the counter (state[1] + i / 4, subsequence)
+ * under the key state[0]; `state` is two int64 in DEVICE memory, read when the kernel runs. Dropped
+ * elements are not read into the result (0, whatever they hold). p = 1 drops everything. */
+int b200_dropout(const void* x, const void* residual, void* out, int64_t n, double p, const int64_t* state,
+                 int64_t subsequence, int dtype, void* stream);
+
+/* Rows to 8 bits: scale[r] = max|x[r]| / 127 (fp32), q[r] = x[r] * (127 / max|x[r]|), rounded to even. Columns
+ * contiguous, rows `row_stride` elements apart; q [rows, cols] contiguous int8. A row whose largest magnitude is below
+ * 2^-118 counts as zeros (scale 0); a row with an infinity or a NaN has that as its scale and zeros. */
+int b200_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t row_stride,
+                       int dtype, void* stream);
+
+/* out[m, n] = (sum_k A[m, k] B[k, n]) * a_scale[m] * b_scale[n] + bias[n]: int8 operands of any strides (rows of K on the
+ * 16-byte grid are read as they are, others copied into `scratch`), exact 32-bit sums on the tensor cores
+ * (K <= B200_INT8_MAX_K, where no sum can overflow), scales fp32, out [M, N] contiguous in dtype_out
+ * (any float dtype), bias (may be NULL) of the same type. */
+#define B200_INT8_MAX_K 131071
+int64_t b200_mm_int8_scratch_bytes(const void* A, const void* B, int64_t M, int64_t N, int64_t K, int64_t sAm,
+                                   int64_t sAk, int64_t sBk, int64_t sBn);
+int b200_mm_int8(const void* A, const void* B, const float* a_scale, const float* b_scale, const void* bias,
+                 void* out, int64_t M, int64_t N, int64_t K, int64_t sAm, int64_t sAk, int64_t sBk,
+                 int64_t sBn, int dtype_out, void* scratch, int64_t scratch_bytes, uint32_t* status,
+                 void* stream);
+
 /* ------------------------------------------------------------- evaluation path */
 
 /* One pass replacing BackendBench/eval.py:68-90 (`allclose`: torch.testing.assert_close
