@@ -10,48 +10,46 @@ namespace {
 constexpr int kFfThreads = 256;
 
 // ------------------------------------------------------------------ the gate
-// h = act(g) * u of projections P = [g | u] (M x 2 N). fp32 products come in two steps (their sums are
+// h = act(g) * u of fp32 projections P = [g | u] (M x 2 N). fp32 products come in two steps (their sums are
 // put together from six plane products over several launches), so the gate has a kernel of its own there.
-// VEC elements to a thread: 16 bytes of each operand where rows are on the grid, else one.
-template <typename T, typename ACT, int VEC>
-__global__ void __launch_bounds__(kFfThreads) gate_forward(const T* p, T* __restrict__ h, int64_t M, int64_t N) {
-  const int64_t per_row = N / VEC, total = M * per_row;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kFfThreads) {
-    const int64_t m = total <= 0xffffffffll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(per_row) : i / per_row;
-    const T* row = p + i * VEC + m * N;  // m rows of 2 N, not N, lie before
-    float g[VEC], u[VEC];
-    if constexpr (VEC > 1) {
-      widen<T>(ld_stream(row), g);
-      widen<T>(ld_stream(row + N), u);
-    } else {
-      g[0] = to_f32(row[0]);
-      u[0] = to_f32(row[N]);
-    }
+// Backward: dP = [dh * u * act'(g) | dh * act(g)], rounded to the type of the operands it is multiplied by next.
+// VEC elements to a thread: whole vectors of every operand where rows are on the grid, else one.
+template <int N> __device__ __forceinline__ void load_f32(const float* p, float* v) {
+  if constexpr (N % 4 == 0) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) g[e] = ACT::template f<sizeof(T) == 2>(g[e]) * u[e];
-    if constexpr (VEC > 1) *reinterpret_cast<uint4*>(h + i * VEC) = narrow<T>(g);
-    else h[i] = from_f32<T>(g[0]);
+    for (int e = 0; e < N; e += 4) widen<float>(ld_stream(p + e), v + e);
+  } else {
+    v[0] = p[0];
   }
 }
 
-// dP = [dh * u * act'(g) | dh * act(g)]
+template <typename ACT, int VEC>
+__global__ void __launch_bounds__(kFfThreads) gate_forward(const float* p, float* __restrict__ h, int64_t M, int64_t N) {
+  const int64_t per_row = N / VEC, total = M * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kFfThreads) {
+    const int64_t m = total <= 0xffffffffll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(per_row) : i / per_row;
+    const float* row = p + i * VEC + m * N;  // m rows of 2 N, not N, lie before
+    float g[VEC], u[VEC];
+    load_f32<VEC>(row, g);
+    load_f32<VEC>(row + N, u);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) g[e] = ACT::template f<false>(g[e]) * u[e];
+    if constexpr (VEC > 1) *reinterpret_cast<uint4*>(h + i * VEC) = narrow<float>(g);
+    else h[i] = g[0];
+  }
+}
+
 template <typename T, typename ACT, int VEC>
-__global__ void __launch_bounds__(kFfThreads) gate_backward(const T* dh, const T* p, T* __restrict__ dp, int64_t M, int64_t N) {
+__global__ void __launch_bounds__(kFfThreads) gate_backward(const T* dh, const float* p, T* __restrict__ dp, int64_t M, int64_t N) {
   const int64_t per_row = N / VEC, total = M * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kFfThreads) {
     const int64_t m = total <= 0xffffffffll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(per_row) : i / per_row;
     const int64_t at = i * VEC + m * N;
     float d[VEC], g[VEC], u[VEC];
-    if constexpr (VEC > 1) {
-      const uint4 rd = ld_stream(dh + i * VEC), rg = ld_stream(p + at), ru = ld_stream(p + at + N);
-      widen<T>(rd, d);
-      widen<T>(rg, g);
-      widen<T>(ru, u);
-    } else {
-      d[0] = to_f32(dh[i]);
-      g[0] = to_f32(p[at]);
-      u[0] = to_f32(p[at + N]);
-    }
+    if constexpr (VEC > 1) widen<T>(ld_stream(dh + i * VEC), d);
+    else d[0] = to_f32(dh[i]);
+    load_f32<VEC>(p + at, g);
+    load_f32<VEC>(p + at + N, u);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       float a, s;
@@ -74,31 +72,25 @@ inline int ff_grid(int64_t items) {
   return static_cast<int>(b < most ? b : most);
 }
 
-template <typename T> int launch_gate(const void* dh, const void* p, void* out, int64_t M, int64_t N, int act, cudaStream_t st) {
-  constexpr int kVec = 16 / sizeof(T);
-  const bool vec = N % kVec == 0 && aligned16(p) && aligned16(out) && (!dh || aligned16(dh));
-  const int grid = ff_grid(M * N / (vec ? kVec : 1));
-  const T *tp = static_cast<const T*>(p), *td = static_cast<const T*>(dh);
-  T* to = static_cast<T*>(out);
+int launch_gate(const float* p, float* out, int64_t M, int64_t N, int act, cudaStream_t st) {
+  const bool vec = N % 4 == 0 && aligned16(p) && aligned16(out);
+  const int grid = ff_grid(M * N / (vec ? 4 : 1));
   gate_act_each(act, [&](auto a) {
-    using A = decltype(a);
-    if (dh) {
-      if (vec) gate_backward<T, A, kVec><<<grid, kFfThreads, 0, st>>>(td, tp, to, M, N);
-      else gate_backward<T, A, 1><<<grid, kFfThreads, 0, st>>>(td, tp, to, M, N);
-    } else {
-      if (vec) gate_forward<T, A, kVec><<<grid, kFfThreads, 0, st>>>(tp, to, M, N);
-      else gate_forward<T, A, 1><<<grid, kFfThreads, 0, st>>>(tp, to, M, N);
-    }
+    if (vec) gate_forward<decltype(a), 4><<<grid, kFfThreads, 0, st>>>(p, out, M, N);
+    else gate_forward<decltype(a), 1><<<grid, kFfThreads, 0, st>>>(p, out, M, N);
   });
   return check_launch();
 }
 
-int gate(const void* dh, const void* p, void* out, int64_t M, int64_t N, int act, int dtype, cudaStream_t st) {
-  switch (dtype) {
-    case B200_F32: return launch_gate<float>(dh, p, out, M, N, act, st);
-    case B200_BF16: return launch_gate<__nv_bfloat16>(dh, p, out, M, N, act, st);
-    default: return launch_gate<__half>(dh, p, out, M, N, act, st);
-  }
+template <typename T> int launch_gate_backward(const void* dh, const float* p, void* out, int64_t M, int64_t N, int act, cudaStream_t st) {
+  constexpr int kVec = 16 / sizeof(T);
+  const bool vec = N % kVec == 0 && aligned16(p) && aligned16(out) && aligned16(dh);
+  const int grid = ff_grid(M * N / (vec ? kVec : 1));
+  gate_act_each(act, [&](auto a) {
+    if (vec) gate_backward<T, decltype(a), kVec><<<grid, kFfThreads, 0, st>>>(static_cast<const T*>(dh), p, static_cast<T*>(out), M, N);
+    else gate_backward<T, decltype(a), 1><<<grid, kFfThreads, 0, st>>>(static_cast<const T*>(dh), p, static_cast<T*>(out), M, N);
+  });
+  return check_launch();
 }
 
 // ------------------------------------------------------------------ dropout
@@ -296,20 +288,24 @@ template <typename T> void launch_quantize(const void* x, void* q, void* scale, 
 
 using namespace b200;
 
-extern "C" int b200_gate(const void* projections, void* out, int64_t M, int64_t N, int activation, int dtype, void* stream) {
+extern "C" int b200_gate(const float* projections, float* out, int64_t M, int64_t N, int activation, void* stream) {
   if (M < 0 || N < 0 || activation < 0 || activation >= B200_ACT_COUNT) return B200_EINVAL;
-  if (!is_float_dtype(dtype)) return B200_EDTYPE;
   if (M == 0 || N == 0) return B200_OK;
   if (!projections || !out) return B200_EINVAL;
-  return gate(nullptr, projections, out, M, N, activation, dtype, static_cast<cudaStream_t>(stream));
+  return launch_gate(projections, out, M, N, activation, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int b200_gate_backward(const void* grad, const void* projections, void* grad_projections, int64_t M, int64_t N, int activation, int dtype, void* stream) {
+extern "C" int b200_gate_backward(const void* grad, const float* projections, void* grad_projections, int64_t M, int64_t N, int activation, int dtype, void* stream) {
   if (M < 0 || N < 0 || activation < 0 || activation >= B200_ACT_COUNT) return B200_EINVAL;
   if (!is_float_dtype(dtype)) return B200_EDTYPE;
   if (M == 0 || N == 0) return B200_OK;
   if (!grad || !projections || !grad_projections) return B200_EINVAL;
-  return gate(grad, projections, grad_projections, M, N, activation, dtype, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case B200_F32: return launch_gate_backward<float>(grad, projections, grad_projections, M, N, activation, st);
+    case B200_BF16: return launch_gate_backward<__nv_bfloat16>(grad, projections, grad_projections, M, N, activation, st);
+    default: return launch_gate_backward<__half>(grad, projections, grad_projections, M, N, activation, st);
+  }
 }
 
 extern "C" int b200_dropout(const void* x, const void* residual, void* out, int64_t n, double p, const int64_t* state, int64_t subsequence, int dtype, void* stream) {

@@ -19,7 +19,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import _abi, ops
+from . import ops
 from ._abi import check, lib
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}  # B200_ACT_*
@@ -81,14 +81,14 @@ def _gated(input: torch.Tensor, weight: torch.Tensor, activation: str, keep: boo
     lead = list(input.shape[:-1])
     out = ops._new(lead + [F], input.dtype, input.device)
     fp32 = input.dtype == torch.float32
-    projections = ops._new(lead + [2 * F], input.dtype, input.device) if keep and not fp32 else None
+    projections = ops._new(lead + [2 * F], torch.float32, input.device) if keep and not fp32 else None
     M = ops._prod(lead)
     if fp32:
         # the tensor cores take fp32 as six products of bf16 planes, over several launches: the projections are put
         # together first, the gate follows
         projections = ops.mm_default(_as_rows(input), weight.t())
         if out.numel():
-            check(lib().b200_gate(projections.data_ptr(), out.data_ptr(), M, F, act, _abi.F32, ops._stream_handle()), "b200_gate")
+            check(lib().b200_gate(projections.data_ptr(), out.data_ptr(), M, F, act, ops._stream_handle()), "b200_gate")
         return out, projections.view(lead + [2 * F])
     if out.numel():
         x = _as_rows(input)
@@ -114,9 +114,8 @@ def gated_linear(input: torch.Tensor, weight: torch.Tensor, activation: str = "s
 
 @_on_device_of
 def gated_linear_train(input: torch.Tensor, weight: torch.Tensor, activation: str = "silu") -> Tuple[torch.Tensor, torch.Tensor]:
-    """(gated_linear's result, the projections [..., 2 F] that its backward pass wants). The result is formed from the fp32
-    sums; the projections are rounded to the input's type, as a layer that kept them between two
-    operators would."""
+    """(gated_linear's result, the projections [..., 2 F] that its backward pass wants: the fp32 sums, whatever the input's
+    type)."""
     return _gated(input, weight, activation, True, "gated_linear_train")
 
 
@@ -131,8 +130,8 @@ def gated_linear_backward(grad_output: torch.Tensor, input: torch.Tensor, weight
     lead = list(input.shape[:-1])
     if list(grad_output.shape) != lead + [F] or list(projections.shape) != lead + [2 * F]:
         raise RuntimeError(f"gated_linear_backward: input {list(input.shape)} and weight {list(weight.shape)} do not go with grad_output {list(grad_output.shape)} and projections {list(projections.shape)}")
-    if grad_output.dtype != input.dtype or projections.dtype != input.dtype:
-        raise RuntimeError(f"gated_linear_backward: expected one dtype, got {grad_output.dtype}, {input.dtype} and {projections.dtype}")
+    if grad_output.dtype != input.dtype or projections.dtype != torch.float32:
+        raise RuntimeError(f"gated_linear_backward: expected grad_output like the input and fp32 projections, got {grad_output.dtype}, {input.dtype} and {projections.dtype}")
     want_dx, want_dw = (bool(m) for m in output_mask)
     if not (want_dx or want_dw):
         return None, None
@@ -140,7 +139,7 @@ def gated_linear_backward(grad_output: torch.Tensor, input: torch.Tensor, weight
     dp = ops._new((M, 2 * F), input.dtype, input.device)
     if dp.numel():
         g, p = ops._contig(grad_output), ops._contig(projections)
-        check(lib().b200_gate_backward(g.data_ptr(), p.data_ptr(), dp.data_ptr(), M, F, act, ops._dt(p.dtype), ops._stream_handle()), "b200_gate_backward")
+        check(lib().b200_gate_backward(g.data_ptr(), p.data_ptr(), dp.data_ptr(), M, F, act, ops._dt(g.dtype), ops._stream_handle()), "b200_gate_backward")
     dx = ops.mm_default(dp, weight).view(input.shape) if want_dx else None
     dw = ops.mm_default(dp.t(), _as_rows(input)) if want_dw else None
     return dx, dw
@@ -311,7 +310,7 @@ def _fake_gated(input, weight, activation="silu"):
 def _fake_gated_train(input, weight, activation="silu"):
     F, _ = _pair_args(input, weight, "gated_linear_train")
     lead = list(input.shape[:-1])
-    return input.new_empty(lead + [F]), input.new_empty(lead + [2 * F])
+    return input.new_empty(lead + [F]), input.new_empty(lead + [2 * F], dtype=torch.float32)
 
 
 def _fake_gated_backward(grad_output, input, weight, projections, activation="silu", output_mask=(True, True)):

@@ -355,18 +355,19 @@ enum { B200_ACT_SILU = 0, B200_ACT_GELU = 1, B200_ACT_GELU_TANH = 2, B200_ACT_RE
 /* out[m, n] = act(g[m, n]) * u[m, n], g = x Wg^T, u = x Wu^T, for bf16 / f16: x [M, K], w = [Wg; Wu] with
  * 2 N rows of K (any strides; row-contiguous operands on the 16-byte grid are read as they are, others are copied
  * into `scratch` first), out [M, N] contiguous. One tcgen05 kernel: fp32 sums, the gate on them, one
- * rounding. `projections` (may be NULL): [M, 2 N] contiguous, takes [g | u], rounded once. A bounded
+ * rounding. `projections` (may be NULL): fp32 [M, 2 N] contiguous, takes the sums [g | u]. A bounded
  * wait that runs out is reported in `status` as by b200_gemm. */
 int64_t b200_gated_linear_scratch_bytes(const void* x, const void* w, int64_t M, int64_t N, int64_t K,
                                         int64_t sxm, int64_t sxk, int64_t swn, int64_t swk);
-int b200_gated_linear(const void* x, const void* w, void* out, void* projections, int64_t M, int64_t N,
+int b200_gated_linear(const void* x, const void* w, void* out, float* projections, int64_t M, int64_t N,
                       int64_t K, int64_t sxm, int64_t sxk, int64_t swn, int64_t swk, int activation,
                       int dtype, void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream);
 
-/* The gate by itself, and its gradient, for contiguous projections [M, 2 N] = [g | u]:
- * out = act(g) * u;  grad_projections = [grad * u * act'(g) | grad * act(g)]. Every float dtype. */
-int b200_gate(const void* projections, void* out, int64_t M, int64_t N, int activation, int dtype, void* stream);
-int b200_gate_backward(const void* grad, const void* projections, void* grad_projections, int64_t M,
+/* The gate by itself (fp32, whose products come in several launches), and its gradient, for contiguous fp32
+ * projections [M, 2 N] = [g | u]: out = act(g) * u;  grad_projections = [grad * u * act'(g) | grad * act(g)], grad and
+ * grad_projections of any float dtype. */
+int b200_gate(const float* projections, float* out, int64_t M, int64_t N, int activation, void* stream);
+int b200_gate_backward(const void* grad, const float* projections, void* grad_projections, int64_t M,
                        int64_t N, int activation, int dtype, void* stream);
 
 /* out[i] = residual[i] + (word(i) >= round(p 2^32) ? x[i] / (1 - p) : 0) for n contiguous elements (residual

@@ -67,7 +67,7 @@ def gated(x, w, name, dtype):
     h = a * u
     fn = act_error(g, name, dtype)  # and |act'| <= 1.13
     tol = U[dtype] * h.abs() + (1.13 * err[:, :F] + fn * a.abs()) * (u.abs() + err[:, F:]) + a.abs() * err[:, F:]
-    return h, 1.001 * tol + TINY[dtype], p, 1.001 * (U[dtype] * p.abs() + err) + TINY[dtype]
+    return h, 1.001 * tol + TINY[dtype], p, 1.001 * err + 1e-37  # (the projections are fp32 sums)
 
 
 def gated_grads(dh, x, w, p, name, dtype):

@@ -40,7 +40,7 @@ def test_fake_kernels_and_gradients_by_shape():
         assert h.shape == (3, 5, 32) and h.dtype == torch.bfloat16 and h.requires_grad
         assert not K.gated_linear(x.detach(), w.detach()).requires_grad
         out, projections = K.gated_linear_train(x, w)
-        assert out.requires_grad and projections.shape == (3, 5, 64) and not projections.requires_grad
+        assert out.requires_grad and projections.shape == (3, 5, 64) and projections.dtype == torch.float32 and not projections.requires_grad
         dx, dw = K.gated_linear_backward(h.detach(), x.detach(), w.detach(), projections, "gelu", [True, False])
         assert dx.shape == x.shape and dw is None
         state = torch.empty(2, dtype=torch.int64, device="cuda")
@@ -89,7 +89,8 @@ def test_refusals(anywhere):
     h, p = torch.randn(4, 3), torch.randn(4, 6)
     _bad(lambda: f.gated_linear_backward(h[:, :2], x, w, p), RuntimeError, "do not go with")
     _bad(lambda: f.gated_linear_backward(h, x, w, p[:, :4]), RuntimeError, "do not go with")
-    _bad(lambda: f.gated_linear_backward(h.half(), x, w, p), RuntimeError, "one dtype")
+    _bad(lambda: f.gated_linear_backward(h.half(), x, w, p), RuntimeError, "like the input and fp32")
+    _bad(lambda: f.gated_linear_backward(h.half(), x.half(), w.half(), p.half()), RuntimeError, "fp32 projections")
     assert f.gated_linear_backward(h, x, w, p, "silu", [False, False]) == (None, None)
     s = torch.zeros(2, dtype=torch.int64)
     for p_drop in (-0.1, 1.1, float("nan")):
@@ -129,5 +130,5 @@ def test_the_library_refuses_what_the_wrappers_would(monkeypatch):
     assert m(4, 4, 131072, 4, 1, 4, 1, BF) == -1 and m(4, 4, 4, 4, 1, 4, 1, _abi.I32) == -2 and m(4, 0, 4, 4, 1, 4, 1, BF) == 0 and m(4, 4, 4, 4, 1, 4, 1, BF) == -1
     assert lib.b200_dropout(None, None, None, 4, 1.5, None, 0, BF, None) == -1 and lib.b200_dropout(None, None, None, 0, 0.5, None, 0, BF, None) == 0
     assert lib.b200_dropout(None, None, None, 4, 0.5, None, 0, _abi.I8, None) == -2 and lib.b200_dropout(None, None, None, 4, 0.5, None, 0, BF, None) == -1
-    assert lib.b200_gate(None, None, 4, 4, 9, BF, None) == -1 and lib.b200_gate_backward(None, None, None, 4, 4, 0, _abi.I32, None) == -2
+    assert lib.b200_gate(None, None, 4, 4, 9, None) == -1 and lib.b200_gate_backward(None, None, None, 4, 4, 0, _abi.I32, None) == -2
     assert lib.b200_quantize_rows(None, None, None, 4, 4, 4, BF, None) == -1 and lib.b200_quantize_rows(None, None, None, 0, 4, 4, BF, None) == 0
