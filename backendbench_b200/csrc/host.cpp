@@ -21,9 +21,11 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/library.h>
 
 #include "../../include/b200ops.h"
 
@@ -34,7 +36,8 @@ namespace {
   F(b200_relu) F(b200_add) F(b200_mul) F(b200_add_scalar) F(b200_mul_scalar) F(b200_where) F(b200_softmax) F(b200_softmax_backward) F(b200_reduce_scratch_bytes) F(b200_sum)           \
   F(b200_layer_norm) F(b200_layer_norm_backward_scratch_bytes) F(b200_layer_norm_backward) F(b200_argmax) F(b200_gather_rows) F(b200_index_select) F(b200_gather)                    \
   F(b200_scatter_add_scratch_bytes) F(b200_scatter_add) F(b200_embedding_backward_scratch_bytes) F(b200_embedding_backward) F(b200_copy_pitched) F(b200_gemm)                        \
-  F(b200_gemm_takes_as_is) F(b200_gemm_f32_scratch_bytes) F(b200_gemm_f32) F(b200_gemm_splitk_scratch_bytes) F(b200_gemm_splitk) F(b200_allclose)
+  F(b200_gemm_takes_as_is) F(b200_gemm_f32_scratch_bytes) F(b200_gemm_f32) F(b200_gemm_splitk_scratch_bytes) F(b200_gemm_splitk) F(b200_allclose)                   \
+  F(b200_gated_linear_scratch_bytes) F(b200_gated_linear) F(b200_gate) F(b200_gate_backward) F(b200_dropout) F(b200_quantize_rows) F(b200_mm_int8_scratch_bytes) F(b200_mm_int8)
 struct Api {
 #define F(name) decltype(&::name) name;
   B200_ENTRIES(F)
@@ -907,8 +910,11 @@ PyObject* compare(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+#include "host_feedforward.h"
+
 PyMethodDef kMethods[] = {{"setup", setup, METH_VARARGS, nullptr},
                           {"make", make, METH_VARARGS, nullptr},
+                          {"feedforward", feedforward, METH_O, nullptr},
                           {"release", release, METH_NOARGS, nullptr},
                           {"compare", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(compare)), METH_FASTCALL, nullptr},
                           {nullptr, nullptr, 0, nullptr}};

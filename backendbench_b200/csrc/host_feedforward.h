@@ -1,0 +1,314 @@
+// The operators of feedforward.py as kernels of the dispatcher (included by host.cpp, whose helpers they use).
+//
+// They have no aten overload, so a user calls them as torch.ops.b200.<name>; what bounds a small call there is the way
+// from the dispatcher into Python and back, twice where a gradient may have to be recorded (dropout of 16 x 256, forward and backward:
+// 30 us through Python kernels, 12 so). As in the callables above, nothing new is decided here: a call of plain
+// tensors that need no conversion goes to the entry point that the wrapper of feedforward.py would call with the same
+// arguments; any other, and any that fails, goes to the wrapper, and one with a gradient to record to its autograd function.
+
+using TensorOpt = std::optional<Tensor>;
+
+struct Gil {  // the dispatcher lets go of the interpreter lock before it enters a native kernel
+  PyGILState_STATE state = PyGILState_Ensure();
+  ~Gil() { PyGILState_Release(state); }
+};
+PyObject* ff_dict = nullptr;  // feedforward.py's names
+
+struct FfOp {
+  const char* name;
+  const char* autograd_name;
+  PyObject *attr = nullptr, *original = nullptr, *autograd = nullptr;
+  bool direct() const {  // nobody has replaced the wrapper or its allocator
+    return PyDict_GetItemWithError(ops_dict, allocator_key) == Py_None && PyDict_GetItemWithError(ff_dict, attr) == original;
+  }
+};
+enum { kFfGated, kFfGatedTrain, kFfGatedBackward, kFfDropout, kFfDropoutBackward, kFfQuantize, kFfInt8, kFfOps };
+FfOp ff_ops[kFfOps] = {{"gated_linear", "gated_linear_autograd"}, {"gated_linear_train", "gated_linear_train_autograd"}, {"gated_linear_backward", nullptr}, {"dropout", "dropout_autograd"},
+                       {"dropout_backward", nullptr}, {"quantize_rows", nullptr}, {"mm_int8", nullptr}};
+
+[[noreturn]] void raise_python() {
+  python_error e;
+  e.persist();
+  throw e;
+}
+PyObject* py(const Tensor& t) { return t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None); }
+PyObject* py(const TensorOpt& t) { return t ? py(*t) : Py_NewRef(Py_None); }
+PyObject* py(double v) { return PyFloat_FromDouble(v); }
+PyObject* py(int64_t v) { return PyLong_FromLongLong(v); }
+PyObject* py(c10::string_view v) { return PyUnicode_FromStringAndSize(v.data(), static_cast<Py_ssize_t>(v.size())); }
+PyObject* py(std::array<bool, 2> v) { return Py_BuildValue("[OO]", v[0] ? Py_True : Py_False, v[1] ? Py_True : Py_False); }
+PyObject* py(std::optional<at::ScalarType> v) { return v ? Py_NewRef(reinterpret_cast<PyObject*>(torch::getTHPDtype(*v))) : Py_NewRef(Py_None); }
+template <typename T> struct Named {
+  const char* name;
+  T value;
+};
+template <typename T> void put(PyObject* args, PyObject*, Py_ssize_t& i, const T& v) { PyTuple_SET_ITEM(args, i++, py(v)); }
+template <typename T> void put(PyObject*, PyObject* kwargs, Py_ssize_t&, const Named<T>& v) {
+  PyObject* o = py(v.value);
+  if (o) PyDict_SetItemString(kwargs, v.name, o);
+  Py_XDECREF(o);
+}
+template <typename T> constexpr int positional(const T&) { return 1; }
+template <typename T> constexpr int positional(const Named<T>&) { return 0; }
+// (with the lock held) `fn` of these arguments, as the interpreter would call it
+template <typename... A> PyObject* in_python(PyObject* fn, const A&... a) {
+  PyObject *args = PyTuple_New((positional(a) + ... + 0)), *kwargs = PyDict_New();
+  Py_ssize_t i = 0;
+  (put(args, kwargs, i, a), ...);
+  PyObject* r = PyErr_Occurred() ? nullptr : PyObject_Call(fn, args, kwargs);
+  Py_DECREF(args);
+  Py_DECREF(kwargs);
+  if (!r) raise_python();
+  return r;
+}
+Tensor taken(PyObject* r) {  // the tensor of a result, which is given up
+  Tensor t = THPVariable_Unpack(r);
+  Py_DECREF(r);
+  return t;
+}
+TensorOpt taken_or_none(PyObject* o) { return o == Py_None ? TensorOpt() : TensorOpt(THPVariable_Unpack(o)); }
+std::tuple<Tensor, Tensor> taken_pair(PyObject* r) {
+  std::tuple<Tensor, Tensor> t{THPVariable_Unpack(PyTuple_GET_ITEM(r, 0)), THPVariable_Unpack(PyTuple_GET_ITEM(r, 1))};
+  Py_DECREF(r);
+  return t;
+}
+template <typename... A> PyObject* wrapper(int op, const A&... a) {
+  PyObject* fn = PyDict_GetItemWithError(ff_dict, ff_ops[op].attr);
+  if (!fn) {
+    PyErr_Format(PyExc_RuntimeError, "feedforward.%s is gone", ff_ops[op].name);
+    raise_python();
+  }
+  return in_python(fn, a...);
+}
+void ff_launched(bool ok) {
+  if (!ok) raise_python();
+}
+
+int activation_code(c10::string_view name) {
+  constexpr const char* kNames[B200_ACT_COUNT] = {"silu", "gelu", "gelu_tanh", "relu", "sigmoid"};
+  for (int i = 0; i < B200_ACT_COUNT; ++i)
+    if (name == kNames[i]) return i;
+  return -1;
+}
+// [..., K] as rows: a matrix as it is, anything else where it is contiguous
+struct Rows {
+  int64_t M = 0, K = 0, s_m = 0, s_k = 0;
+  bool of(const Tensor& t) {
+    if (t.dim() < 1) return false;
+    K = t.size(t.dim() - 1);
+    M = product(t.sizes(), 0, t.dim() - 1);
+    if (t.dim() == 2) {
+      s_m = t.stride(0);
+      s_k = t.stride(1);
+      return true;
+    }
+    s_m = K;
+    s_k = 1;
+    return t.is_contiguous();
+  }
+};
+at::DimVector with_last(const Tensor& t, int64_t last) {
+  at::DimVector s(t.sizes().begin(), t.sizes().end());
+  s.back() = last;
+  return s;
+}
+
+// (output, projections); an undefined output: the wrapper has to take the call
+std::tuple<Tensor, Tensor> gated_direct(const Tensor& x, const Tensor& w, c10::string_view activation, bool keep) {
+  Rows r;
+  const int act = activation_code(activation);
+  if (act < 0 || !floating(x) || x.scalar_type() != w.scalar_type() || w.dim() != 2 || w.size(0) % 2 || !r.of(x) || w.size(1) != r.K || !plain(x, w)) return {};
+  const int64_t F = w.size(0) / 2;
+  if (r.M == 0 || F == 0 || r.K == 0) return {};
+  Tensor projections;
+  if (dt(x) == B200_F32) {
+    PyObject* p = gemm(Operand{x, 0, r.s_m, r.s_k}, Operand{w, 0, w.stride(1), w.stride(0)}, Tensor(), 1, r.M, 2 * F, r.K, 1.0, 0.0, with_last(x, 2 * F));
+    if (!p) raise_python();
+    projections = taken(p);
+    Tensor out = new_tensor(with_last(x, F), x.scalar_type(), x);
+    ff_launched(launched("b200_gate", [&, st = stream()] { return api.b200_gate(static_cast<const float*>(ptr(projections)), static_cast<float*>(ptr(out)), r.M, F, act, st); }));
+    return {out, projections};
+  }
+  uint32_t* status = status_word(x);
+  if (!status) raise_python();
+  Tensor out = new_tensor(with_last(x, F), x.scalar_type(), x);
+  if (keep) projections = new_tensor(with_last(x, 2 * F), at::kFloat, x);
+  const int64_t ws0 = w.stride(0), ws1 = w.stride(1), need = api.b200_gated_linear_scratch_bytes(ptr(x), ptr(w), r.M, F, r.K, r.s_m, r.s_k, ws0, ws1);
+  Scratch s(x, need);
+  ff_launched(launched("b200_gated_linear", [&, st = stream()] {
+    return api.b200_gated_linear(ptr(x), ptr(w), ptr(out), static_cast<float*>(ptr(projections)), r.M, F, r.K, r.s_m, r.s_k, ws0, ws1, act, dt(x), s.data(), need, status, st);
+  }));
+  return {out, projections};
+}
+
+Tensor ff_gated_linear(const Tensor& x, const Tensor& w, c10::string_view activation) {
+  Gil gil;
+  if (ff_ops[kFfGated].direct()) {
+    Tensor out = std::get<0>(gated_direct(x, w, activation, false));
+    if (out.defined()) return out;
+  }
+  return taken(wrapper(kFfGated, x, w, activation));
+}
+std::tuple<Tensor, Tensor> ff_gated_linear_train(const Tensor& x, const Tensor& w, c10::string_view activation) {
+  Gil gil;
+  if (ff_ops[kFfGatedTrain].direct()) {
+    auto out = gated_direct(x, w, activation, true);
+    if (std::get<0>(out).defined()) return out;
+  }
+  return taken_pair(wrapper(kFfGatedTrain, x, w, activation));
+}
+std::tuple<TensorOpt, TensorOpt> ff_gated_linear_backward(const Tensor& g, const Tensor& x, const Tensor& w, const Tensor& p, c10::string_view activation, std::array<bool, 2> mask) {
+  Gil gil;
+  Rows r;
+  const int act = activation_code(activation);
+  if (ff_ops[kFfGatedBackward].direct() && act >= 0 && floating(x) && w.dim() == 2 && w.size(0) % 2 == 0 && r.of(x) && w.size(1) == r.K && (mask[0] || mask[1]) && plain(g, x, w, p)) {
+    const int64_t F = w.size(0) / 2;
+    if (r.M && F && r.K && w.scalar_type() == x.scalar_type() && g.scalar_type() == x.scalar_type() && p.scalar_type() == at::kFloat && g.is_contiguous() && p.is_contiguous() &&
+        g.sizes() == at::IntArrayRef(with_last(x, F)) && p.sizes() == at::IntArrayRef(with_last(x, 2 * F))) {
+      Tensor dp = new_tensor({r.M, 2 * F}, x.scalar_type(), x);
+      ff_launched(launched("b200_gate_backward", [&, st = stream()] { return api.b200_gate_backward(ptr(g), static_cast<const float*>(ptr(p)), ptr(dp), r.M, F, act, dt(x), st); }));
+      std::tuple<TensorOpt, TensorOpt> out;
+      if (mask[0]) {
+        PyObject* dx = gemm(Operand{dp, 0, 2 * F, 1}, Operand{w, 0, w.stride(0), w.stride(1)}, Tensor(), 1, r.M, r.K, 2 * F, 1.0, 0.0, x.sizes());
+        if (!dx) raise_python();
+        std::get<0>(out) = taken(dx);
+      }
+      if (mask[1]) {
+        PyObject* dw = gemm(Operand{dp, 0, 1, 2 * F}, Operand{x, 0, r.s_m, r.s_k}, Tensor(), 1, 2 * F, r.K, r.M, 1.0, 0.0, w.sizes());
+        if (!dw) raise_python();
+        std::get<1>(out) = taken(dw);
+      }
+      return out;
+    }
+  }
+  PyObject* o = wrapper(kFfGatedBackward, g, x, w, p, activation, mask);
+  std::tuple<TensorOpt, TensorOpt> out{taken_or_none(PyTuple_GET_ITEM(o, 0)), taken_or_none(PyTuple_GET_ITEM(o, 1))};
+  Py_DECREF(o);
+  return out;
+}
+
+Tensor dropout_direct(const Tensor& x, double p, const Tensor& state, const Tensor& residual, int64_t subsequence) {
+  if (!floating(x) || !(p >= 0. && p <= 1.) || !x.is_contiguous() || x.numel() == 0 || state.scalar_type() != at::kLong || state.dim() != 1 || state.size(0) != 2 || !state.is_contiguous() ||
+      (residual.defined() && (residual.scalar_type() != x.scalar_type() || residual.sizes() != x.sizes() || !residual.is_contiguous())) || !plain(x, state, residual))
+    return {};
+  Tensor out = new_like(x);
+  ff_launched(launched("b200_dropout", [&, st = stream()] { return api.b200_dropout(ptr(x), ptr(residual), ptr(out), x.numel(), p, static_cast<const int64_t*>(ptr(state)), subsequence, dt(x), st); }));
+  return out;
+}
+Tensor ff_dropout(const Tensor& x, double p, const Tensor& state, const TensorOpt& residual, int64_t subsequence) {
+  Gil gil;
+  if (ff_ops[kFfDropout].direct()) {
+    Tensor out = dropout_direct(x, p, state, residual ? *residual : Tensor(), subsequence);
+    if (out.defined()) return out;
+  }
+  return taken(wrapper(kFfDropout, x, p, state, residual, Named<int64_t>{"subsequence", subsequence}));
+}
+Tensor ff_dropout_backward(const Tensor& g, double p, const Tensor& state, int64_t subsequence) {
+  Gil gil;
+  if (ff_ops[kFfDropoutBackward].direct()) {
+    Tensor out = dropout_direct(g, p, state, Tensor(), subsequence);
+    if (out.defined()) return out;
+  }
+  return taken(wrapper(kFfDropoutBackward, g, p, state, Named<int64_t>{"subsequence", subsequence}));
+}
+
+std::tuple<Tensor, Tensor> ff_quantize_rows(const Tensor& x) {
+  Gil gil;
+  Rows r;
+  if (ff_ops[kFfQuantize].direct() && floating(x) && r.of(x) && r.s_k == 1 && x.numel() && plain(x)) {
+    Tensor q = new_tensor(x.sizes(), at::kChar, x), scale = new_tensor(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
+    ff_launched(launched("b200_quantize_rows", [&, st = stream()] { return api.b200_quantize_rows(ptr(x), ptr(q), static_cast<float*>(ptr(scale)), r.M, r.K, r.s_m, dt(x), st); }));
+    return {q, scale};
+  }
+  return taken_pair(wrapper(kFfQuantize, x));
+}
+
+bool scale_of(const Tensor& t, int64_t n, bool column) {
+  return t.scalar_type() == at::kFloat && t.is_contiguous() && ((t.dim() == 1 && t.size(0) == n) || (t.dim() == 2 && t.size(column ? 0 : 1) == n && t.size(column ? 1 : 0) == 1));
+}
+Tensor ff_mm_int8(const Tensor& a, const Tensor& b, const Tensor& sa, const Tensor& sb, const TensorOpt& bias, std::optional<at::ScalarType> out_dtype) {
+  Gil gil;
+  const Tensor none, &c = bias ? *bias : none;
+  const at::ScalarType type = out_dtype ? *out_dtype : c.defined() ? c.scalar_type() : at::kBFloat16;
+  if (ff_ops[kFfInt8].direct() && a.dim() == 2 && b.dim() == 2 && a.size(1) == b.size(0) && a.numel() && b.numel() && a.size(1) <= B200_INT8_MAX_K && a.scalar_type() == at::kChar &&
+      b.scalar_type() == at::kChar && scale_of(sa, a.size(0), true) && scale_of(sb, b.size(1), false) && (type == at::kFloat || type == at::kHalf || type == at::kBFloat16) &&
+      (!c.defined() || (c.scalar_type() == type && c.dim() == 1 && c.size(0) == b.size(1) && c.is_contiguous())) && plain(a, b, sa, sb, c)) {
+    const int64_t M = a.size(0), K = a.size(1), N = b.size(1), s[4] = {a.stride(0), a.stride(1), b.stride(0), b.stride(1)};
+    uint32_t* status = status_word(a);
+    if (!status) raise_python();
+    Tensor out = new_tensor({M, N}, type, a);
+    const int64_t need = api.b200_mm_int8_scratch_bytes(ptr(a), ptr(b), M, N, K, s[0], s[1], s[2], s[3]);
+    Scratch scratch(a, need);
+    ff_launched(launched("b200_mm_int8", [&, st = stream()] {
+      return api.b200_mm_int8(ptr(a), ptr(b), static_cast<const float*>(ptr(sa)), static_cast<const float*>(ptr(sb)), ptr(c), ptr(out), M, N, K, s[0], s[1], s[2], s[3], dt(out), scratch.data(), need,
+                              status, st);
+    }));
+    return out;
+  }
+  return taken(wrapper(kFfInt8, a, b, sa, sb, bias, Named<std::optional<at::ScalarType>>{"out_dtype", out_dtype}));
+}
+
+// Where a gradient may have to be recorded: the autograd function of feedforward.py if so, the kernel below if not
+// (which refuses a forward-mode one)
+bool wants_gradient(const Tensor& a, const Tensor& b) {
+  auto of = [](const Tensor& t) { return t.defined() && ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined()); };
+  return of(a) || of(b);
+}
+template <typename F> auto below(const char* name) { return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>(); }
+
+Tensor ff_gated_linear_autograd(const Tensor& x, const Tensor& w, c10::string_view activation) {
+  if (wants_gradient(x, w)) {
+    Gil gil;
+    return taken(in_python(ff_ops[kFfGated].autograd, x, w, activation));
+  }
+  static const auto op = below<Tensor(const Tensor&, const Tensor&, c10::string_view)>("b200::gated_linear");
+  at::AutoDispatchBelowAutograd guard;
+  return op.call(x, w, activation);
+}
+std::tuple<Tensor, Tensor> ff_gated_linear_train_autograd(const Tensor& x, const Tensor& w, c10::string_view activation) {
+  if (wants_gradient(x, w)) {
+    Gil gil;
+    return taken_pair(in_python(ff_ops[kFfGatedTrain].autograd, x, w, activation));
+  }
+  static const auto op = below<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, c10::string_view)>("b200::gated_linear_train");
+  at::AutoDispatchBelowAutograd guard;
+  return op.call(x, w, activation);
+}
+Tensor ff_dropout_autograd(const Tensor& x, double p, const Tensor& state, const TensorOpt& residual, int64_t subsequence) {
+  if (wants_gradient(x, residual ? *residual : Tensor())) {
+    Gil gil;
+    return taken(in_python(ff_ops[kFfDropout].autograd, x, p, state, residual, Named<int64_t>{"subsequence", subsequence}));
+  }
+  static const auto op = below<Tensor(const Tensor&, double, const Tensor&, const TensorOpt&, int64_t)>("b200::dropout");
+  at::AutoDispatchBelowAutograd guard;
+  return op.call(x, p, state, residual, subsequence);
+}
+
+// feedforward(module): the kernels above take the CUDA and Autograd keys of the operators that custom_ops.py has defined
+PyObject* feedforward(PyObject*, PyObject* module) {
+  HANDLE_TH_ERRORS
+  if (!ops_dict || ff_dict) return PyErr_Format(PyExc_RuntimeError, "setup() comes first, and this once");
+  PyObject* dict = PyModule_GetDict(module);
+  for (FfOp& op : ff_ops) {
+    op.attr = PyUnicode_InternFromString(op.name);
+    op.original = op.attr ? Py_XNewRef(PyDict_GetItemWithError(dict, op.attr)) : nullptr;
+    op.autograd = op.autograd_name ? PyObject_GetAttrString(module, op.autograd_name) : nullptr;
+    if (!op.original || (op.autograd_name && !op.autograd)) return PyErr_Format(PyExc_RuntimeError, "feedforward.%s is missing", op.name);
+  }
+  ff_dict = Py_NewRef(dict);
+  static auto* library = new torch::Library(torch::Library::FRAGMENT, "b200", std::nullopt, __FILE__, __LINE__);
+  auto cuda = [&](const char* name, auto* f) { library->impl(name, torch::dispatch(c10::DispatchKey::CUDA, f)); };
+  auto grad = [&](const char* name, auto* f) { library->impl(name, torch::dispatch(c10::DispatchKey::Autograd, f)); };
+  cuda("gated_linear", ff_gated_linear);
+  cuda("gated_linear_train", ff_gated_linear_train);
+  cuda("gated_linear_backward", ff_gated_linear_backward);
+  cuda("dropout", ff_dropout);
+  cuda("dropout_backward", ff_dropout_backward);
+  cuda("quantize_rows", ff_quantize_rows);
+  cuda("mm_int8", ff_mm_int8);
+  grad("gated_linear", ff_gated_linear_autograd);
+  grad("gated_linear_train", ff_gated_linear_train_autograd);
+  grad("dropout", ff_dropout_autograd);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}

@@ -96,11 +96,15 @@ for _name, (_schema, (_module, _attr), _aten_op) in OPERATORS.items():
 # the linear layers of a feed-forward block: operators without an aten overload, so their schemas, fake kernels and gradients are their own
 for _name, (_schema, _fake, _autograd) in _ff.OPERATORS.items():
     _library.define(_name + _schema)
-    _library.impl(_name, _kernel_for(_ff, _name), "CUDA")
     _library.impl(_name, _kernel_for(_ff, _name), "CPU")  # raises UnsupportedByB200
-    if _autograd is not None:
-        _library.impl(_name, _autograd, "Autograd")
     torch.library.register_fake(f"b200::{_name}", _fake, lib=_library)
+if _native.module() is not None:
+    _native.module().feedforward(_ff)  # native kernels, which come back to the wrappers and autograd functions for what is not a plain call
+else:
+    for _name, (_schema, _fake, _autograd) in _ff.OPERATORS.items():
+        _library.impl(_name, _kernel_for(_ff, _name), "CUDA")
+        if _autograd is not None:
+            _library.impl(_name, _autograd, "Autograd")
 
 
 def operator(name: str):

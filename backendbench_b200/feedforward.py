@@ -277,6 +277,8 @@ class _Dropout(torch.autograd.Function):
 
 
 def _wants_gradient(*tensors) -> bool:
+    if torch.autograd.forward_ad._current_level >= 0:  # the autograd functions refuse a forward-mode gradient
+        return any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors)
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 

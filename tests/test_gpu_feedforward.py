@@ -468,6 +468,60 @@ def _all_args(M=70, k=136, F=72, odd=0):
 
 
 @pytest.mark.parametrize("odd", [0, 3])
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "f16", "f32"])
+def test_native_calls_give_what_the_wrappers_give(dtype, odd, bands):
+    """With the bands' allocator in place every call goes through the wrappers; without it plain ones come from native code."""
+    M, k, F = 70, 136 + odd, 72
+    x, w = _pair(M, k, F, dtype)
+    q, w8, sa, sb, bias = _int8(M, k), _int8(96, k), torch.rand(M, device=DEV), torch.rand(96, device=DEV), _randn(96, dtype=dtype)
+    dh, s, r = _randn(M, F, dtype=dtype), _state(3, 4), _randn(M, k, dtype=dtype, seed=6)
+    wide = _randn(M, k + 8, dtype=dtype)
+
+    def calls():
+        for v in (x, wide[:, :k], x.t().contiguous().t(), x.view(2, 35, k)):
+            h, projections = K.gated_linear_train(v, w, "gelu")
+            g = dh.view(h.shape)
+            yield from (K.gated_linear(v, w), h, projections)
+            yield from K.gated_linear_backward(g, v, w, projections, "gelu")
+            yield K.gated_linear_backward(g, v, w, projections, "gelu", [True, False])[0]
+            yield from (K.dropout(v, 0.3, s, r.view(v.shape), subsequence=9), K.dropout(v, 0.3, s), K.dropout_backward(v, 0.3, s, subsequence=9))
+            yield from K.quantize_rows(v)
+        yield from (K.mm_int8(q, w8.t(), sa, sb), K.mm_int8(q, w8.t(), sa[:, None], sb[None], bias), K.mm_int8(q, w8.t(), sa, sb, out_dtype=dtype), K.mm_int8(q, w8.t().contiguous(), sa, sb))
+
+    want = list(calls())
+    assert bands.allocations > 50
+    ops._allocator = None
+    count = bands.allocations
+    got = list(calls())
+    assert bands.allocations == count
+    assert len(got) == len(want) and all(a.dtype == b.dtype and a.shape == b.shape and bits_equal(a, b) for a, b in zip(got, want))
+
+
+def test_refusals_come_back_as_the_wrappers_raise_them(bands):
+    ops._allocator = None
+    x, w = _pair(4, 64, 8, BF)
+    s, q, one = _state(1, 2), _int8(4, 64), torch.ones(4, device=DEV)
+    for call, error, match in (
+        (lambda: K.gated_linear(x, w, "tanh"), ValueError, "not one of"),
+        (lambda: K.gated_linear(x, w[:5]), RuntimeError, "5 rows"),
+        (lambda: K.gated_linear(x, w.half()), RuntimeError, "same dtype"),
+        (lambda: K.gated_linear(x, w.cpu()), ops.UnsupportedByB200, "no CPU path"),
+        (lambda: K.gated_linear_backward(x, x, w, x), RuntimeError, "do not go with"),
+        (lambda: K.dropout(x, 2.0, s), ValueError, "between 0 and 1"),
+        (lambda: K.dropout(x, 0.1, s, x[:1]), RuntimeError, "like the input"),
+        (lambda: K.dropout(x, 0.1, s.cpu()), ops.UnsupportedByB200, "no CPU path"),
+        (lambda: K.quantize_rows(q), ops.UnsupportedByB200, "int8"),
+        (lambda: K.mm_int8(q, q.t(), one, one[:3]), RuntimeError, "fp32 values"),
+        (lambda: K.mm_int8(q, q, one, one), RuntimeError, "cannot be multiplied"),
+    ):
+        with pytest.raises(error, match=match):
+            call()
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward mode|jvp"):
+            K.gated_linear(torch.autograd.forward_ad.make_dual(x, x), w)
+
+
+@pytest.mark.parametrize("odd", [0, 3])
 def test_calls_repeat_bit_for_bit_on_other_streams_and_side_by_side(odd):
     args = _all_args(odd=odd)
     want = _all_calls(*args)
