@@ -1,5 +1,7 @@
 // What stands around the products of a feed-forward block: the gate of a projection pair and its gradient, dropout
 // whose mask is drawn from a counter, and the quantisation of rows to 8 bits. All are one pass over their data.
+#include <type_traits>
+
 #include "b200_common.cuh"
 #include "gate_act.cuh"
 
@@ -99,9 +101,17 @@ template <typename T> int launch_gate_backward(const void* dh, const float* p, v
 // (offset + i / 4, subsequence) under the 64-bit key `seed`. Nothing but the counter goes into an element's
 // word, so the backward pass draws the same mask again instead of reading one, whatever the launch shape.
 // What is dropped is not multiplied: an infinity or a NaN in a dropped place leaves nothing.
-struct PhiloxKeys {
-  uint32_t k[20];
-  __device__ __forceinline__ explicit PhiloxKeys(uint64_t seed) {
+//
+// What bounds it is the generator's multiplications as much as memory: 20 of 32 x 32 bits to four elements. The counter's upper three
+// words hardly ever change, so the products of the first two rounds that depend on them alone are kept (18 remain), and
+// the next elements are on their way while the words of these are worked out. 8192 x 4096 in bf16: 33.4 us, 37.2 with a residual (4.0 and
+// 5.4 TB/s; with p = 0, where nothing is drawn, 21.9), fp32 47 and 64 us (5.7 and 6.3 TB/s). The words of that many elements
+// alone take 20.6 us: a 32-bit multiplication keeps its pipe for four cycles, wide or not.
+struct Philox {
+  uint32_t k[20];                  // the rounds' keys
+  uint32_t sub0, sub1;             // the counter's words 2 and 3
+  uint32_t hi, a1, b1, c2, d2;     // word 1, and what the first two rounds make of words 1 to 3 alone
+  __device__ __forceinline__ Philox(uint64_t seed, uint64_t subsequence) : sub0(static_cast<uint32_t>(subsequence)), sub1(static_cast<uint32_t>(subsequence >> 32)) {
     uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
@@ -110,88 +120,171 @@ struct PhiloxKeys {
       k0 += 0x9E3779B9u;
       k1 += 0xBB67AE85u;
     }
+    upper(0u);
+  }
+  __device__ __forceinline__ void upper(uint32_t word1) {
+    hi = word1;
+    const uint64_t q = static_cast<uint64_t>(sub0) * 0xCD9E8D57u;
+    a1 = static_cast<uint32_t>(q >> 32) ^ hi ^ k[0];
+    b1 = static_cast<uint32_t>(q) ^ k[2];
+    const uint64_t p = static_cast<uint64_t>(a1) * 0xD2511F53u;
+    c2 = static_cast<uint32_t>(p >> 32) ^ k[3];
+    d2 = static_cast<uint32_t>(p);
+  }
+  // (word 1 of the counter is `hi`)
+  __device__ __forceinline__ void words(uint32_t word0, uint32_t* w) const {
+    const uint64_t p1 = static_cast<uint64_t>(word0) * 0xD2511F53u;
+    const uint64_t q2 = static_cast<uint64_t>(static_cast<uint32_t>(p1 >> 32) ^ sub1 ^ k[1]) * 0xCD9E8D57u;
+    uint32_t a = static_cast<uint32_t>(q2 >> 32) ^ b1, b = static_cast<uint32_t>(q2), c = c2 ^ static_cast<uint32_t>(p1), d = d2;
+#pragma unroll
+    for (int r = 2; r < 10; ++r) {
+      const uint64_t p = static_cast<uint64_t>(a) * 0xD2511F53u, q = static_cast<uint64_t>(c) * 0xCD9E8D57u;
+      a = static_cast<uint32_t>(q >> 32) ^ b ^ k[2 * r];
+      c = static_cast<uint32_t>(p >> 32) ^ d ^ k[2 * r + 1];
+      b = static_cast<uint32_t>(q);
+      d = static_cast<uint32_t>(p);
+    }
+    w[0] = a;
+    w[1] = b;
+    w[2] = c;
+    w[3] = d;
   }
 };
-__device__ __forceinline__ void philox(const PhiloxKeys& key, uint64_t count, uint64_t subsequence, uint32_t* w) {
-  uint32_t a = static_cast<uint32_t>(count), b = static_cast<uint32_t>(count >> 32), c = static_cast<uint32_t>(subsequence), d = static_cast<uint32_t>(subsequence >> 32);
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint64_t p = static_cast<uint64_t>(a) * 0xD2511F53u, q = static_cast<uint64_t>(c) * 0xCD9E8D57u;
-    a = static_cast<uint32_t>(q >> 32) ^ b ^ key.k[2 * r];
-    c = static_cast<uint32_t>(p >> 32) ^ d ^ key.k[2 * r + 1];
-    b = static_cast<uint32_t>(q);
-    d = static_cast<uint32_t>(p);
-  }
-  w[0] = a;
-  w[1] = b;
-  w[2] = c;
-  w[3] = d;
-}
 
 struct DropoutArgs {
   int64_t n;
   uint64_t subsequence;
   const int64_t* state;  // seed, offset
   uint32_t threshold;
-  int mode;              // 0: nothing is dropped, 1: by the words, 2: everything
   float scale;
 };
+enum : int { kKeepAll = 0, kByWords = 1, kDropAll = 2 };
 
-// VEC = 16 bytes of elements (one or two counters) or four elements (unaligned: one counter)
-template <typename T, bool VECTOR>
-__global__ void __launch_bounds__(kFfThreads) dropout_kernel(const T* x, const T* residual, T* __restrict__ y, DropoutArgs A) {
-  constexpr int kPer = VECTOR ? 16 / static_cast<int>(sizeof(T)) : 4;
-  const PhiloxKeys key(static_cast<uint64_t>(A.state[0]));
+// Said so that it stays a byte permutation: a shift may become a multiplication, and these are what there is too much of (8192 x 4096
+// in bf16 35.1 -> 33.4 us, with a residual 39.3 -> 37.2).
+__device__ __forceinline__ uint32_t byte_order(uint32_t v, uint32_t order) {
+  uint32_t r;
+  asm volatile("prmt.b32 %0, %1, 0, %2;" : "=r"(r) : "r"(v), "r"(order));
+  return r;
+}
+// Two elements of a 16-bit word, or an fp32 pair, as fp32 bits: what is dropped becomes zero here, before any arithmetic
+template <typename T> __device__ __forceinline__ void kept_pair(uint32_t lo, uint32_t hi, bool keep0, bool keep1, float& a, float& b) {
+  if constexpr (sizeof(T) == 4) {
+    a = keep0 ? __uint_as_float(lo) : 0.f;
+    b = keep1 ? __uint_as_float(hi) : 0.f;
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    a = __uint_as_float(keep0 ? byte_order(lo, 0x1044u) : 0u);
+    b = __uint_as_float(keep1 ? byte_order(lo, 0x3244u) : 0u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+    a = keep0 ? f.x : 0.f;
+    b = keep1 ? f.y : 0.f;
+  }
+}
+
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ uint4 ld_shared(uint32_t from) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+  return v;
+}
+
+// Sixteen bytes of elements to a thread and step, the next ones on their way to its own slot in shared memory; whatever is behind the last whole sixteen, or all of them where the operands are off
+// the grid (VECTOR false), goes four elements to a thread.
+template <typename T, int MODE, bool RESIDUAL, bool VECTOR>
+__global__ void __launch_bounds__(kFfThreads, 4) dropout_kernel(const T* x, const T* residual, T* __restrict__ y, DropoutArgs A) {
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T)), kWords = sizeof(T) == 4 ? 2 : 1;
+  Philox gen(static_cast<uint64_t>(A.state[0]), A.subsequence);
   const uint64_t offset = static_cast<uint64_t>(A.state[1]);
-  const int64_t groups = (A.n + kPer - 1) / kPer;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x; i < groups; i += static_cast<int64_t>(gridDim.x) * kFfThreads) {
-    const int64_t at = i * kPer;
-    const int left = A.n - at < kPer ? static_cast<int>(A.n - at) : kPer;
-    float v[kPer], r[kPer];
-    uint4 rx, rr;
-    const bool whole = VECTOR && left == kPer;
-    if (whole) {
-      rx = ld_stream(x + at);
-      if (residual) rr = ld_stream(residual + at);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        v[e] = e < left ? to_f32(x[at + e]) : 0.f;
-        r[e] = residual && e < left ? to_f32(residual[at + e]) : 0.f;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * kFfThreads;
+  const int64_t vecs = VECTOR ? A.n / kPer : 0;
+  if constexpr (VECTOR) {
+    __shared__ uint4 slots[2][RESIDUAL ? 2 : 1][kFfThreads];
+    int trips = first < vecs ? static_cast<int>((vecs - first + step - 1) / step) : 0;
+    const uint4 *px = reinterpret_cast<const uint4*>(x) + first, *pr = reinterpret_cast<const uint4*>(residual) + first;
+    uint4* py = reinterpret_cast<uint4*>(y) + first;
+    uint64_t count = offset + static_cast<uint64_t>(first) * (kPer / 4);
+    const uint64_t counts = static_cast<uint64_t>(step) * (kPer / 4);
+    const F2 scale = F2::of(A.scale, A.scale);
+    const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(&slots[0][0][threadIdx.x]));
+    constexpr uint32_t kOther = kFfThreads * 16, kSlot = (RESIDUAL ? 2 : 1) * kOther;
+    auto load = [&](uint32_t slot) {
+      if constexpr (MODE != kDropAll) copy_async(mine + slot, px);
+      if constexpr (RESIDUAL) copy_async(mine + slot + kOther, pr);
+      px += step;
+      pr += step;
+    };
+    auto take = [&](uint32_t slot, uint32_t next) {
+      if (trips > 1) load(next);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      uint32_t w[kPer];
+      if constexpr (MODE == kByWords) {
+        const uint32_t word0 = static_cast<uint32_t>(count);
+        if (static_cast<uint32_t>(count >> 32) != gen.hi) gen.upper(static_cast<uint32_t>(count >> 32));
+        gen.words(word0, w);
+        if constexpr (kPer == 8) {
+          if (word0 == 0xffffffffu) gen.upper(gen.hi + 1);
+          gen.words(word0 + 1, w + 4);
+        }
+        count += counts;
       }
-    }
-    uint32_t w[kPer];
-    if (A.mode == 1) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      const uint4 rx = MODE != kDropAll ? ld_shared(mine + slot) : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t in[4] = {rx.x, rx.y, rx.z, rx.w};
+      float v[kPer], r[kPer];
+      if constexpr (RESIDUAL) widen<T>(ld_shared(mine + slot + kOther), r);
 #pragma unroll
-      for (int c = 0; c < kPer / 4; ++c) philox(key, offset + static_cast<uint64_t>(i) * (kPer / 4) + c, A.subsequence, w + 4 * c);
+      for (int e = 0; e < kPer; e += 2) {
+        auto keep = [&](int k) { return MODE == kKeepAll || (MODE == kByWords && w[k] >= A.threshold); };
+        kept_pair<T>(in[e / 2 * kWords], in[e / 2 * kWords + kWords - 1], keep(e), keep(e + 1), v[e], v[e + 1]);
+        const F2 of = F2::of(v[e], v[e + 1]);
+        p_parts(RESIDUAL ? p_fma(of, scale, F2::of(r[e], r[e + 1])) : p_mul(of, scale), v[e], v[e + 1]);
+      }
+      __stcs(py, narrow<T>(v));
+      py += step;
+    };
+    if (trips) load(0);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    while (trips > 0) {
+      take(0, kSlot);
+      if (--trips == 0) break;
+      take(kSlot, 0);
+      --trips;
     }
-    if (whole) {
-      widen<T>(rx, v);
-      if (residual) widen<T>(rr, r);
+  }
+  const int64_t groups = (A.n + 3) / 4;
+  for (int64_t i = vecs * (kPer / 4) + first; i < groups; i += step) {
+    uint32_t w[4];
+    const uint64_t count = offset + static_cast<uint64_t>(i);
+    if constexpr (MODE == kByWords) {
+      if (static_cast<uint32_t>(count >> 32) != gen.hi) gen.upper(static_cast<uint32_t>(count >> 32));
+      gen.words(static_cast<uint32_t>(count), w);
     }
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const bool keep = A.mode == 0 || (A.mode == 1 && w[e] >= A.threshold);
-      v[e] = keep ? v[e] * A.scale : 0.f;
-      if (residual) v[e] += r[e];
-    }
-    if (whole) {
-      st_stream(y + at, narrow<T>(v));
-    } else {
-#pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        if (e < left) y[at + e] = from_f32<T>(v[e]);
+    for (int e = 0; e < 4; ++e) {
+      const int64_t at = 4 * i + e;
+      if (at >= A.n) break;
+      const float v = MODE == kKeepAll || (MODE == kByWords && w[e] >= A.threshold) ? to_f32(x[at]) : 0.f;
+      y[at] = from_f32<T>(RESIDUAL ? fmaf(v, A.scale, to_f32(residual[at])) : v * A.scale);
     }
   }
 }
 
-template <typename T> int launch_dropout(const void* x, const void* residual, void* y, const DropoutArgs& A, cudaStream_t st) {
+template <typename T> int launch_dropout(const void* x, const void* residual, void* y, int mode, const DropoutArgs& A, cudaStream_t st) {
   const bool vec = aligned16(x) && aligned16(y) && (!residual || aligned16(residual));
-  const int64_t per = vec ? 16 / static_cast<int>(sizeof(T)) : 4;
-  const int grid = ff_grid((A.n + per - 1) / per);
+  const int64_t per = vec ? 16 / static_cast<int>(sizeof(T)) : 4, blocks = (A.n + per * kFfThreads - 1) / (per * kFfThreads), most = kNumSMs * 8LL;
+  const int grid = static_cast<int>(blocks < most ? blocks : most);
   const T *tx = static_cast<const T*>(x), *tr = static_cast<const T*>(residual);
-  if (vec) dropout_kernel<T, true><<<grid, kFfThreads, 0, st>>>(tx, tr, static_cast<T*>(y), A);
-  else dropout_kernel<T, false><<<grid, kFfThreads, 0, st>>>(tx, tr, static_cast<T*>(y), A);
+  T* ty = static_cast<T*>(y);
+  auto go = [&](auto kernel) { kernel<<<grid, kFfThreads, 0, st>>>(tx, tr, ty, A); };
+  auto by_mode = [&](auto r, auto v) {
+    constexpr bool kR = decltype(r)::value, kV = decltype(v)::value;
+    if (mode == kKeepAll) go(dropout_kernel<T, kKeepAll, kR, kV>);
+    else if (mode == kByWords) go(dropout_kernel<T, kByWords, kR, kV>);
+    else go(dropout_kernel<T, kDropAll, kR, kV>);
+  };
+  if (residual) vec ? by_mode(std::true_type{}, std::true_type{}) : by_mode(std::true_type{}, std::false_type{});
+  else vec ? by_mode(std::false_type{}, std::true_type{}) : by_mode(std::false_type{}, std::false_type{});
   return check_launch();
 }
 
@@ -319,14 +412,14 @@ extern "C" int b200_dropout(const void* x, const void* residual, void* out, int6
   A.subsequence = static_cast<uint64_t>(subsequence);
   A.state = state;
   const uint64_t threshold = static_cast<uint64_t>(nearbyint(words));
-  A.mode = threshold == 0 ? 0 : threshold > 0xffffffffull ? 2 : 1;
+  const int mode = threshold == 0 ? kKeepAll : threshold > 0xffffffffull ? kDropAll : kByWords;
   A.threshold = static_cast<uint32_t>(threshold);
   A.scale = p < 1. ? static_cast<float>(1. / (1. - p)) : 0.f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case B200_F32: return launch_dropout<float>(x, residual, out, A, st);
-    case B200_BF16: return launch_dropout<__nv_bfloat16>(x, residual, out, A, st);
-    default: return launch_dropout<__half>(x, residual, out, A, st);
+    case B200_F32: return launch_dropout<float>(x, residual, out, mode, A, st);
+    case B200_BF16: return launch_dropout<__nv_bfloat16>(x, residual, out, mode, A, st);
+    default: return launch_dropout<__half>(x, residual, out, mode, A, st);
   }
 }
 

@@ -393,13 +393,41 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
 
 // ------------------------------------------------------------------ operands off the grid
 // A matrix [rows, K] of any strides into rows along K with a pitch that is a multiple of 16 bytes, for the copy engine.
-// 32 x 32 tiles through shared memory, read along whichever dimension is contiguous.
+//
+// Rows that lie along K, off the 16-byte grid: a thread to 16 bytes of the result, from the one or two aligned blocks that its bytes
+// lie in, shifted into place. A block holds a byte of the matrix or is not read, so that no load leaves the
+// 16-byte granules of the matrix itself. What lands behind a row's end is padding that the tensor map leaves out.
+__global__ void __launch_bounds__(256) pack_rows_shifted(const unsigned char* x, unsigned char* __restrict__ to, int64_t rows, int64_t row_bytes, int64_t s_bytes, uint32_t pieces) {
+  const int64_t total = rows * pieces;
+  const unsigned char* end = x + (rows - 1) * s_bytes + row_bytes;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t r = total <= 0xffffffffll ? static_cast<uint32_t>(i) / pieces : i / pieces;
+    const int64_t j = i - r * pieces;
+    const unsigned char* from = x + r * s_bytes + j * 16;
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from)) & 15u;
+    const unsigned char* block = from - off;
+    const uint4 lo = ld_keep(block);
+    uint4 hi = make_uint4(0u, 0u, 0u, 0u);
+    if (off && block + 16 < end) hi = ld_keep(block + 16);
+    const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    const uint32_t skip = off >> 2, bits = (off & 3u) * 8u;
+    uint32_t v[5];  // the five words that the sixteen bytes lie in
+#pragma unroll
+    for (int k = 0; k < 5; ++k) {
+      const uint32_t a = skip & 1u ? w[k + 1 < 8 ? k + 1 : 7] : w[k], b = skip & 1u ? w[k + 3 < 8 ? k + 3 : 7] : w[k + 2 < 8 ? k + 2 : 7];
+      v[k] = skip & 2u ? b : a;
+    }
+    *reinterpret_cast<uint4*>(to + i * 16) = make_uint4(__funnelshift_r(v[0], v[1], bits), __funnelshift_r(v[1], v[2], bits), __funnelshift_r(v[2], v[3], bits), __funnelshift_r(v[3], v[4], bits));
+  }
+}
+
+// Any other strides: 32 x 32 tiles through shared memory, read along whichever dimension is contiguous.
 template <typename E>
 __global__ void __launch_bounds__(256) pack_rows(const E* x, E* __restrict__ to, int64_t rows, int64_t K, int64_t s_r, int64_t s_k, int64_t pitch) {
   __shared__ E tile[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t kt = (K + 31) / 32, tiles = ((rows + 31) / 32) * kt;
-  const bool along_k = s_k == 1 || s_r != 1;
+  const bool along_k = s_r != 1;
   for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
     const int64_t r0 = t / kt * 32, k0 = (t % kt) * 32;
     __syncthreads();
@@ -429,10 +457,16 @@ int pack(LinOperand& o, unsigned char*& at, cudaStream_t st, int& launches) {
     if (o.rows == 1) o.s_r = o.pitch();  // never used
     return B200_OK;
   }
-  const int64_t tiles = ((o.rows + 31) / 32) * ((o.K + 31) / 32), most = kNumSMs * 8;
-  const int grid = static_cast<int>(tiles < most ? tiles : most);
-  if (o.esize == 2) pack_rows<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(o.base), reinterpret_cast<uint16_t*>(at), o.rows, o.K, o.s_r, o.s_k, o.pitch());
-  else pack_rows<uint8_t><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(o.base), at, o.rows, o.K, o.s_r, o.s_k, o.pitch());
+  const int64_t most = kNumSMs * 8;
+  if (o.s_k == 1 || o.K == 1) {
+    const int64_t pieces = o.pitch() * o.esize / 16, blocks = (o.rows * pieces + 255) / 256;
+    pack_rows_shifted<<<static_cast<int>(blocks < most ? blocks : most), 256, 0, st>>>(static_cast<const unsigned char*>(o.base), at, o.rows, o.K * o.esize, o.s_r * o.esize, static_cast<uint32_t>(pieces));
+  } else {
+    const int64_t tiles = ((o.rows + 31) / 32) * ((o.K + 31) / 32);
+    const int grid = static_cast<int>(tiles < most ? tiles : most);
+    if (o.esize == 2) pack_rows<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(o.base), reinterpret_cast<uint16_t*>(at), o.rows, o.K, o.s_r, o.s_k, o.pitch());
+    else pack_rows<uint8_t><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(o.base), at, o.rows, o.K, o.s_r, o.s_k, o.pitch());
+  }
   const int64_t bytes = o.packed_bytes();
   o.s_r = o.pitch();
   o.s_k = 1;
