@@ -20,6 +20,8 @@
 // rows as there are; the MMA's other rows multiply whatever lies behind it and are never stored.
 #include <cuda.h>
 
+#include <cmath>
+
 #include "b200_common.cuh"
 #include "gate_act.cuh"
 #include "tc_common.cuh"
@@ -33,11 +35,13 @@ constexpr int kSlabBytes = 128;                         // of K to a slab: one r
 constexpr int kLinRing = 192 * 1024;
 constexpr int kLinEpiWarps = 8, kLinEpiBytes = 4096;    // staging: 32 rows x 128 bytes per epilogue warp
 constexpr int kLinMaxStages = 16;
-constexpr int kLinAccCols = 256, kLinAccs = 2;
-constexpr size_t kLinSmem = static_cast<size_t>(kLinRing) + kLinEpiWarps * kLinEpiBytes + 1024 /*align*/ + 512 /*barriers*/;
+constexpr int kLinAccs = 2;  // at most
+constexpr int kLinHalfRing = 108 * 1024;                // two CTAs to an SM: 110 KB each (and never three, which would be more tensor memory than there is)
+constexpr size_t lin_smem(int ring) { return static_cast<size_t>(ring) + (ring == kLinRing ? kLinEpiWarps * kLinEpiBytes : 0) + 1024 /*align*/ + 512 /*barriers*/; }
 constexpr uint64_t kLinWaitNs = 2000000000ull;
 
 enum : int { kGated = 0, kInt8 = 1 };
+enum : int { kSingle = 0, kPaired = 1, kSplit = 2 };  // a CTA to a tile; a pair to a tile of 256 rows; a cluster that shares a tile's K
 
 struct LinParams {
   int64_t M, N, K;        // outputs M x N; K in elements
@@ -46,6 +50,10 @@ struct LinParams {
   int b_boxes;            // boxes of B in this CTA's stage (gated on a single CTA: gate and up)
   int k_step;             // elements of K to a slab
   int group_m;            // row blocks per rasterisation group
+  int splits;             // kSplit: CTAs that share a tile's K
+  int ring, stages;       // bytes of shared memory for the slabs, and how many that is (see ring_stages)
+  int acc_cols, accs;     // accumulators in tensor memory: columns of one, how many
+  int early;              // the next grid may start beside this one
   uint32_t idesc;
   int act;                // gated: activation
   float* side;            // gated: the projections [M, 2 N], or NULL
@@ -74,12 +82,23 @@ __device__ __forceinline__ void lin_mma_pair(uint32_t d, uint64_t a, uint64_t b,
   }
 }
 
+__device__ __forceinline__ void prefetch_l2_3d(const CUtensorMap* map, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+
 __device__ __forceinline__ void lin_tile(int64_t t, int64_t mt, int64_t nt, int group_m, int& mb, int& nb) {
   const int64_t per_group = static_cast<int64_t>(group_m) * nt;
   const int64_t g = t / per_group, in_g = t - g * per_group;
   const int64_t left = mt - g * group_m, gm = left < group_m ? left : group_m;
   mb = static_cast<int>(g * group_m + in_g % gm);
   nb = static_cast<int>(in_g / gm);
+}
+
+// 16 bytes of a cluster CTA's shared memory
+template <typename V> __device__ __forceinline__ V ld_cluster(uint32_t from) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+  return *reinterpret_cast<const V*>(&v);
 }
 
 // 32 values of a lane's row to 32 columns of `out` (row pitch `pitch`, column 0 at `col`): rounded once into the warp's
@@ -108,14 +127,32 @@ __device__ __forceinline__ void lin_store(const float* v, unsigned char* mine, T
   }
 }
 
-template <int MODE, typename TO, bool kPair>
+// One output of a sum (gated: of both) and where it goes
+template <int MODE, typename TO> __device__ __forceinline__ void lin_out(const LinParams& p, TO* out, const float* a_scale, const float* b_scale, const TO* bias, int64_t m, int64_t n, float g, float u) {
+  if constexpr (MODE == kInt8) {
+    float v = g * a_scale[m] * b_scale[n];
+    if (bias) v += to_f32(bias[n]);
+    out[m * p.N + n] = from_f32<TO>(v);
+  } else {
+    if (p.side) {
+      p.side[m * 2 * p.N + n] = g;
+      p.side[m * 2 * p.N + p.N + n] = u;
+    }
+    float h = 0.f;
+    gate_act_each(p.act, [&](auto act) { h = act.fast(g) * u; });
+    out[m * p.N + n] = from_f32<TO>(h);
+  }
+}
+
+template <int MODE, typename TO, int SHARE>
 __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, TO* __restrict__ out, LinParams p, uint32_t* __restrict__ status) {
-  constexpr bool kI8 = MODE == kInt8;
+  constexpr bool kI8 = MODE == kInt8, kPair = SHARE == kPaired;
   constexpr int kTileM = kPair ? 256 : 128;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  unsigned char* epi_stage = smem + kLinRing;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kLinRing + kLinEpiWarps * kLinEpiBytes);
+  // (a CTA with one tile has multiplied all of its slabs when it stores: it stages where they were)
+  unsigned char* epi_stage = smem + (p.ring == kLinRing ? kLinRing : 0);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.ring + (p.ring == kLinRing ? kLinEpiWarps * kLinEpiBytes : 0));
   uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(bars + 2 * kLinMaxStages + 2 * kLinAccs);
   volatile uint32_t* abort_flag = tmem_base_slot + 1;
 
@@ -127,8 +164,8 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
   auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * kLinMaxStages + kLinAccs + a); };
   const uint32_t a_bytes = static_cast<uint32_t>(p.a_rows) * kSlabBytes, b_bytes = static_cast<uint32_t>(p.b_rows) * kSlabBytes;
   const uint32_t stage_bytes = a_bytes + static_cast<uint32_t>(p.b_boxes) * b_bytes;
-  const int fit = kLinRing / static_cast<int>(stage_bytes), stages = fit < kLinMaxStages ? fit : kLinMaxStages;
-  const uint32_t cta_rank = kPair ? cluster_ctarank() : 0u;
+  const int stages = p.stages;
+  const uint32_t rank = SHARE != kSingle ? cluster_ctarank() : 0u, cta_rank = kPair ? rank : 0u;
 
   if (threadIdx.x == 64) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_a)) : "memory");
@@ -139,7 +176,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
     }
-    for (int a = 0; a < kLinAccs; ++a) {
+    for (int a = 0; a < p.accs; ++a) {
       mbar_init(tfull_bar(a), 1);
       mbar_init(tempty_bar(a), kPair ? 16 : 8);
     }
@@ -148,10 +185,10 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
   }
   if (warp == 1) {
     if (kPair) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)), "r"(kLinAccs * kLinAccCols) : "memory");
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)), "r"(p.accs * p.acc_cols) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     } else {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)), "r"(kLinAccs * kLinAccCols) : "memory");
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)), "r"(p.accs * p.acc_cols) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
   }
@@ -160,13 +197,30 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
   if (kPair) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_base_slot;
+  if constexpr (!kPair) {
+    // Beside this grid there is room for the next one's CTAs (which start here, where every CTA has its tensor memory): they set
+    // themselves up and bring the first of their weights into L2, which holds whatever this grid writes all the same.
+    if (p.early) next_grid_may_start();
+    if (p.early && warp == 0 && lane == 0) {
+      const int64_t t = SHARE == kSplit ? blockIdx.x / p.splits : blockIdx.x, mt = (p.M + 127) / 128, nt = (p.N + p.w - 1) / p.w;
+      const int all = static_cast<int>((p.K + p.k_step - 1) / p.k_step), k0 = SHARE == kSplit ? static_cast<int>(static_cast<int64_t>(all) * rank / p.splits) : 0;
+      int mb, nb;
+      lin_tile(t, mt, nt, p.group_m, mb, nb);
+      for (int s = 0; s < stages && k0 + s < all; ++s) {
+        prefetch_l2_3d(&map_b, (k0 + s) * p.k_step, nb * p.w, 0);
+        if (!kI8) prefetch_l2_3d(&map_b, (k0 + s) * p.k_step, nb * p.w + static_cast<int>(p.N), 0);
+      }
+    }
+  }
   after_grids_before();
   const float *a_scale = waited(p.a_scale), *b_scale = waited(p.b_scale);
   const TO* bias = waited(static_cast<const TO*>(p.bias));
 
   const int64_t mt = (p.M + kTileM - 1) / kTileM, nt = (p.N + p.w - 1) / p.w, tiles = mt * nt;
-  const int64_t tile_first = kPair ? (blockIdx.x >> 1) : blockIdx.x, tile_step = kPair ? (gridDim.x >> 1) : gridDim.x;
-  const int slabs = static_cast<int>((p.K + p.k_step - 1) / p.k_step);
+  const int64_t tile_first = kPair ? (blockIdx.x >> 1) : SHARE == kSplit ? blockIdx.x / p.splits : blockIdx.x, tile_step = kPair ? (gridDim.x >> 1) : SHARE == kSplit ? tiles : gridDim.x;
+  const int all_slabs = static_cast<int>((p.K + p.k_step - 1) / p.k_step);
+  const int slab0 = SHARE == kSplit ? static_cast<int>(static_cast<int64_t>(all_slabs) * rank / p.splits) : 0;
+  const int slabs = SHARE == kSplit ? static_cast<int>(static_cast<int64_t>(all_slabs) * (rank + 1) / p.splits) - slab0 : all_slabs;
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -184,7 +238,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
         for (int kb = 0; kb < slabs; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, kLinWaitNs)) { ok = false; break; }
           const uint32_t a_dst = smem_base + stage * stage_bytes, b_dst = a_dst + a_bytes;
-          const int k = kb * p.k_step;
+          const int k = (slab0 + kb) * p.k_step;
           if (kPair) {
             const uint32_t fbar = map_to_cta(full_bar(stage), 0u);
             if (cta_rank == 0u) mbar_expect_tx(full_bar(stage), 2 * stage_bytes);
@@ -223,7 +277,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
       for (int64_t t = tile_first; t < tiles && ok; t += tile_step) {
         if (!warp_wait(tempty_bar(acc), acc_phase ^ 1u)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kLinAccCols);
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * p.acc_cols);
         for (int kb = 0; kb < slabs; ++kb) {
           if (!warp_wait(full_bar(stage), phase)) { ok = false; break; }
           tc_fence_after();
@@ -261,7 +315,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
           }
         }
         __syncwarp();
-        if (++acc == kLinAccs) { acc = 0; acc_phase ^= 1u; }
+        if (++acc == p.accs) { acc = 0; acc_phase ^= 1u; }
       }
       if (!ok && lane == 0) {
         *abort_flag = 1;
@@ -292,7 +346,25 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
       got = __shfl_sync(0xffffffffu, got, 0);
       if (!got) { ok = false; break; }
       tc_fence_after();
-      const uint32_t t_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * kLinAccCols);
+      const uint32_t t_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * p.acc_cols);
+      if constexpr (SHARE == kSplit) {
+        // this CTA's sums to its own shared memory (everything that was in the ring has been multiplied), a row to a lane
+        const int columns = p.w * (kI8 ? 1 : 2);
+        if (q * 32 < p.a_rows) {
+          for (int c = half * 32; c < columns; c += 64) {
+            uint32_t r[32];
+            tc_ld_32x32(t_base + static_cast<uint32_t>(c), r);
+            tc_ld_wait();
+            unsigned char* row = smem + (q * 32 + lane) * (columns * 4 + 16) + c * 4;
+            if (q * 32 + lane < p.a_rows) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                if (c + e < columns) *reinterpret_cast<uint4*>(row + e * 4) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
+            }
+          }
+        }
+        break;
+      }
       uint32_t r[kRegs];
       auto fetch = [&](int i) {
         const uint32_t col = static_cast<uint32_t>((half + 2 * i) * 32);
@@ -367,13 +439,46 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
         }
         if (nrows > 0) lin_store<TO>(v, mine, out + mr0 * p.N + n, p.N, nrows, ncols, vec, lane);
       }
-      if (++acc == kLinAccs) { acc = 0; acc_phase ^= 1u; }
+      if (++acc == p.accs) { acc = 0; acc_phase ^= 1u; }
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
       if (status) atomicOr(status, B200_DEV_WAIT_TIMEOUT);
     }
     __syncwarp();
+  }
+
+  if constexpr (SHARE == kSplit) {
+    // Every CTA of the cluster puts together its share of the tile: four columns to a thread, the CTAs' sums added in the order of
+    // their ranges of K.
+    cluster_sync_all();
+    const int columns = p.w * (kI8 ? 1 : 2), quads = p.w / 4;
+    const uint32_t pitch = static_cast<uint32_t>(columns) * 4 + 16;
+    int mb, nb;
+    lin_tile(tile_first, mt, nt, p.group_m, mb, nb);
+    const int64_t mr0 = static_cast<int64_t>(mb) * 128, n0 = static_cast<int64_t>(nb) * p.w;
+    const int rows = p.M - mr0 < p.a_rows ? static_cast<int>(p.M - mr0) : p.a_rows, units = rows * quads;
+    for (int i = static_cast<int>(rank) * kLinThreads + static_cast<int>(threadIdx.x); i < units; i += p.splits * kLinThreads) {
+      const int r = i / quads, c = (i - r * quads) * 4;
+      const uint32_t at = smem_base + static_cast<uint32_t>(r) * pitch + static_cast<uint32_t>(c) * 4;
+      float g[4] = {}, u[4] = {};
+      int s[4] = {};
+      for (int k = 0; k < p.splits; ++k) {
+        const uint32_t from = map_to_cta(at, static_cast<uint32_t>(k));
+        if constexpr (kI8) {
+          const int4 v = ld_cluster<int4>(from);
+          s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+        } else {
+          const float4 v = ld_cluster<float4>(from), w = ld_cluster<float4>(from + static_cast<uint32_t>(p.w) * 4);
+          g[0] += v.x; g[1] += v.y; g[2] += v.z; g[3] += v.w;
+          u[0] += w.x; u[1] += w.y; u[2] += w.z; u[3] += w.w;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n0 + c + e < p.N) lin_out<MODE, TO>(p, out, a_scale, b_scale, bias, mr0 + r, n0 + c + e, kI8 ? static_cast<float>(s[e]) : g[e], u[e]);
+    }
+    cluster_sync_all();  // nobody leaves while another reads its sums
   }
 
   // ---------------------------------------------------------------- teardown
@@ -386,8 +491,8 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
   }
   if (kPair) cluster_sync_all();
   if (warp == 1) {
-    if (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kLinAccs * kLinAccCols) : "memory");
-    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kLinAccs * kLinAccCols) : "memory");
+    if (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(p.accs * p.acc_cols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(p.accs * p.acc_cols) : "memory");
   }
 }
 
@@ -485,59 +590,100 @@ bool encode_rows(CUtensorMap* map, const LinOperand& o, CUtensorMapDataType dt, 
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Slabs that fit into `ring` bytes. The MMA reads 128 rows of A whatever the box holds, so the last slab has that much room too.
+constexpr int kMmaABytes = 128 * kSlabBytes;
+int ring_stages(int ring, int stage_bytes) {
+  const int last = stage_bytes > kMmaABytes ? stage_bytes : kMmaABytes, fit = 1 + (ring - last) / stage_bytes;
+  return fit < kLinMaxStages ? fit : kLinMaxStages;
+}
+
+// CTAs of a whole SM's shared memory that are resident at once in clusters of 1 .. 8 (cudaOccupancyMaxActiveClusters on a B200)
+constexpr int kResident[9] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
+
 struct LinPlan {
-  bool pair;
-  int w, a_rows;
+  int share, w, a_rows, splits;
 };
-// `per`: rows of B to an output column (gated 2, int8 1).
+int lin_stage_bytes(int per, int w, int a_rows) { return (a_rows + per * w) * kSlabBytes; }  // (a CTA of a pair: half of them)
+bool half_an_sm(int per, int w, int a_rows, int splits) {
+  return 4 * lin_stage_bytes(per, w, a_rows) <= kLinHalfRing && (splits == 1 || a_rows * (w * per * 4 + 16) <= kLinHalfRing);
+}
+
+// What a plan takes, in us, with `per` rows of B to an output column (gated 2, int8 1) and slabs of 128 bytes of K. The terms: what
+// starting, handing over and storing take; the weights out of HBM; every CTA's bytes over the fabric; the latency of the loads
+// (longer for B, which comes from HBM, than for A, which comes from L2) over the bytes that are in flight; the issue of a
+// slab. Their constants were fitted to 1,111 timings of 42 products (1 to 4096 rows, K 160 to 11008, 128 to 11008 columns, both
+// types); the plan with the least of these is 2 % slower than the best one that was timed, on average, and at most 19 %.
+double time_of(const LinPlan& q, int64_t M, int64_t N, int64_t slabs, int per) {
+  const double k = static_cast<double>(slabs), cols = q.w * per;
+  const int64_t across = (N + q.w - 1) / q.w;
+  if (q.share == kPaired) {
+    const int64_t tiles = ((M + 255) / 256) * across, rounds = (tiles + kNumSMs / 2 - 1) / (kNumSMs / 2);
+    return 9.0 + static_cast<double>(rounds) * (1.2 + k * (cols == 256 ? 0.31 : cols == 192 ? 0.20 : 0.167));
+  }
+  const int64_t tiles = ((M + 127) / 128) * across;
+  const bool half = half_an_sm(per, q.w, q.a_rows, q.splits) && tiles * q.splits <= 2 * kResident[q.splits];
+  const int64_t room = (half ? 2 : 1) * kResident[q.splits];
+  double ctas = static_cast<double>(tiles * q.splits), rounds = 1;
+  if (tiles * q.splits > room) {
+    if (q.splits > 1) return 1e30;  // a cluster has one tile
+    rounds = static_cast<double>((tiles + kNumSMs - 1) / kNumSMs);
+    ctas = kNumSMs;
+  }
+  const double each = static_cast<double>((slabs + q.splits - 1) / q.splits) * rounds, a = each * kSlabBytes * q.a_rows * ctas, b = each * kSlabBytes * cols * ctas;
+  const double deep = ctas > kNumSMs ? 2. : 1.;  // CTAs to an SM
+  double t = k * kSlabBytes * static_cast<double>(N * per) / 10.3e6;
+  t = fmax(t, (a + b) / 17e6);
+  t = fmax(t, (1.8 * b + 0.83 * a) / (ctas * (half ? kLinHalfRing : kLinRing)));
+  t = fmax(t, each * (0.235 * (deep > 1. ? 1.5 : 1.) + 0.00024 * cols * deep));
+  return 4.2 + (half ? 0. : 0.4) + t + 1.1 * rounds + 0.0045 * cols * deep + (q.splits > 1 ? 0.6 + q.a_rows * cols / 5e3 : 0.);
+}
+LinPlan best_plan(int64_t M, int64_t N, int64_t slabs, int per) {
+  const int most = 256 / per, grain = 16 / per, a_rows = M >= 128 ? 128 : static_cast<int>((M + 7) / 8 * 8);
+  LinPlan best{kSingle, most, a_rows, 1};
+  double least = 1e30;
+  auto offer = [&](const LinPlan& q) {
+    const double t = time_of(q, M, N, slabs, per);
+    if (t < least) { least = t; best = q; }
+  };
+  if (M > 128)
+    for (int w : {most, most * 3 / 4, most / 2}) offer(LinPlan{kPaired, w, 128, 1});
+  for (int s : {1, 2, 3, 4, 6, 8})
+    for (int w : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16})
+      if (s <= slabs) offer(LinPlan{s > 1 ? kSplit : kSingle, w * grain, a_rows, s});
+  return best;
+}
+// (a look at some seventy plans takes longer than a launch: each thread keeps those of the sizes it saw last)
 LinPlan plan_linear(int64_t M, int64_t N, int64_t K, int per, int k_step) {
+  struct Seen {
+    int64_t M, N, slabs;
+    int per;
+    LinPlan plan;
+  };
+  static thread_local Seen seen[64] = {};
   const int64_t slabs = (K + k_step - 1) / k_step;
-  const int most = 256 / per, grain = 16 / per;
-  if (M > 128 && N * per > 128 && slabs > 4) {
-    const int64_t mt = (M + 255) / 256;
-    auto rounds = [&](int w) { return (mt * ((N + w - 1) / w) + kNumSMs / 2 - 1) / (kNumSMs / 2); };
-    int best = most;
-    double least = static_cast<double>(rounds(most));
-    if (least <= 4.0) {
-      least *= 0.95;
-      for (const auto& c : {std::make_pair(most * 3 / 4, 0.83), std::make_pair(most / 2, 0.69)}) {
-        const double t = static_cast<double>(rounds(c.first)) * c.second;
-        if (t < least) { least = t; best = c.first; }
-      }
-    }
-    return LinPlan{true, best, 128};
-  }
-  const int a_rows = M >= 128 ? 128 : static_cast<int>((M + 7) / 8 * 8);
-  const int64_t mt = (M + 127) / 128;
-  int best = most;
-  double least = 0.;
-  for (int w = most; w >= grain; w -= grain) {
-    const int64_t tiles = mt * ((N + w - 1) / w), r = (tiles + kNumSMs - 1) / kNumSMs;
-    const double t = static_cast<double>(r) * (w * per + 0.4 * a_rows + 8);
-    if (least == 0. || t < least) { least = t; best = w; }
-  }
-  return LinPlan{false, best, a_rows};
+  Seen& s = seen[(static_cast<uint64_t>(M) * 31 + static_cast<uint64_t>(N) * 7 + static_cast<uint64_t>(slabs) * 3 + per) % 64];
+  if (s.M != M || s.N != N || s.slabs != slabs || s.per != per) s = Seen{M, N, slabs, per, best_plan(M, N, slabs, per)};
+  return s.plan;
 }
 
 template <typename Kernel, typename TO>
-int launch_linear(Kernel kernel, bool pair, int64_t tiles, cudaStream_t st, const CUtensorMap& map_a, const CUtensorMap& map_b, TO* out, const LinParams& p, uint32_t* status) {
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLinSmem));
+int launch_linear(Kernel kernel, int cluster, int64_t ctas, cudaStream_t st, const CUtensorMap& map_a, const CUtensorMap& map_b, TO* out, const LinParams& p, uint32_t* status) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lin_smem(kLinRing)));
   if (e != cudaSuccess) { set_last_cuda_error(e); return B200_ELAUNCH; }
-  const int64_t slots = pair ? kNumSMs / 2 : kNumSMs;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((tiles < slots ? tiles : slots) * (pair ? 2 : 1)), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
   cfg.blockDim = dim3(kLinThreads, 1, 1);
-  cfg.dynamicSmemBytes = kLinSmem;
+  cfg.dynamicSmemBytes = lin_smem(p.ring);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // (see launch_after)
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pair ? 2 : 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t le = cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, out, p, status);
   if (le != cudaSuccess) { set_last_cuda_error(le); return B200_ELAUNCH; }
   return B200_OK;
@@ -558,9 +704,11 @@ int run_linear(LinOperand a, LinOperand b, void* out, int64_t M, int64_t N, int6
   const LinPlan plan = plan_linear(M, N, K, per, p.k_step);
   p.w = plan.w;
   p.a_rows = plan.a_rows;
-  p.b_rows = MODE == kGated ? plan.w : plan.pair ? plan.w / 2 : plan.w;
-  p.b_boxes = MODE == kGated && !plan.pair ? 2 : 1;
-  const int tile_m = plan.pair ? 256 : 128;
+  const bool pair = plan.share == kPaired;
+  p.b_rows = MODE == kGated ? plan.w : pair ? plan.w / 2 : plan.w;
+  p.b_boxes = MODE == kGated && !pair ? 2 : 1;
+  p.splits = plan.splits;
+  const int tile_m = pair ? 256 : 128;
   int64_t rows = (32ll << 20) / (K * a.esize) / 256 * 256;  // a group's panel of A stays in L2 while B goes by
   rows = rows < 2048 ? 2048 : rows > 65536 ? 65536 : rows;
   p.group_m = static_cast<int>(rows / tile_m);
@@ -570,9 +718,20 @@ int run_linear(LinOperand a, LinOperand b, void* out, int64_t M, int64_t N, int6
   alignas(64) CUtensorMap map_a, map_b;
   if (!encode_rows(&map_a, a, dt, p.a_rows) || !encode_rows(&map_b, b, dt, p.b_rows)) return B200_EDRIVER;
   const int64_t tiles = ((M + tile_m - 1) / tile_m) * ((N + plan.w - 1) / plan.w);
+  const int stage_bytes = (p.a_rows + p.b_boxes * p.b_rows) * kSlabBytes;
+  // a tile to a CTA, room for four slabs and for its sums: half an SM is enough
+  const bool half = !pair && half_an_sm(per, plan.w, p.a_rows, plan.splits) && tiles * plan.splits <= 2 * kResident[plan.splits];
+  const int64_t slots = pair ? kNumSMs / 2 : half ? 2 * kNumSMs : kNumSMs, resident = tiles < slots ? tiles : slots;
+  p.ring = half ? kLinHalfRing : kLinRing;
+  p.stages = ring_stages(p.ring, stage_bytes);
+  p.acc_cols = 256;
+  p.accs = half ? 1 : 2;
+  p.early = half ? 1 : 0;
   auto go = [&](auto* o) {
     using TO = std::remove_pointer_t<decltype(o)>;
-    return plan.pair ? launch_linear(linear_tc<MODE, TO, true>, true, tiles, st, map_a, map_b, o, p, status) : launch_linear(linear_tc<MODE, TO, false>, false, tiles, st, map_a, map_b, o, p, status);
+    if (pair) return launch_linear(linear_tc<MODE, TO, kPaired>, 2, 2 * resident, st, map_a, map_b, o, p, status);
+    if (plan.share == kSplit) return launch_linear(linear_tc<MODE, TO, kSplit>, plan.splits, tiles * plan.splits, st, map_a, map_b, o, p, status);
+    return launch_linear(linear_tc<MODE, TO, kSingle>, 1, resident, st, map_a, map_b, o, p, status);
   };
   int rc;
   if (dtype_out == B200_BF16) rc = go(static_cast<__nv_bfloat16*>(out));
