@@ -27,6 +27,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
+#include <atomic>
+
 #include "../../include/b200ops.h"
 
 namespace {

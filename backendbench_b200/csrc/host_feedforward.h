@@ -83,6 +83,32 @@ template <typename... A> PyObject* wrapper(int op, const A&... a) {
 void ff_launched(bool ok) {
   if (!ok) raise_python();
 }
+// The lock is needed to look whether a call is direct and nowhere else on its way: where the entry point launches and returns, it
+// is held for that look alone.
+bool ff_direct(int op) {
+  Gil gil;
+  return ff_ops[op].direct();
+}
+void ff_check(int rc, const char* what) {
+  if (rc == 0) return;
+  Gil gil;
+  PyObject* r = PyObject_CallFunction(check_fn, "is", rc, what);  // raises
+  Py_XDECREF(r);
+  if (!PyErr_Occurred()) PyErr_Format(PyExc_RuntimeError, "%s failed with code %d", what, rc);
+  raise_python();
+}
+uint32_t* ff_status(const Tensor& t) {
+  static std::atomic<uint32_t*> words[64];
+  const size_t d = static_cast<size_t>(t.get_device());
+  uint32_t* w = d < 64 ? words[d].load(std::memory_order_acquire) : nullptr;
+  if (w) return w;
+  Gil gil;
+  w = status_word(t);
+  if (!w) raise_python();
+  if (d < 64) words[d].store(w, std::memory_order_release);
+  return w;
+}
+Tensor ff_scratch(const Tensor& like, int64_t bytes) { return bytes > 0 ? new_tensor({bytes}, at::kByte, like) : Tensor(); }
 
 int activation_code(c10::string_view name) {
   constexpr const char* kNames[B200_ACT_COUNT] = {"silu", "gelu", "gelu_tanh", "relu", "sigmoid"};
@@ -122,6 +148,7 @@ std::tuple<Tensor, Tensor> gated_direct(const Tensor& x, const Tensor& w, c10::s
   if (r.M == 0 || F == 0 || r.K == 0) return {};
   Tensor projections;
   if (dt(x) == B200_F32) {
+    Gil gil;
     PyObject* p = gemm(Operand{x, 0, r.s_m, r.s_k}, Operand{w, 0, w.stride(1), w.stride(0)}, Tensor(), 1, r.M, 2 * F, r.K, 1.0, 0.0, with_last(x, 2 * F));
     if (!p) raise_python();
     projections = taken(p);
@@ -129,32 +156,29 @@ std::tuple<Tensor, Tensor> gated_direct(const Tensor& x, const Tensor& w, c10::s
     ff_launched(launched("b200_gate", [&, st = stream()] { return api.b200_gate(static_cast<const float*>(ptr(projections)), static_cast<float*>(ptr(out)), r.M, F, act, st); }));
     return {out, projections};
   }
-  uint32_t* status = status_word(x);
-  if (!status) raise_python();
   Tensor out = new_tensor(with_last(x, F), x.scalar_type(), x);
   if (keep) projections = new_tensor(with_last(x, 2 * F), at::kFloat, x);
   const int64_t ws0 = w.stride(0), ws1 = w.stride(1), need = api.b200_gated_linear_scratch_bytes(ptr(x), ptr(w), r.M, F, r.K, r.s_m, r.s_k, ws0, ws1);
-  Scratch s(x, need);
-  ff_launched(launched("b200_gated_linear", [&, st = stream()] {
-    return api.b200_gated_linear(ptr(x), ptr(w), ptr(out), static_cast<float*>(ptr(projections)), r.M, F, r.K, r.s_m, r.s_k, ws0, ws1, act, dt(x), s.data(), need, status, st);
-  }));
+  const Tensor s = ff_scratch(x, need);
+  ff_check(api.b200_gated_linear(ptr(x), ptr(w), ptr(out), static_cast<float*>(ptr(projections)), r.M, F, r.K, r.s_m, r.s_k, ws0, ws1, act, dt(x), ptr(s), need, ff_status(x), stream()),
+           "b200_gated_linear");
   return {out, projections};
 }
 
 Tensor ff_gated_linear(const Tensor& x, const Tensor& w, c10::string_view activation) {
-  Gil gil;
-  if (ff_ops[kFfGated].direct()) {
+  if (ff_direct(kFfGated)) {
     Tensor out = std::get<0>(gated_direct(x, w, activation, false));
     if (out.defined()) return out;
   }
+  Gil gil;
   return taken(wrapper(kFfGated, x, w, activation));
 }
 std::tuple<Tensor, Tensor> ff_gated_linear_train(const Tensor& x, const Tensor& w, c10::string_view activation) {
-  Gil gil;
-  if (ff_ops[kFfGatedTrain].direct()) {
+  if (ff_direct(kFfGatedTrain)) {
     auto out = gated_direct(x, w, activation, true);
     if (std::get<0>(out).defined()) return out;
   }
+  Gil gil;
   return taken_pair(wrapper(kFfGatedTrain, x, w, activation));
 }
 std::tuple<TensorOpt, TensorOpt> ff_gated_linear_backward(const Tensor& g, const Tensor& x, const Tensor& w, const Tensor& p, c10::string_view activation, std::array<bool, 2> mask) {
@@ -192,34 +216,34 @@ Tensor dropout_direct(const Tensor& x, double p, const Tensor& state, const Tens
       (residual.defined() && (residual.scalar_type() != x.scalar_type() || residual.sizes() != x.sizes() || !residual.is_contiguous())) || !plain(x, state, residual))
     return {};
   Tensor out = new_like(x);
-  ff_launched(launched("b200_dropout", [&, st = stream()] { return api.b200_dropout(ptr(x), ptr(residual), ptr(out), x.numel(), p, static_cast<const int64_t*>(ptr(state)), subsequence, dt(x), st); }));
+  ff_check(api.b200_dropout(ptr(x), ptr(residual), ptr(out), x.numel(), p, static_cast<const int64_t*>(ptr(state)), subsequence, dt(x), stream()), "b200_dropout");
   return out;
 }
 Tensor ff_dropout(const Tensor& x, double p, const Tensor& state, const TensorOpt& residual, int64_t subsequence) {
-  Gil gil;
-  if (ff_ops[kFfDropout].direct()) {
+  if (ff_direct(kFfDropout)) {
     Tensor out = dropout_direct(x, p, state, residual ? *residual : Tensor(), subsequence);
     if (out.defined()) return out;
   }
+  Gil gil;
   return taken(wrapper(kFfDropout, x, p, state, residual, Named<int64_t>{"subsequence", subsequence}));
 }
 Tensor ff_dropout_backward(const Tensor& g, double p, const Tensor& state, int64_t subsequence) {
-  Gil gil;
-  if (ff_ops[kFfDropoutBackward].direct()) {
+  if (ff_direct(kFfDropoutBackward)) {
     Tensor out = dropout_direct(g, p, state, Tensor(), subsequence);
     if (out.defined()) return out;
   }
+  Gil gil;
   return taken(wrapper(kFfDropoutBackward, g, p, state, Named<int64_t>{"subsequence", subsequence}));
 }
 
 std::tuple<Tensor, Tensor> ff_quantize_rows(const Tensor& x) {
-  Gil gil;
   Rows r;
-  if (ff_ops[kFfQuantize].direct() && floating(x) && r.of(x) && r.s_k == 1 && x.numel() && plain(x)) {
+  if (ff_direct(kFfQuantize) && floating(x) && r.of(x) && r.s_k == 1 && x.numel() && plain(x)) {
     Tensor q = new_tensor(x.sizes(), at::kChar, x), scale = new_tensor(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
-    ff_launched(launched("b200_quantize_rows", [&, st = stream()] { return api.b200_quantize_rows(ptr(x), ptr(q), static_cast<float*>(ptr(scale)), r.M, r.K, r.s_m, dt(x), st); }));
+    ff_check(api.b200_quantize_rows(ptr(x), ptr(q), static_cast<float*>(ptr(scale)), r.M, r.K, r.s_m, dt(x), stream()), "b200_quantize_rows");
     return {q, scale};
   }
+  Gil gil;
   return taken_pair(wrapper(kFfQuantize, x));
 }
 
@@ -227,24 +251,21 @@ bool scale_of(const Tensor& t, int64_t n, bool column) {
   return t.scalar_type() == at::kFloat && t.is_contiguous() && ((t.dim() == 1 && t.size(0) == n) || (t.dim() == 2 && t.size(column ? 0 : 1) == n && t.size(column ? 1 : 0) == 1));
 }
 Tensor ff_mm_int8(const Tensor& a, const Tensor& b, const Tensor& sa, const Tensor& sb, const TensorOpt& bias, std::optional<at::ScalarType> out_dtype) {
-  Gil gil;
   const Tensor none, &c = bias ? *bias : none;
   const at::ScalarType type = out_dtype ? *out_dtype : c.defined() ? c.scalar_type() : at::kBFloat16;
-  if (ff_ops[kFfInt8].direct() && a.dim() == 2 && b.dim() == 2 && a.size(1) == b.size(0) && a.numel() && b.numel() && a.size(1) <= B200_INT8_MAX_K && a.scalar_type() == at::kChar &&
+  if (ff_direct(kFfInt8) && a.dim() == 2 && b.dim() == 2 && a.size(1) == b.size(0) && a.numel() && b.numel() && a.size(1) <= B200_INT8_MAX_K && a.scalar_type() == at::kChar &&
       b.scalar_type() == at::kChar && scale_of(sa, a.size(0), true) && scale_of(sb, b.size(1), false) && (type == at::kFloat || type == at::kHalf || type == at::kBFloat16) &&
       (!c.defined() || (c.scalar_type() == type && c.dim() == 1 && c.size(0) == b.size(1) && c.is_contiguous())) && plain(a, b, sa, sb, c)) {
     const int64_t M = a.size(0), K = a.size(1), N = b.size(1), s[4] = {a.stride(0), a.stride(1), b.stride(0), b.stride(1)};
-    uint32_t* status = status_word(a);
-    if (!status) raise_python();
     Tensor out = new_tensor({M, N}, type, a);
     const int64_t need = api.b200_mm_int8_scratch_bytes(ptr(a), ptr(b), M, N, K, s[0], s[1], s[2], s[3]);
-    Scratch scratch(a, need);
-    ff_launched(launched("b200_mm_int8", [&, st = stream()] {
-      return api.b200_mm_int8(ptr(a), ptr(b), static_cast<const float*>(ptr(sa)), static_cast<const float*>(ptr(sb)), ptr(c), ptr(out), M, N, K, s[0], s[1], s[2], s[3], dt(out), scratch.data(), need,
-                              status, st);
-    }));
+    const Tensor scratch = ff_scratch(a, need);
+    ff_check(api.b200_mm_int8(ptr(a), ptr(b), static_cast<const float*>(ptr(sa)), static_cast<const float*>(ptr(sb)), ptr(c), ptr(out), M, N, K, s[0], s[1], s[2], s[3], dt(out), ptr(scratch), need,
+                              ff_status(a), stream()),
+             "b200_mm_int8");
     return out;
   }
+  Gil gil;
   return taken(wrapper(kFfInt8, a, b, sa, sb, bias, Named<std::optional<at::ScalarType>>{"out_dtype", out_dtype}));
 }
 
@@ -254,6 +275,8 @@ bool wants_gradient(const Tensor& a, const Tensor& b) {
   auto of = [](const Tensor& t) { return t.defined() && ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined()); };
   return of(a) || of(b);
 }
+// Plain tensors would come to the CUDA kernel by the dispatcher, too
+bool straight(const Tensor& a, const Tensor& b) { return !a.requires_grad() && !b.requires_grad() && plain(a, b); }
 template <typename F> auto below(const char* name) { return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>(); }
 
 Tensor ff_gated_linear_autograd(const Tensor& x, const Tensor& w, c10::string_view activation) {
@@ -261,6 +284,7 @@ Tensor ff_gated_linear_autograd(const Tensor& x, const Tensor& w, c10::string_vi
     Gil gil;
     return taken(in_python(ff_ops[kFfGated].autograd, x, w, activation));
   }
+  if (straight(x, w)) return ff_gated_linear(x, w, activation);
   static const auto op = below<Tensor(const Tensor&, const Tensor&, c10::string_view)>("b200::gated_linear");
   at::AutoDispatchBelowAutograd guard;
   return op.call(x, w, activation);
@@ -270,6 +294,7 @@ std::tuple<Tensor, Tensor> ff_gated_linear_train_autograd(const Tensor& x, const
     Gil gil;
     return taken_pair(in_python(ff_ops[kFfGatedTrain].autograd, x, w, activation));
   }
+  if (straight(x, w)) return ff_gated_linear_train(x, w, activation);
   static const auto op = below<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, c10::string_view)>("b200::gated_linear_train");
   at::AutoDispatchBelowAutograd guard;
   return op.call(x, w, activation);
@@ -279,6 +304,7 @@ Tensor ff_dropout_autograd(const Tensor& x, double p, const Tensor& state, const
     Gil gil;
     return taken(in_python(ff_ops[kFfDropout].autograd, x, p, state, residual, Named<int64_t>{"subsequence", subsequence}));
   }
+  if (straight(x, state) && (!residual || straight(*residual, state))) return ff_dropout(x, p, state, residual, subsequence);
   static const auto op = below<Tensor(const Tensor&, double, const Tensor&, const TensorOpt&, int64_t)>("b200::dropout");
   at::AutoDispatchBelowAutograd guard;
   return op.call(x, p, state, residual, subsequence);

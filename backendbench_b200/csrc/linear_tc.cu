@@ -20,6 +20,7 @@
 // rows as there are; the MMA's other rows multiply whatever lies behind it and are never stored.
 #include <cuda.h>
 
+#include <atomic>
 #include <cmath>
 
 #include "b200_common.cuh"
@@ -666,9 +667,17 @@ LinPlan plan_linear(int64_t M, int64_t N, int64_t K, int per, int k_step) {
   return s.plan;
 }
 
-template <typename Kernel, typename TO>
-int launch_linear(Kernel kernel, int cluster, int64_t ctas, cudaStream_t st, const CUtensorMap& map_a, const CUtensorMap& map_b, TO* out, const LinParams& p, uint32_t* status) {
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lin_smem(kLinRing)));
+template <int MODE, typename TO, int SHARE>
+int launch_linear(int cluster, int64_t ctas, cudaStream_t st, const CUtensorMap& map_a, const CUtensorMap& map_b, TO* out, const LinParams& p, uint32_t* status) {
+  const auto kernel = linear_tc<MODE, TO, SHARE>;
+  static std::atomic<uint64_t> allowed{0};  // devices on which this kernel may have that much shared memory (0.4 us a call to say so each time)
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (e == cudaSuccess && !(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lin_smem(kLinRing)));
+    if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
   if (e != cudaSuccess) { set_last_cuda_error(e); return B200_ELAUNCH; }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
@@ -729,9 +738,9 @@ int run_linear(LinOperand a, LinOperand b, void* out, int64_t M, int64_t N, int6
   p.early = half ? 1 : 0;
   auto go = [&](auto* o) {
     using TO = std::remove_pointer_t<decltype(o)>;
-    if (pair) return launch_linear(linear_tc<MODE, TO, kPaired>, 2, 2 * resident, st, map_a, map_b, o, p, status);
-    if (plan.share == kSplit) return launch_linear(linear_tc<MODE, TO, kSplit>, plan.splits, tiles * plan.splits, st, map_a, map_b, o, p, status);
-    return launch_linear(linear_tc<MODE, TO, kSingle>, 1, resident, st, map_a, map_b, o, p, status);
+    if (pair) return launch_linear<MODE, TO, kPaired>(2, 2 * resident, st, map_a, map_b, o, p, status);
+    if (plan.share == kSplit) return launch_linear<MODE, TO, kSplit>(plan.splits, tiles * plan.splits, st, map_a, map_b, o, p, status);
+    return launch_linear<MODE, TO, kSingle>(1, resident, st, map_a, map_b, o, p, status);
   };
   int rc;
   if (dtype_out == B200_BF16) rc = go(static_cast<__nv_bfloat16*>(out));
