@@ -15,71 +15,103 @@ constexpr int kFfThreads = 256;
 // h = act(g) * u of fp32 projections P = [g | u] (M x 2 N). fp32 products come in two steps (their sums are
 // put together from six plane products over several launches), so the gate has a kernel of its own there.
 // Backward: dP = [dh * u * act'(g) | dh * act(g)], rounded to the type of the operands it is multiplied by next.
-// VEC elements to a thread: whole vectors of every operand where rows are on the grid, else one.
 template <int N> __device__ __forceinline__ void load_f32(const float* p, float* v) {
-  if constexpr (N % 4 == 0) {
 #pragma unroll
-    for (int e = 0; e < N; e += 4) widen<float>(ld_stream(p + e), v + e);
-  } else {
-    v[0] = p[0];
-  }
+  for (int e = 0; e < N; e += 4) widen<float>(ld_stream(p + e), v + e);
+}
+__device__ __forceinline__ int64_t row_of(int64_t i, int64_t per_row, int64_t total) {
+  return total <= 0xffff0000ll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(per_row) : i / per_row;  // (i may run past total, by less than four CTAs' worth)
 }
 
-template <typename ACT, int VEC>
+// Rows off the grid: four single elements to a thread, a CTA's width apart and all on their way together (fp32 1531 x 1365 11.1 us
+// with one).
+template <typename ACT, bool VECTOR>
 __global__ void __launch_bounds__(kFfThreads) gate_forward(const float* p, float* __restrict__ h, int64_t M, int64_t N) {
-  const int64_t per_row = N / VEC, total = M * per_row;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kFfThreads) {
-    const int64_t m = total <= 0xffffffffll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(per_row) : i / per_row;
-    const float* row = p + i * VEC + m * N;  // m rows of 2 N, not N, lie before
-    float g[VEC], u[VEC];
-    load_f32<VEC>(row, g);
-    load_f32<VEC>(row + N, u);
+  if constexpr (VECTOR) {
+    const int64_t per_row = N / 4, total = M * per_row;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kFfThreads) {
+      const int64_t m = row_of(i, per_row, total);
+      const float* row = p + i * 4 + m * N;  // m rows of 2 N, not N, lie before
+      float g[4], u[4];
+      load_f32<4>(row, g);
+      load_f32<4>(row + N, u);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) g[e] = ACT::template f<false>(g[e]) * u[e];
-    if constexpr (VEC > 1) *reinterpret_cast<uint4*>(h + i * VEC) = narrow<float>(g);
-    else h[i] = g[0];
+      for (int e = 0; e < 4; ++e) g[e] = ACT::template f<false>(g[e]) * u[e];
+      *reinterpret_cast<uint4*>(h + i * 4) = narrow<float>(g);
+    }
+  } else {
+    const int64_t total = M * N;
+    for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * (4 * kFfThreads) + threadIdx.x; i0 < total; i0 += static_cast<int64_t>(gridDim.x) * (4 * kFfThreads)) {
+      float g[4], u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t i = i0 + e * kFfThreads, at = i + row_of(i, N, total) * N;
+        g[e] = i < total ? p[at] : 0.f;
+        u[e] = i < total ? p[at + N] : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i0 + e * kFfThreads < total) h[i0 + e * kFfThreads] = ACT::template f<false>(g[e]) * u[e];
+    }
   }
 }
 
-template <typename T, typename ACT, int VEC>
+template <typename T, typename ACT, bool VECTOR>
 __global__ void __launch_bounds__(kFfThreads) gate_backward(const T* dh, const float* p, T* __restrict__ dp, int64_t M, int64_t N) {
-  const int64_t per_row = N / VEC, total = M * per_row;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kFfThreads) {
-    const int64_t m = total <= 0xffffffffll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(per_row) : i / per_row;
-    const int64_t at = i * VEC + m * N;
-    float d[VEC], g[VEC], u[VEC];
-    if constexpr (VEC > 1) widen<T>(ld_stream(dh + i * VEC), d);
-    else d[0] = to_f32(dh[i]);
-    load_f32<VEC>(p + at, g);
-    load_f32<VEC>(p + at + N, u);
+  constexpr int kVec = VECTOR ? 16 / static_cast<int>(sizeof(T)) : 4;
+  auto slope = [](float& d, float& g, float& u) {
+    float a, s;
+    ACT::template both<sizeof(T) == 2>(g, a, s);
+    g = d * u * s;
+    u = d * a;
+  };
+  float d[kVec], g[kVec], u[kVec];
+  if constexpr (VECTOR) {
+    const int64_t per_row = N / kVec, total = M * per_row;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kFfThreads) {
+      const int64_t at = i * kVec + row_of(i, per_row, total) * N;
+      widen<T>(ld_stream(dh + i * kVec), d);
+      load_f32<kVec>(p + at, g);
+      load_f32<kVec>(p + at + N, u);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      float a, s;
-      ACT::template both<sizeof(T) == 2>(g[e], a, s);
-      g[e] = d[e] * u[e] * s;
-      u[e] = d[e] * a;
-    }
-    if constexpr (VEC > 1) {  // (both products read it next: not streamed past L2)
-      *reinterpret_cast<uint4*>(dp + at) = narrow<T>(g);
+      for (int e = 0; e < kVec; ++e) slope(d[e], g[e], u[e]);
+      *reinterpret_cast<uint4*>(dp + at) = narrow<T>(g);  // (both products read it next: not streamed past L2)
       *reinterpret_cast<uint4*>(dp + at + N) = narrow<T>(u);
-    } else {
-      dp[at] = from_f32<T>(g[0]);
-      dp[at + N] = from_f32<T>(u[0]);
+    }
+  } else {
+    const int64_t total = M * N;
+    for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * (4 * kFfThreads) + threadIdx.x; i0 < total; i0 += static_cast<int64_t>(gridDim.x) * (4 * kFfThreads)) {
+      int64_t at[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t i = i0 + e * kFfThreads;
+        at[e] = i + row_of(i, N, total) * N;
+        d[e] = i < total ? to_f32(dh[i]) : 0.f;
+        g[e] = i < total ? p[at[e]] : 0.f;
+        u[e] = i < total ? p[at[e] + N] : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (i0 + e * kFfThreads >= total) break;
+        slope(d[e], g[e], u[e]);
+        dp[at[e]] = from_f32<T>(g[e]);
+        dp[at[e] + N] = from_f32<T>(u[e]);
+      }
     }
   }
 }
 
 inline int ff_grid(int64_t items) {
   const int64_t b = (items + kFfThreads - 1) / kFfThreads, most = kNumSMs * 16LL;
-  return static_cast<int>(b < most ? b : most);
+  return static_cast<int>(b < 1 ? 1 : b < most ? b : most);
 }
 
 int launch_gate(const float* p, float* out, int64_t M, int64_t N, int act, cudaStream_t st) {
   const bool vec = N % 4 == 0 && aligned16(p) && aligned16(out);
-  const int grid = ff_grid(M * N / (vec ? 4 : 1));
+  const int grid = ff_grid(M * N / 4);
   gate_act_each(act, [&](auto a) {
-    if (vec) gate_forward<decltype(a), 4><<<grid, kFfThreads, 0, st>>>(p, out, M, N);
-    else gate_forward<decltype(a), 1><<<grid, kFfThreads, 0, st>>>(p, out, M, N);
+    if (vec) gate_forward<decltype(a), true><<<grid, kFfThreads, 0, st>>>(p, out, M, N);
+    else gate_forward<decltype(a), false><<<grid, kFfThreads, 0, st>>>(p, out, M, N);
   });
   return check_launch();
 }
@@ -87,10 +119,10 @@ int launch_gate(const float* p, float* out, int64_t M, int64_t N, int act, cudaS
 template <typename T> int launch_gate_backward(const void* dh, const float* p, void* out, int64_t M, int64_t N, int act, cudaStream_t st) {
   constexpr int kVec = 16 / sizeof(T);
   const bool vec = N % kVec == 0 && aligned16(p) && aligned16(out) && aligned16(dh);
-  const int grid = ff_grid(M * N / (vec ? kVec : 1));
+  const int grid = ff_grid(M * N / (vec ? kVec : 4));
   gate_act_each(act, [&](auto a) {
-    if (vec) gate_backward<T, decltype(a), kVec><<<grid, kFfThreads, 0, st>>>(static_cast<const T*>(dh), p, static_cast<T*>(out), M, N);
-    else gate_backward<T, decltype(a), 1><<<grid, kFfThreads, 0, st>>>(static_cast<const T*>(dh), p, static_cast<T*>(out), M, N);
+    if (vec) gate_backward<T, decltype(a), true><<<grid, kFfThreads, 0, st>>>(static_cast<const T*>(dh), p, static_cast<T*>(out), M, N);
+    else gate_backward<T, decltype(a), false><<<grid, kFfThreads, 0, st>>>(static_cast<const T*>(dh), p, static_cast<T*>(out), M, N);
   });
   return check_launch();
 }

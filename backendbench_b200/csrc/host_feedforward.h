@@ -139,6 +139,24 @@ at::DimVector with_last(const Tensor& t, int64_t last) {
   return s;
 }
 
+// (with the lock held) a @ b as feedforward._product forms it
+constexpr int64_t kF32Range = 4096;  // F32_RANGE
+Tensor ff_product(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t K, at::IntArrayRef shape) {
+  Tensor out;
+  const int64_t step = dt(a.t) == B200_F32 && K > kF32Range ? kF32Range : K;
+  for (int64_t k = 0; k < K; k += step) {
+    Operand x = a, y = b;
+    if (k) {
+      x.t = a.t.as_strided({1}, {1}, a.t.storage_offset() + k * a.col);  // (its data pointer is what counts)
+      y.t = b.t.as_strided({1}, {1}, b.t.storage_offset() + k * b.row);
+    }
+    PyObject* r = gemm(x, y, out.defined() ? out.view({M, N}) : Tensor(), 1, M, N, std::min(step, K - k), 1.0, out.defined() ? 1.0 : 0.0, shape);
+    if (!r) raise_python();
+    out = taken(r);
+  }
+  return out;
+}
+
 // (output, projections); an undefined output: the wrapper has to take the call
 std::tuple<Tensor, Tensor> gated_direct(const Tensor& x, const Tensor& w, c10::string_view activation, bool keep) {
   Rows r;
@@ -149,9 +167,7 @@ std::tuple<Tensor, Tensor> gated_direct(const Tensor& x, const Tensor& w, c10::s
   Tensor projections;
   if (dt(x) == B200_F32) {
     Gil gil;
-    PyObject* p = gemm(Operand{x, 0, r.s_m, r.s_k}, Operand{w, 0, w.stride(1), w.stride(0)}, Tensor(), 1, r.M, 2 * F, r.K, 1.0, 0.0, with_last(x, 2 * F));
-    if (!p) raise_python();
-    projections = taken(p);
+    projections = ff_product(Operand{x, 0, r.s_m, r.s_k}, Operand{w, 0, w.stride(1), w.stride(0)}, r.M, 2 * F, r.K, with_last(x, 2 * F));
     Tensor out = new_tensor(with_last(x, F), x.scalar_type(), x);
     ff_launched(launched("b200_gate", [&, st = stream()] { return api.b200_gate(static_cast<const float*>(ptr(projections)), static_cast<float*>(ptr(out)), r.M, F, act, st); }));
     return {out, projections};
@@ -192,16 +208,8 @@ std::tuple<TensorOpt, TensorOpt> ff_gated_linear_backward(const Tensor& g, const
       Tensor dp = new_tensor({r.M, 2 * F}, x.scalar_type(), x);
       ff_launched(launched("b200_gate_backward", [&, st = stream()] { return api.b200_gate_backward(ptr(g), static_cast<const float*>(ptr(p)), ptr(dp), r.M, F, act, dt(x), st); }));
       std::tuple<TensorOpt, TensorOpt> out;
-      if (mask[0]) {
-        PyObject* dx = gemm(Operand{dp, 0, 2 * F, 1}, Operand{w, 0, w.stride(0), w.stride(1)}, Tensor(), 1, r.M, r.K, 2 * F, 1.0, 0.0, x.sizes());
-        if (!dx) raise_python();
-        std::get<0>(out) = taken(dx);
-      }
-      if (mask[1]) {
-        PyObject* dw = gemm(Operand{dp, 0, 1, 2 * F}, Operand{x, 0, r.s_m, r.s_k}, Tensor(), 1, 2 * F, r.K, r.M, 1.0, 0.0, w.sizes());
-        if (!dw) raise_python();
-        std::get<1>(out) = taken(dw);
-      }
+      if (mask[0]) std::get<0>(out) = ff_product(Operand{dp, 0, 2 * F, 1}, Operand{w, 0, w.stride(0), w.stride(1)}, r.M, r.K, 2 * F, x.sizes());
+      if (mask[1]) std::get<1>(out) = ff_product(Operand{dp, 0, 1, 2 * F}, Operand{x, 0, r.s_m, r.s_k}, 2 * F, r.K, r.M, w.sizes());
       return out;
     }
   }
@@ -276,7 +284,11 @@ bool wants_gradient(const Tensor& a, const Tensor& b) {
   return of(a) || of(b);
 }
 // Plain tensors would come to the CUDA kernel by the dispatcher, too
-bool straight(const Tensor& a, const Tensor& b) { return !a.requires_grad() && !b.requires_grad() && plain(a, b); }
+bool straight(const Tensor& a, const Tensor& b) {
+  const auto tls = c10::impl::tls_local_dispatch_key_set();
+  if (((a.key_set() | b.key_set() | tls.included_) - tls.excluded_).has_any(c10::python_ks)) return false;  // (fake tensors, where there may be no device to ask)
+  return !a.requires_grad() && !b.requires_grad() && plain(a, b);
+}
 template <typename F> auto below(const char* name) { return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>(); }
 
 Tensor ff_gated_linear_autograd(const Tensor& x, const Tensor& w, c10::string_view activation) {

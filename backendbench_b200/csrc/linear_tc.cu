@@ -22,6 +22,8 @@
 
 #include <atomic>
 #include <cmath>
+#include <type_traits>
+#include <utility>
 
 #include "b200_common.cuh"
 #include "gate_act.cuh"
@@ -102,6 +104,30 @@ template <typename V> __device__ __forceinline__ V ld_cluster(uint32_t from) {
   return *reinterpret_cast<const V*>(&v);
 }
 
+// What is staged (see lin_store) to rows off the grid: a column to a lane, eight rows on their way together. (A call, so that
+// its registers are not the epilogue's.)
+template <typename TO> __device__ __noinline__ void lin_copy_ragged(const unsigned char* mine, TO* out, int64_t pitch, int nrows, int ncols, int lane) {
+  constexpr int kRow = 32 * static_cast<int>(sizeof(TO)), kPieces = kRow / 16, kPer = 16 / static_cast<int>(sizeof(TO)), kShift = sizeof(TO) == 2 ? 1 : 0;
+  const unsigned char* from = mine + lane % kPer * static_cast<int>(sizeof(TO));
+  const int j = lane / kPer;
+  out += lane;
+  auto rows = [&](int r0, auto whole) {
+    TO w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const TO*>(from + i * kRow + ((j ^ ((i >> kShift) & (kPieces - 1))) << 4));
+#pragma unroll
+    for (int i = 0; i < 8; ++i, out += pitch)
+      if (decltype(whole)::value || (lane < ncols && r0 + i < nrows)) *out = w[i];
+  };
+  if (nrows >= 32 && ncols >= 32) {
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += 8, from += 8 * kRow) rows(r0, std::true_type{});
+  } else {
+#pragma unroll 1
+    for (int r0 = 0; r0 < nrows; r0 += 8, from += 8 * kRow) rows(r0, std::false_type{});
+  }
+}
+
 // 32 values of a lane's row to 32 columns of `out` (row pitch `pitch`, column 0 at `col`): rounded once into the warp's
 // staging buffer (16-byte pieces swizzled so that neither side meets a bank twice), then out in 16-byte pieces of
 // eight (fp32: four) rows at a time, or element by element where rows are off the grid.
@@ -116,32 +142,62 @@ __device__ __forceinline__ void lin_store(const float* v, unsigned char* mine, T
     constexpr int kRowsAt = 32 / kPieces;
     const int j = lane % kPieces, r0 = lane / kPieces;
     if (j * kPer < ncols) {
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < kPieces; ++i) {
         const int r = r0 + i * kRowsAt;
         if (r < nrows) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * pitch + j * kPer) = *reinterpret_cast<const uint4*>(mine + r * kRow + ((j ^ ((r >> kShift) & (kPieces - 1))) << 4));
       }
     }
-  } else if (lane < ncols) {
-    const int j = lane / kPer, e = lane % kPer;
-    for (int r = 0; r < nrows; ++r) out[static_cast<int64_t>(r) * pitch + lane] = *(reinterpret_cast<const TO*>(mine + r * kRow + ((j ^ ((r >> kShift) & (kPieces - 1))) << 4)) + e);
+  } else {
+    lin_copy_ragged<TO>(mine, out, pitch, nrows, ncols, lane);
   }
 }
 
-// One output of a sum (gated: of both) and where it goes
-template <int MODE, typename TO> __device__ __forceinline__ void lin_out(const LinParams& p, TO* out, const float* a_scale, const float* b_scale, const TO* bias, int64_t m, int64_t n, float g, float u) {
+// Four outputs of a row, from sums (gated: of both projections), and where they go
+template <int MODE, typename TO>
+__device__ __forceinline__ void lin_out(const LinParams& p, TO* out, const float* a_scale, const float* b_scale, const TO* bias, int64_t m, int64_t n, const float* g, const float* u, bool vec) {
+  float v[4];
+  const int left = p.N - n < 4 ? static_cast<int>(p.N - n) : 4;
   if constexpr (MODE == kInt8) {
-    float v = g * a_scale[m] * b_scale[n];
-    if (bias) v += to_f32(bias[n]);
-    out[m * p.N + n] = from_f32<TO>(v);
-  } else {
-    if (p.side) {
-      p.side[m * 2 * p.N + n] = g;
-      p.side[m * 2 * p.N + p.N + n] = u;
+    const float sa = a_scale[m];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = e < left ? g[e] * sa * b_scale[n + e] : 0.f;
+      if (bias && e < left) v[e] += to_f32(bias[n + e]);
     }
-    float h = 0.f;
-    gate_act_each(p.act, [&](auto act) { h = act.fast(g) * u; });
-    out[m * p.N + n] = from_f32<TO>(h);
+  } else {
+    gate_act_each(p.act, [&](auto act) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = act.fast(g[e]) * u[e];
+    });
+    if (p.side) {
+      float* to = p.side + m * 2 * p.N + n;
+      if (vec) {
+        *reinterpret_cast<uint4*>(to) = narrow<float>(g);
+        *reinterpret_cast<uint4*>(to + p.N) = narrow<float>(u);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < left) {
+            to[e] = g[e];
+            to[p.N + e] = u[e];
+          }
+      }
+    }
+  }
+  TO* to = out + m * p.N + n;
+  if (vec) {
+    if constexpr (sizeof(TO) == 4) {
+      *reinterpret_cast<uint4*>(to) = narrow<float>(v);
+    } else {
+      const float w[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
+      const uint4 r = narrow<TO>(w);
+      *reinterpret_cast<uint2*>(to) = make_uint2(r.x, r.y);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) to[e] = from_f32<TO>(v[e]);
   }
 }
 
@@ -330,7 +386,6 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
     unsigned char* mine = epi_stage + (warp - 2) * kLinEpiBytes;
     constexpr int kPer = 16 / static_cast<int>(sizeof(TO)), kRegs = kI8 ? 32 : 64;
     const bool vec = p.N % kPer == 0 && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(p.side)) & 15u) == 0;
-    const bool scales_vec = kI8 && ((reinterpret_cast<uintptr_t>(p.b_scale) | reinterpret_cast<uintptr_t>(p.bias)) & 15u) == 0;  // (a chunk starts at a multiple of 16)
     const uint32_t tempty_target = kPair ? map_to_cta(tempty_bar(0), 0u) : 0u;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -342,6 +397,15 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
       const int wide = p.N - n0 < p.w ? static_cast<int>(p.N - n0) : p.w;  // columns of this tile that exist
       const int nrows = p.M - mr0 < 32 ? static_cast<int>(p.M - mr0) : 32;  // <= 0: none
       const int chunks = (wide + 31) / 32, count = (chunks + 1 - half) / 2;  // this warp takes chunks half, half + 2, ...
+      float scale_next = 0.f, bias_next = 0.f;
+      auto ahead = [&](int64_t n, int left) {
+        if constexpr (kI8) {
+          scale_next = lane < left ? b_scale[n + lane] : 0.f;
+          bias_next = bias && lane < left ? to_f32(bias[n + lane]) : 0.f;
+        }
+      };
+      ahead(n0 + half * 32, wide - half * 32);
+      const float sa = kI8 && lane < nrows ? a_scale[mr0 + lane] : 0.f;
       int got = 0;
       if (lane == 0) got = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, kLinWaitNs) ? 1 : 0;
       got = __shfl_sync(0xffffffffu, got, 0);
@@ -395,35 +459,23 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
         float v[32];
         tc_ld_wait();
         if constexpr (kI8) {
-          const float sa = lane < nrows ? a_scale[mr0 + lane] : 0.f;
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = static_cast<float>(static_cast<int>(r[e])) * sa;
           next(i);
-          if (ncols == 32 && scales_vec) {
+          // this chunk's scales and bias, a column to a lane since the chunk before, to every lane by way of the staging buffer
+          float* shared = reinterpret_cast<float*>(mine);
+          __syncwarp();
+          shared[lane] = scale_next;
+          shared[32 + lane] = bias_next;
+          __syncwarp();
+          ahead(n + 64, wide - c0 - 64);
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const uint4 b = ld_keep_after(b_scale + n + e);
-              v[e] *= __uint_as_float(b.x);
-              v[e + 1] *= __uint_as_float(b.y);
-              v[e + 2] *= __uint_as_float(b.z);
-              v[e + 3] *= __uint_as_float(b.w);
-            }
-            if (bias) {
-#pragma unroll
-              for (int e = 0; e < 32; e += kPer) {
-                float b[kPer];
-                widen<TO>(ld_keep_after(bias + n + e), b);
-#pragma unroll
-                for (int j = 0; j < kPer; ++j) v[e + j] += b[j];
-              }
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const bool in = e < ncols;
-              v[e] *= in ? b_scale[n + e] : 0.f;
-              if (bias) v[e] += in ? to_f32(bias[n + e]) : 0.f;
-            }
+          for (int e = 0; e < 32; e += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(shared + e), c = *reinterpret_cast<const float4*>(shared + 32 + e);
+            v[e] = v[e] * b.x + c.x;
+            v[e + 1] = v[e + 1] * b.y + c.y;
+            v[e + 2] = v[e + 2] * b.z + c.z;
+            v[e + 3] = v[e + 3] * b.w + c.w;
           }
         } else {
           const float *g = reinterpret_cast<const float*>(r), *u = reinterpret_cast<const float*>(r + 32);
@@ -458,6 +510,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
     int mb, nb;
     lin_tile(tile_first, mt, nt, p.group_m, mb, nb);
     const int64_t mr0 = static_cast<int64_t>(mb) * 128, n0 = static_cast<int64_t>(nb) * p.w;
+    const bool quad_vec = p.N % 4 == 0 && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(p.side)) & 15u) == 0;
     const int rows = p.M - mr0 < p.a_rows ? static_cast<int>(p.M - mr0) : p.a_rows, units = rows * quads;
     for (int i = static_cast<int>(rank) * kLinThreads + static_cast<int>(threadIdx.x); i < units; i += p.splits * kLinThreads) {
       const int r = i / quads, c = (i - r * quads) * 4;
@@ -475,9 +528,12 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
           u[0] += w.x; u[1] += w.y; u[2] += w.z; u[3] += w.w;
         }
       }
+      if (n0 + c >= p.N) continue;
+      if constexpr (kI8) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n0 + c + e < p.N) lin_out<MODE, TO>(p, out, a_scale, b_scale, bias, mr0 + r, n0 + c + e, kI8 ? static_cast<float>(s[e]) : g[e], u[e]);
+        for (int e = 0; e < 4; ++e) g[e] = static_cast<float>(s[e]);
+      }
+      lin_out<MODE, TO>(p, out, a_scale, b_scale, bias, mr0 + r, n0 + c, g, u, quad_vec);
     }
     cluster_sync_all();  // nobody leaves while another reads its sums
   }
@@ -503,10 +559,23 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
 // Rows that lie along K, off the 16-byte grid: a thread to 16 bytes of the result, from the one or two aligned blocks that its bytes
 // lie in, shifted into place. A block holds a byte of the matrix or is not read, so that no load leaves the
 // 16-byte granules of the matrix itself. What lands behind a row's end is padding that the tensor map leaves out.
-__global__ void __launch_bounds__(256) pack_rows_shifted(const unsigned char* x, unsigned char* __restrict__ to, int64_t rows, int64_t row_bytes, int64_t s_bytes, uint32_t pieces) {
-  const int64_t total = rows * pieces;
-  const unsigned char* end = x + (rows - 1) * s_bytes + row_bytes;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
+// Both operands of a call that need it go in one launch, the first `blocks0` CTAs taking the one.
+struct PackRows {
+  const unsigned char* x;
+  unsigned char* to;
+  int64_t rows, row_bytes, s_bytes;
+  uint32_t pieces;  // of sixteen bytes to a row of the result
+};
+__global__ void __launch_bounds__(256) pack_rows_shifted(PackRows A, PackRows B, unsigned blocks0) {
+  next_grid_may_start();  // (the product's CTAs set themselves up meanwhile)
+  const bool second = blockIdx.x >= blocks0;
+  const PackRows& P = second ? B : A;
+  const unsigned char* x = P.x;
+  unsigned char* to = P.to;
+  const int64_t s_bytes = P.s_bytes, total = P.rows * P.pieces, step = static_cast<int64_t>(second ? gridDim.x - blocks0 : blocks0) * 256;
+  const uint32_t pieces = P.pieces;
+  const unsigned char* end = x + (P.rows - 1) * s_bytes + P.row_bytes;
+  for (int64_t i = static_cast<int64_t>(second ? blockIdx.x - blocks0 : blockIdx.x) * 256 + threadIdx.x; i < total; i += step) {
     const int64_t r = total <= 0xffffffffll ? static_cast<uint32_t>(i) / pieces : i / pieces;
     const int64_t j = i - r * pieces;
     const unsigned char* from = x + r * s_bytes + j * 16;
@@ -531,6 +600,7 @@ __global__ void __launch_bounds__(256) pack_rows_shifted(const unsigned char* x,
 template <typename E>
 __global__ void __launch_bounds__(256) pack_rows(const E* x, E* __restrict__ to, int64_t rows, int64_t K, int64_t s_r, int64_t s_k, int64_t pitch) {
   __shared__ E tile[32][33];
+  next_grid_may_start();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t kt = (K + 31) / 32, tiles = ((rows + 31) / 32) * kt;
   const bool along_k = s_r != 1;
@@ -558,28 +628,38 @@ struct LinOperand {
   int64_t packed_bytes() const { return ready() ? 0 : (rows * pitch() * esize + 255) / 256 * 256; }
 };
 
-int pack(LinOperand& o, unsigned char*& at, cudaStream_t st, int& launches) {
-  if (o.ready()) {
-    if (o.rows == 1) o.s_r = o.pitch();  // never used
-    return B200_OK;
-  }
+// The operands that are not ready are copied behind `at`, and the operands become their copies.
+void pack(LinOperand& a, LinOperand& b, unsigned char* at, cudaStream_t st, int& launches) {
   const int64_t most = kNumSMs * 8;
-  if (o.s_k == 1 || o.K == 1) {
-    const int64_t pieces = o.pitch() * o.esize / 16, blocks = (o.rows * pieces + 255) / 256;
-    pack_rows_shifted<<<static_cast<int>(blocks < most ? blocks : most), 256, 0, st>>>(static_cast<const unsigned char*>(o.base), at, o.rows, o.K * o.esize, o.s_r * o.esize, static_cast<uint32_t>(pieces));
-  } else {
-    const int64_t tiles = ((o.rows + 31) / 32) * ((o.K + 31) / 32);
-    const int grid = static_cast<int>(tiles < most ? tiles : most);
-    if (o.esize == 2) pack_rows<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(o.base), reinterpret_cast<uint16_t*>(at), o.rows, o.K, o.s_r, o.s_k, o.pitch());
-    else pack_rows<uint8_t><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(o.base), at, o.rows, o.K, o.s_r, o.s_k, o.pitch());
+  PackRows rows[2] = {};
+  unsigned blocks[2] = {};
+  int n = 0;
+  for (LinOperand* o : {&a, &b}) {
+    if (o->ready()) {
+      if (o->rows == 1) o->s_r = o->pitch();  // never used
+      continue;
+    }
+    const int64_t pitch = o->pitch(), bytes = o->packed_bytes();
+    if (o->s_k == 1 || o->K == 1) {
+      const int64_t pieces = pitch * o->esize / 16, needed = (o->rows * pieces + 255) / 256;
+      rows[n] = PackRows{static_cast<const unsigned char*>(o->base), at, o->rows, o->K * o->esize, o->s_r * o->esize, static_cast<uint32_t>(pieces)};
+      blocks[n++] = static_cast<unsigned>(needed < most ? needed : most);
+    } else {
+      const int64_t tiles = ((o->rows + 31) / 32) * ((o->K + 31) / 32);
+      const int grid = static_cast<int>(tiles < most ? tiles : most);
+      if (o->esize == 2) pack_rows<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(o->base), reinterpret_cast<uint16_t*>(at), o->rows, o->K, o->s_r, o->s_k, pitch);
+      else pack_rows<uint8_t><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(o->base), at, o->rows, o->K, o->s_r, o->s_k, pitch);
+      ++launches;
+    }
+    o->s_r = pitch;
+    o->s_k = 1;
+    o->base = at;
+    at += bytes;
   }
-  const int64_t bytes = o.packed_bytes();
-  o.s_r = o.pitch();
-  o.s_k = 1;
-  o.base = at;
-  at += bytes;
-  ++launches;
-  return B200_OK;
+  if (n) {
+    pack_rows_shifted<<<blocks[0] + blocks[1], 256, 0, st>>>(rows[0], rows[1], blocks[0]);
+    ++launches;
+  }
 }
 
 bool encode_rows(CUtensorMap* map, const LinOperand& o, CUtensorMapDataType dt, int box_rows) {
@@ -706,8 +786,7 @@ int run_linear(LinOperand a, LinOperand b, void* out, int64_t M, int64_t N, int6
   if (need && (!scratch || scratch_bytes < need + 256)) return B200_ESCRATCH;
   unsigned char* at = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(scratch) + 255) & ~static_cast<uintptr_t>(255));
   int launches = 1;
-  if (int rc = pack(a, at, st, launches)) return rc;
-  if (int rc = pack(b, at, st, launches)) return rc;
+  pack(a, b, at, st, launches);
   p.M = M; p.N = N; p.K = K;
   p.k_step = kSlabBytes / a.esize;
   const LinPlan plan = plan_linear(M, N, K, per, p.k_step);
