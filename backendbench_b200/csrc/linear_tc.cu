@@ -56,7 +56,7 @@ struct LinParams {
   int splits;             // kSplit: CTAs that share a tile's K
   int ring, stages;       // bytes of shared memory for the slabs, and how many that is (see ring_stages)
   int acc_cols, accs;     // accumulators in tensor memory: columns of one, how many
-  int early;              // the next grid may start beside this one
+  int early, ahead;       // the next grid may start beside this one; slabs of weights that it brings into L2 then
   uint32_t idesc;
   int act;                // gated: activation
   float* side;            // gated: the projections [M, 2 N], or NULL
@@ -260,10 +260,11 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
     if (p.early) next_grid_may_start();
     if (p.early && warp == 0 && lane == 0) {
       const int64_t t = SHARE == kSplit ? blockIdx.x / p.splits : blockIdx.x, mt = (p.M + 127) / 128, nt = (p.N + p.w - 1) / p.w;
-      const int all = static_cast<int>((p.K + p.k_step - 1) / p.k_step), k0 = SHARE == kSplit ? static_cast<int>(static_cast<int64_t>(all) * rank / p.splits) : 0;
+      const int all = static_cast<int>((p.K + p.k_step - 1) / p.k_step), k0 = SHARE == kSplit ? static_cast<int>(static_cast<int64_t>(all) * rank / p.splits) : 0,
+                k1 = SHARE == kSplit ? static_cast<int>(static_cast<int64_t>(all) * (rank + 1) / p.splits) : all;
       int mb, nb;
       lin_tile(t, mt, nt, p.group_m, mb, nb);
-      for (int s = 0; s < stages && k0 + s < all; ++s) {
+      for (int s = 0; s < p.ahead && k0 + s < k1; ++s) {
         prefetch_l2_3d(&map_b, (k0 + s) * p.k_step, nb * p.w, 0);
         if (!kI8) prefetch_l2_3d(&map_b, (k0 + s) * p.k_step, nb * p.w + static_cast<int>(p.N), 0);
       }
@@ -787,45 +788,54 @@ int run_linear(LinOperand a, LinOperand b, void* out, int64_t M, int64_t N, int6
   unsigned char* at = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(scratch) + 255) & ~static_cast<uintptr_t>(255));
   int launches = 1;
   pack(a, b, at, st, launches);
-  p.M = M; p.N = N; p.K = K;
+  p.M = M;
+  p.N = N;
+  p.K = K;
   p.k_step = kSlabBytes / a.esize;
-  const LinPlan plan = plan_linear(M, N, K, per, p.k_step);
-  p.w = plan.w;
-  p.a_rows = plan.a_rows;
-  const bool pair = plan.share == kPaired;
-  p.b_rows = MODE == kGated ? plan.w : pair ? plan.w / 2 : plan.w;
-  p.b_boxes = MODE == kGated && !pair ? 2 : 1;
-  p.splits = plan.splits;
-  const int tile_m = pair ? 256 : 128;
   int64_t rows = (32ll << 20) / (K * a.esize) / 256 * 256;  // a group's panel of A stays in L2 while B goes by
   rows = rows < 2048 ? 2048 : rows > 65536 ? 65536 : rows;
-  p.group_m = static_cast<int>(rows / tile_m);
-  const uint32_t fmt = MODE == kInt8 ? 1u /* signed */ : is_bf16 ? 1u : 0u, acc = MODE == kInt8 ? 2u /* s32 */ : 1u /* f32 */;
-  p.idesc = (acc << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(plan.w * per >> 3) << 17) | (static_cast<uint32_t>(tile_m >> 4) << 24);
+  const uint32_t fmt = MODE == kInt8 ? 1u /* signed */ : is_bf16 ? 1u : 0u, sums = MODE == kInt8 ? 2u /* s32 */ : 1u /* f32 */;
   const CUtensorMapDataType dt = MODE == kInt8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  alignas(64) CUtensorMap map_a, map_b;
-  if (!encode_rows(&map_a, a, dt, p.a_rows) || !encode_rows(&map_b, b, dt, p.b_rows)) return B200_EDRIVER;
-  const int64_t tiles = ((M + tile_m - 1) / tile_m) * ((N + plan.w - 1) / plan.w);
-  const int stage_bytes = (p.a_rows + p.b_boxes * p.b_rows) * kSlabBytes;
-  // a tile to a CTA, room for four slabs and for its sums: half an SM is enough
-  const bool half = !pair && half_an_sm(per, plan.w, p.a_rows, plan.splits) && tiles * plan.splits <= 2 * kResident[plan.splits];
-  const int64_t slots = pair ? kNumSMs / 2 : half ? 2 * kNumSMs : kNumSMs, resident = tiles < slots ? tiles : slots;
-  p.ring = half ? kLinHalfRing : kLinRing;
-  p.stages = ring_stages(p.ring, stage_bytes);
-  p.acc_cols = 256;
-  p.accs = half ? 1 : 2;
-  p.early = half ? 1 : 0;
-  auto go = [&](auto* o) {
-    using TO = std::remove_pointer_t<decltype(o)>;
-    if (pair) return launch_linear<MODE, TO, kPaired>(2, 2 * resident, st, map_a, map_b, o, p, status);
-    if (plan.share == kSplit) return launch_linear<MODE, TO, kSplit>(plan.splits, tiles * plan.splits, st, map_a, map_b, o, p, status);
-    return launch_linear<MODE, TO, kSingle>(1, resident, st, map_a, map_b, o, p, status);
+  auto run = [&](const LinPlan& plan) -> int {
+    const bool pair = plan.share == kPaired;
+    const int tile_m = pair ? 256 : 128;
+    p.w = plan.w;
+    p.a_rows = plan.a_rows;
+    p.b_rows = MODE == kGated ? plan.w : pair ? plan.w / 2 : plan.w;
+    p.b_boxes = MODE == kGated && !pair ? 2 : 1;
+    p.splits = plan.splits;
+    p.group_m = static_cast<int>(rows / tile_m);
+    p.idesc = (sums << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(plan.w * per >> 3) << 17) | (static_cast<uint32_t>(tile_m >> 4) << 24);
+    alignas(64) CUtensorMap map_a, map_b;
+    if (!encode_rows(&map_a, a, dt, p.a_rows) || !encode_rows(&map_b, b, dt, p.b_rows)) return B200_EDRIVER;
+    const int64_t tiles = ((M + tile_m - 1) / tile_m) * ((N + plan.w - 1) / plan.w);
+    // a tile to a CTA, room for four slabs and for its sums: half an SM is enough
+    const bool half = !pair && half_an_sm(per, plan.w, p.a_rows, plan.splits) && tiles * plan.splits <= 2 * kResident[plan.splits];
+    const int64_t slots = pair ? kNumSMs / 2 : half ? 2 * kNumSMs : kNumSMs, resident = tiles < slots ? tiles : slots;
+    p.ring = half ? kLinHalfRing : kLinRing;
+    p.stages = ring_stages(p.ring, (p.a_rows + p.b_boxes * p.b_rows) * kSlabBytes);
+    p.acc_cols = 256;
+    p.accs = half ? 1 : 2;
+    p.early = half ? 1 : 0;
+    p.ahead = kLinHalfRing / (p.b_boxes * p.b_rows * kSlabBytes);  // (two or three times as much is no faster, and much more slower: bf16 1 x 4096 x 11008 31.1 us, 36.6 with 500 KB a CTA)
+    auto go = [&](auto* o) {
+      using TO = std::remove_pointer_t<decltype(o)>;
+      if (pair) return launch_linear<MODE, TO, kPaired>(2, 2 * resident, st, map_a, map_b, o, p, status);
+      if (plan.share == kSplit) return launch_linear<MODE, TO, kSplit>(plan.splits, tiles * plan.splits, st, map_a, map_b, o, p, status);
+      return launch_linear<MODE, TO, kSingle>(1, resident, st, map_a, map_b, o, p, status);
+    };
+    if (dtype_out == B200_BF16) return go(static_cast<__nv_bfloat16*>(out));
+    if (dtype_out == B200_F16) return go(static_cast<__half*>(out));
+    if constexpr (MODE == kInt8) return go(static_cast<float*>(out));
+    return B200_EDTYPE;
   };
-  int rc;
-  if (dtype_out == B200_BF16) rc = go(static_cast<__nv_bfloat16*>(out));
-  else if (dtype_out == B200_F16) rc = go(static_cast<__half*>(out));
-  else if constexpr (MODE == kInt8) rc = go(static_cast<float*>(out));
-  else return B200_EDTYPE;
+  const LinPlan plan = plan_linear(M, N, K, per, p.k_step);
+  int rc = run(plan);
+  if (rc == B200_ELAUNCH && plan.share != kSingle) {
+    // the cluster launch was refused (a device or a partition without thread-block clusters): the same on single CTAs
+    (void)cudaGetLastError();
+    rc = run(LinPlan{kSingle, 256 / per, M >= 128 ? 128 : static_cast<int>((M + 7) / 8 * 8), 1});
+  }
   if (rc) return rc;
   return check_launch(launches);
 }

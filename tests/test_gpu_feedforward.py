@@ -51,6 +51,7 @@ SIZES = [
     (1, 64, 8), (1, 8, 1), (1, 1, 1), (2, 1000, 300), (1, 4096, 1500), (3, 17, 5), (7, 512, 80), (16, 128, 40), (17, 72, 129), (53, 2048, 704),
     (64, 640, 2368), (100, 96, 24), (127, 200, 129), (128, 256, 256), (129, 320, 64), (129, 328, 65), (130, 1000, 520), (255, 384, 130), (257, 2056, 200), (300, 64, 7),
     (512, 512, 1024), (700, 1027, 333), (1000, 4096, 96), (2048, 448, 1376),
+    (4096, 320, 2104), (4096, 328, 1001), (5000, 64, 1504), (40, 11008, 1024), (60, 4096, 4096),
 ]
 
 
@@ -114,6 +115,26 @@ def test_gated_linear_backward(size, dtype):
     ref.assert_within(gw, dw, tw, "dw")
     only = K.gated_linear_backward(dh, x, w, projections, name, [False, True])
     assert only[0] is None and bits_equal(only[1], gw)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_products_of_drawn_sizes(seed):
+    """Tiles of every width, clusters of every size and pairs, as the plan takes them for sizes nobody chose."""
+    import random
+
+    rng = random.Random(seed)
+    for _ in range(14):
+        M, k, F = (int(2 ** rng.uniform(0, top)) for top in (11, 13, 11.5))
+        if rng.random() < 0.5:
+            k, F = (k + 15) // 16 * 16, (F + 7) // 8 * 8
+        dtype, name = rng.choice((BF, F16)), rng.choice(ref.ACTS)
+        x, w = _pair(M, k, F, dtype)
+        h, th, p, tp = ref.gated(x, w, name, dtype)
+        out, projections = K.gated_linear_train(x, w, name)
+        ref.assert_within(out, h, th, f"{M} x {k} x {F}: h")
+        ref.assert_within(projections, p, tp, f"{M} x {k} x {F}: projections")
+        a, b = _int8(M, k), _int8(F, k, seed=1)
+        _check_int8(a, b.t(), rng.choice((BF, F16, F32)), what=f"{M} x {k} x {F}: 8 bits")
 
 
 def _layouts(M, k, F, dtype):
@@ -322,6 +343,7 @@ def _check_int8(a, b, dtype, bias=None, what=""):
 INT8_SIZES = [
     (1, 1, 1), (1, 16, 16), (1, 4096, 1504), (2, 17, 3), (5, 128, 16), (16, 256, 40), (33, 1000, 130), (64, 11008, 512), (100, 144, 2400), (128, 512, 256), (129, 640, 128),
     (130, 656, 129), (255, 1024, 264), (257, 1027, 515), (300, 100, 20), (1000, 2048, 96), (700, 4096, 1000), (2537, 1027, 301), (1024, 1040, 2048),
+    (4096, 384, 2112), (6000, 64, 1501), (24, 8192, 3001), (300, 8192, 520),
 ]
 
 
