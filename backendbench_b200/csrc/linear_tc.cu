@@ -693,14 +693,14 @@ bool half_an_sm(int per, int w, int a_rows, int splits) {
 // What a plan takes, in us, with `per` rows of B to an output column (gated 2, int8 1) and slabs of 128 bytes of K. The terms: what
 // starting, handing over and storing take; the weights out of HBM; every CTA's bytes over the fabric; the latency of the loads
 // (longer for B, which comes from HBM, than for A, which comes from L2) over the bytes that are in flight; the issue of a
-// slab. Their constants were fitted to 1,207 timings of 55 products (1 to 8192 rows, K 160 to 11008, 128 to 11008 columns, both
+// slab. Their constants were fitted to 1,500 timings of 68 products (1 to 8192 rows, K 160 to 11008, 128 to 11008 columns, both
 // types); the plan with the least of these is 2 % slower than the best one that was timed, on average, and at most 16 %.
 double time_of(const LinPlan& q, int64_t M, int64_t N, int64_t slabs, int per) {
   const double k = static_cast<double>(slabs), cols = q.w * per;
   const int64_t across = (N + q.w - 1) / q.w;
   if (q.share == kPaired) {
     const int64_t tiles = ((M + 255) / 256) * across, rounds = (tiles + kNumSMs / 2 - 1) / (kNumSMs / 2);
-    return 9.1 + static_cast<double>(rounds) * (1.5 + k * (cols == 256 ? 0.307 : cols == 192 ? 0.241 : 0.197));
+    return 6.8 + static_cast<double>(rounds) * (2.16 + k * (cols == 256 ? 0.31 : cols == 192 ? 0.242 : 0.192));
   }
   const int64_t tiles = ((M + 127) / 128) * across;
   const bool half = half_an_sm(per, q.w, q.a_rows, q.splits) && tiles * q.splits <= 2 * kResident[q.splits];
@@ -713,11 +713,11 @@ double time_of(const LinPlan& q, int64_t M, int64_t N, int64_t slabs, int per) {
   }
   const double each = static_cast<double>((slabs + q.splits - 1) / q.splits) * rounds, a = each * kSlabBytes * q.a_rows * ctas, b = each * kSlabBytes * cols * ctas;
   const double deep = ctas > kNumSMs ? 2. : 1.;  // CTAs to an SM
-  double t = k * kSlabBytes * static_cast<double>(N * per) / 10.3e6;
-  t = fmax(t, (a + b) / 17e6);
-  t = fmax(t, (1.73 * b + 0.82 * a) / (ctas * (half ? kLinHalfRing : kLinRing)));
-  t = fmax(t, each * (0.228 * (deep > 1. ? 1.5 : 1.) + 0.00028 * cols * deep));
-  return 4.2 + (half ? 0. : 0.4) + t + 1.1 * rounds + 0.0058 * cols * deep + (q.splits > 1 ? 0.6 + q.a_rows * cols / 5e3 : 0.);
+  double t = k * kSlabBytes * static_cast<double>(N * per) / 11e6;
+  t = fmax(t, (a + b) / 16.8e6);
+  t = fmax(t, (1.98 * b + 0.6 * a) / (ctas * (half ? kLinHalfRing : kLinRing)));
+  t = fmax(t, each * (0.225 * (deep > 1. ? 1.44 : 1.) + 0.000225 * cols * deep));
+  return 3.64 + (half ? 0. : 0.12) + t + 1.29 * rounds + 0.007 * cols * deep + (q.splits > 1 ? 0.68 + q.a_rows * cols / 3.9e3 : 0.);
 }
 LinPlan best_plan(int64_t M, int64_t N, int64_t slabs, int per) {
   const int most = 256 / per, grain = 16 / per, a_rows = M >= 128 ? 128 : static_cast<int>((M + 7) / 8 * 8);

@@ -451,6 +451,25 @@ def test_gradients_flow_only_where_they_are_wanted():
         y.sum().backward()
 
 
+@without_bands
+@pytest.mark.parametrize("name", sorted(feedforward.OPERATORS))
+def test_operators_hold_up_to_torchs_own_checks(name):
+    """Schema, fake kernel, autograd registration and tracing, as torch.library.opcheck looks at them."""
+    x, w = _pair(4, 64, 8, BF)
+    x, w, s, q, one = x.requires_grad_(), w.requires_grad_(), _state(1, 2), _int8(8, 64), torch.ones(8, device=DEV)
+    plain, p = x.detach(), _randn(4, 16, dtype=F32)
+    args = {
+        "gated_linear": ((x, w, "gelu"), {}),
+        "gated_linear_train": ((x, w), {}),
+        "gated_linear_backward": ((_randn(4, 8, dtype=BF), plain, w.detach(), p, "silu", [True, False]), {}),
+        "dropout": ((x, 0.3, s, x), {"subsequence": 2}),
+        "dropout_backward": ((plain, 0.3, s), {}),
+        "quantize_rows": ((plain,), {}),
+        "mm_int8": ((q, q.t(), one, one, _randn(8, dtype=F16)), {"out_dtype": F16}),
+    }[name]
+    torch.library.opcheck(getattr(K, name).default, *args)
+
+
 def test_gradients_of_broadcast_inputs():
     """x and its gradient's memory shared along rows: the gradient sums over them, whatever the strides say."""
     w = _randn(48, 64, dtype=F32, std=0.125)
