@@ -1,7 +1,8 @@
 /*
  * b200ops.h -- C ABI of libb200ops.so: hand-written sm_100a CUDA kernels for the
- * sixteen ATen operators that a BackendBench directory backend overrides, plus the
- * two device-side helpers of the evaluation path (allclose/error scan, L2 flush).
+ * sixteen ATen operators that a BackendBench directory backend overrides, the linear
+ * layers of a feed-forward block beside them, plus the two device-side helpers of the
+ * evaluation path (allclose/error scan, L2 flush).
  *
  * The reference project (meta-pytorch/BackendBench) is pure Python and has no FFI
  * of its own: the arithmetic it checks against is `torch.ops.aten.<op>` reached at
