@@ -28,6 +28,7 @@ struct ActSilu {
     d = s * (1.f + g * (1.f - s));
   }
   __device__ __forceinline__ float fast(float g) const { return f<true>(g); }
+  __device__ __forceinline__ float exact(float g) const { return f<false>(g); }
 };
 struct ActGelu {
   template <bool FAST> static __device__ __forceinline__ float f(float g) { return g * normcdff(g); }
@@ -37,6 +38,7 @@ struct ActGelu {
     d = c + g * 0.3989422804014327f * (FAST ? __expf(e) : expf(e));
   }
   __device__ __forceinline__ float fast(float g) const { return f<true>(g); }
+  __device__ __forceinline__ float exact(float g) const { return f<false>(g); }
 };
 struct ActGeluTanh {
   template <bool FAST> static __device__ __forceinline__ float f(float g) {
@@ -51,6 +53,7 @@ struct ActGeluTanh {
     d = s + h * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * h * h);
   }
   __device__ __forceinline__ float fast(float g) const { return f<true>(g); }
+  __device__ __forceinline__ float exact(float g) const { return f<false>(g); }
 };
 struct ActRelu {
   template <bool FAST> static __device__ __forceinline__ float f(float g) { return g <= 0.f ? 0.f : g; }
@@ -59,6 +62,7 @@ struct ActRelu {
     d = g <= 0.f ? 0.f : 1.f;
   }
   __device__ __forceinline__ float fast(float g) const { return f<true>(g); }
+  __device__ __forceinline__ float exact(float g) const { return f<false>(g); }
 };
 struct ActSigmoid {
   template <bool FAST> static __device__ __forceinline__ float f(float g) { return gate_sigmoid<FAST>(g); }
@@ -67,6 +71,7 @@ struct ActSigmoid {
     d = a * (1.f - a);
   }
   __device__ __forceinline__ float fast(float g) const { return f<true>(g); }
+  __device__ __forceinline__ float exact(float g) const { return f<false>(g); }
 };
 
 // `body` with the activation as its argument: one look per tile or thread, not one per value

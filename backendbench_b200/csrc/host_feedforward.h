@@ -140,21 +140,19 @@ at::DimVector with_last(const Tensor& t, int64_t last) {
 }
 
 // (with the lock held) a @ b as feedforward._product forms it
-constexpr int64_t kF32Range = 4096;  // F32_RANGE
 Tensor ff_product(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t K, at::IntArrayRef shape) {
-  Tensor out;
-  const int64_t step = dt(a.t) == B200_F32 && K > kF32Range ? kF32Range : K;
-  for (int64_t k = 0; k < K; k += step) {
-    Operand x = a, y = b;
-    if (k) {
-      x.t = a.t.as_strided({1}, {1}, a.t.storage_offset() + k * a.col);  // (its data pointer is what counts)
-      y.t = b.t.as_strided({1}, {1}, b.t.storage_offset() + k * b.row);
-    }
-    PyObject* r = gemm(x, y, out.defined() ? out.view({M, N}) : Tensor(), 1, M, N, std::min(step, K - k), 1.0, out.defined() ? 1.0 : 0.0, shape);
-    if (!r) raise_python();
-    out = taken(r);
+  const int64_t need = dt(a.t) == B200_F32 ? api.b200_linear_f32_scratch_bytes(M, N, K) : 0;
+  if (need > 0) {
+    Tensor out = new_tensor(shape, a.t.scalar_type(), a.t);
+    const Tensor s = ff_scratch(a.t, need);
+    ff_check(api.b200_linear_f32(static_cast<const float*>(ptr(a.t)), static_cast<const float*>(ptr(b.t)), static_cast<float*>(ptr(out)), M, N, K, a.row, a.col, b.row, b.col, ptr(s), need,
+                                 ff_status(a.t), stream()),
+             "b200_linear_f32");
+    return out;
   }
-  return out;
+  PyObject* r = gemm(a, b, Tensor(), 1, M, N, K, 1.0, 0.0, shape);
+  if (!r) raise_python();
+  return taken(r);
 }
 
 // (output, projections); an undefined output: the wrapper has to take the call
@@ -165,15 +163,25 @@ std::tuple<Tensor, Tensor> gated_direct(const Tensor& x, const Tensor& w, c10::s
   const int64_t F = w.size(0) / 2;
   if (r.M == 0 || F == 0 || r.K == 0) return {};
   Tensor projections;
-  if (dt(x) == B200_F32) {
+  const int64_t planes = dt(x) == B200_F32 ? api.b200_linear_f32_scratch_bytes(r.M, 2 * F, r.K) : 0;
+  if (dt(x) == B200_F32 && planes == 0) {
     Gil gil;
-    projections = ff_product(Operand{x, 0, r.s_m, r.s_k}, Operand{w, 0, w.stride(1), w.stride(0)}, r.M, 2 * F, r.K, with_last(x, 2 * F));
+    PyObject* p = gemm(Operand{x, 0, r.s_m, r.s_k}, Operand{w, 0, w.stride(1), w.stride(0)}, Tensor(), 1, r.M, 2 * F, r.K, 1.0, 0.0, with_last(x, 2 * F));
+    if (!p) raise_python();
+    projections = taken(p);
     Tensor out = new_tensor(with_last(x, F), x.scalar_type(), x);
     ff_launched(launched("b200_gate", [&, st = stream()] { return api.b200_gate(static_cast<const float*>(ptr(projections)), static_cast<float*>(ptr(out)), r.M, F, act, st); }));
     return {out, projections};
   }
   Tensor out = new_tensor(with_last(x, F), x.scalar_type(), x);
   if (keep) projections = new_tensor(with_last(x, 2 * F), at::kFloat, x);
+  if (planes > 0) {
+    const Tensor s = ff_scratch(x, planes);
+    ff_check(api.b200_gated_linear_f32(static_cast<const float*>(ptr(x)), static_cast<const float*>(ptr(w)), static_cast<float*>(ptr(out)), static_cast<float*>(ptr(projections)), r.M, F, r.K, r.s_m,
+                                       r.s_k, w.stride(0), w.stride(1), act, ptr(s), planes, ff_status(x), stream()),
+             "b200_gated_linear_f32");
+    return {out, projections};
+  }
   const int64_t ws0 = w.stride(0), ws1 = w.stride(1), need = api.b200_gated_linear_scratch_bytes(ptr(x), ptr(w), r.M, F, r.K, r.s_m, r.s_k, ws0, ws1);
   const Tensor s = ff_scratch(x, need);
   ff_check(api.b200_gated_linear(ptr(x), ptr(w), ptr(out), static_cast<float*>(ptr(projections)), r.M, F, r.K, r.s_m, r.s_k, ws0, ws1, act, dt(x), ptr(s), need, ff_status(x), stream()),

@@ -1,0 +1,92 @@
+// What the kernels of linear_tc.cu and linear_f32.cu share: sizes, the order of tiles, stores of 32 x 32 values, shared memory of a
+// cluster.
+#pragma once
+
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "b200_common.cuh"
+#include "tc_common.cuh"
+
+namespace b200 {
+
+constexpr int kLinThreads = 320;                        // TMA warp, MMA warp, 8 epilogue warps
+constexpr int kSlabBytes = 128;                         // of K to a slab: one row of the 128-byte swizzle
+constexpr int kLinRing = 192 * 1024;
+constexpr int kLinEpiWarps = 8, kLinEpiBytes = 4096;    // staging: 32 rows x 128 bytes per epilogue warp
+constexpr uint64_t kLinWaitNs = 2000000000ull;          // every mbarrier wait gives up after 2 s
+enum : int { kSingle = 0, kPaired = 1, kSplit = 2 };  // a CTA to a tile; a pair to a tile of 256 rows; a cluster that shares a tile's K
+
+// CTAs of a whole SM's shared memory that are resident at once in clusters of 1 .. 8 (cudaOccupancyMaxActiveClusters on a B200)
+constexpr int kResident[9] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
+
+__device__ __forceinline__ void prefetch_l2_3d(const CUtensorMap* map, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+
+__device__ __forceinline__ void lin_tile(int64_t t, int64_t mt, int64_t nt, int group_m, int& mb, int& nb) {
+  const int64_t per_group = static_cast<int64_t>(group_m) * nt;
+  const int64_t g = t / per_group, in_g = t - g * per_group;
+  const int64_t left = mt - g * group_m, gm = left < group_m ? left : group_m;
+  mb = static_cast<int>(g * group_m + in_g % gm);
+  nb = static_cast<int>(in_g / gm);
+}
+
+// 16 bytes of a cluster CTA's shared memory
+template <typename V> __device__ __forceinline__ V ld_cluster(uint32_t from) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+  return *reinterpret_cast<const V*>(&v);
+}
+
+// What is staged (see lin_store) to rows off the grid: a column to a lane, eight rows on their way together. (A call, so that
+// its registers are not the epilogue's.)
+template <typename TO> __device__ __noinline__ void lin_copy_ragged(const unsigned char* mine, TO* out, int64_t pitch, int nrows, int ncols, int lane) {
+  constexpr int kRow = 32 * static_cast<int>(sizeof(TO)), kPieces = kRow / 16, kPer = 16 / static_cast<int>(sizeof(TO)), kShift = sizeof(TO) == 2 ? 1 : 0;
+  const unsigned char* from = mine + lane % kPer * static_cast<int>(sizeof(TO));
+  const int j = lane / kPer;
+  out += lane;
+  auto rows = [&](int r0, auto whole) {
+    TO w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const TO*>(from + i * kRow + ((j ^ ((i >> kShift) & (kPieces - 1))) << 4));
+#pragma unroll
+    for (int i = 0; i < 8; ++i, out += pitch)
+      if (decltype(whole)::value || (lane < ncols && r0 + i < nrows)) *out = w[i];
+  };
+  if (nrows >= 32 && ncols >= 32) {
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += 8, from += 8 * kRow) rows(r0, std::true_type{});
+  } else {
+#pragma unroll 1
+    for (int r0 = 0; r0 < nrows; r0 += 8, from += 8 * kRow) rows(r0, std::false_type{});
+  }
+}
+
+// 32 values of a lane's row to 32 columns of `out` (row pitch `pitch`, column 0 at `col`): rounded once into the warp's
+// staging buffer (16-byte pieces swizzled so that neither side meets a bank twice), then out in 16-byte pieces of
+// eight (fp32: four) rows at a time, or element by element where rows are off the grid.
+template <typename TO>
+__device__ __forceinline__ void lin_store(const float* v, unsigned char* mine, TO* out, int64_t pitch, int nrows, int ncols, bool vec, int lane) {
+  constexpr int kRow = 32 * static_cast<int>(sizeof(TO)), kPieces = kRow / 16, kPer = 16 / static_cast<int>(sizeof(TO)), kShift = sizeof(TO) == 2 ? 1 : 0;
+  __syncwarp();  // what was there has been read out
+#pragma unroll
+  for (int j = 0; j < kPieces; ++j) *reinterpret_cast<uint4*>(mine + lane * kRow + ((j ^ ((lane >> kShift) & (kPieces - 1))) << 4)) = narrow<TO>(v + j * kPer);
+  __syncwarp();
+  if (vec) {
+    constexpr int kRowsAt = 32 / kPieces;
+    const int j = lane % kPieces, r0 = lane / kPieces;
+    if (j * kPer < ncols) {
+#pragma unroll 4
+      for (int i = 0; i < kPieces; ++i) {
+        const int r = r0 + i * kRowsAt;
+        if (r < nrows) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * pitch + j * kPer) = *reinterpret_cast<const uint4*>(mine + r * kRow + ((j ^ ((r >> kShift) & (kPieces - 1))) << 4));
+      }
+    }
+  } else {
+    lin_copy_ragged<TO>(mine, out, pitch, nrows, ncols, lane);
+  }
+}
+
+}  // namespace b200

@@ -74,20 +74,20 @@ def _pair_args(input: torch.Tensor, weight: torch.Tensor, what: str) -> Tuple[in
     return weight.shape[0] // 2, weight.shape[1]
 
 
-F32_RANGE = 4096
-
-
 def _product(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
-    """a @ b. fp32 sums on the tensor cores lose half a unit in the last place with each of their K / 16 additions, always the same
-    way: a contraction of 22016 was 8.4e-6 of the norm off 64 bits. Long ones are therefore summed up in ranges of
-    F32_RANGE (2.1e-6), each rounded to nearest onto the ones before."""
-    K = a.shape[1]
-    if a.dtype != torch.float32 or K <= F32_RANGE:
+    """a @ b. Large fp32 products take two f16 planes an operand, whose sums are rounded to nearest slab by slab: their
+    contractions are as long as a layer is wide, where sums that truncate drift."""
+    (M, K), N = a.shape, b.shape[1]
+    need = int(lib().b200_linear_f32_scratch_bytes(M, N, K)) if a.dtype == torch.float32 else 0
+    if not need:
         return ops.mm_default(a, b)
-    out = None
-    for k in range(0, K, F32_RANGE):
-        x, y = a[:, k : k + F32_RANGE], b[k : k + F32_RANGE]
-        out = ops.mm_default(x, y) if out is None else ops.addmm_default(out, x, y)
+    out, scratch = ops._new((M, N), a.dtype, a.device), ops._scratch(a.device, need)
+    check(
+        lib().b200_linear_f32(
+            a.data_ptr(), b.data_ptr(), out.data_ptr(), M, N, K, a.stride(0), a.stride(1), b.stride(0), b.stride(1), scratch.data_ptr(), need, ops._status(a.device).data_ptr(), ops._stream_handle()
+        ),
+        "b200_linear_f32",
+    )
     return out
 
 
@@ -97,16 +97,25 @@ def _gated(input: torch.Tensor, weight: torch.Tensor, activation: str, keep: boo
     F, K = _pair_args(input, weight, what)
     lead = list(input.shape[:-1])
     out = ops._new(lead + [F], input.dtype, input.device)
-    fp32 = input.dtype == torch.float32
-    projections = ops._new(lead + [2 * F], torch.float32, input.device) if keep and not fp32 else None
-    M = ops._prod(lead)
-    if fp32:
-        # the tensor cores take fp32 as six products of bf16 planes, over several launches: the projections are put
-        # together first, the gate follows
-        projections = _product(_as_rows(input), weight.t())
+    M, fp32 = ops._prod(lead), input.dtype == torch.float32
+    planes = int(lib().b200_linear_f32_scratch_bytes(M, 2 * F, K)) if fp32 else 0
+    if fp32 and not planes:
+        # small fp32 products leave their sums to a gate of its own
+        projections = ops.mm_default(_as_rows(input), weight.t())
         if out.numel():
             check(lib().b200_gate(projections.data_ptr(), out.data_ptr(), M, F, act, ops._stream_handle()), "b200_gate")
         return out, projections.view(lead + [2 * F])
+    projections = ops._new(lead + [2 * F], torch.float32, input.device) if keep else None
+    if fp32:
+        x, scratch = _as_rows(input), ops._scratch(out.device, planes)
+        check(
+            lib().b200_gated_linear_f32(
+                x.data_ptr(), weight.data_ptr(), out.data_ptr(), projections.data_ptr() if projections is not None else None, M, F, K, x.stride(0), x.stride(1), weight.stride(0), weight.stride(1), act,
+                scratch.data_ptr(), planes, ops._status(out.device).data_ptr(), ops._stream_handle(),
+            ),
+            "b200_gated_linear_f32",
+        )
+        return out, projections
     if out.numel():
         x = _as_rows(input)
         args = (M, F, K, x.stride(0), x.stride(1), weight.stride(0), weight.stride(1))
@@ -124,8 +133,9 @@ def _gated(input: torch.Tensor, weight: torch.Tensor, activation: str, keep: boo
 
 @_on_device_of
 def gated_linear(input: torch.Tensor, weight: torch.Tensor, activation: str = "silu") -> torch.Tensor:
-    """act(input @ weight[:F].T) * (input @ weight[F:].T), [..., K] x [2 F, K] -> [..., F]. bf16 / f16: one kernel, fp32
-    sums, one rounding. `activation`: silu, gelu (erf), gelu_tanh, relu or sigmoid."""
+    """act(input @ weight[:F].T) * (input @ weight[F:].T), [..., K] x [2 F, K] -> [..., F]. One kernel on fp32 sums, with one
+    rounding; large fp32 operands are split into two f16 planes before it (2^-22 of an element, 2^-40 of its row's largest
+    magnitude), small ones take the package's fp32 product and a gate behind it. `activation`: silu, gelu (erf), gelu_tanh, relu or sigmoid."""
     return _gated(input, weight, activation, False, "gated_linear")[0]
 
 

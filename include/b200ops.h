@@ -364,6 +364,19 @@ int b200_gated_linear(const void* x, const void* w, void* out, float* projection
                       int64_t K, int64_t sxm, int64_t sxk, int64_t swn, int64_t swk, int activation,
                       int dtype, void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream);
 
+/* fp32 products on the tensor cores in two f16 planes an operand: rows (of K elements) scaled by a power of two each, elements
+ * split into h + l, h h + h l + l h summed up in fp32, slab by slab and rounded to nearest. An element is resolved to 2^-22 of
+ * itself or 2^-40 of its row's largest magnitude, whichever is more; an infinity or a NaN makes the outputs that
+ * its row enters NaN or infinite. Any operand strides; C, out [M, N] and projections [M, 2 N] (may be NULL) contiguous.
+ * b200_linear_f32_scratch_bytes (gated: with 2 N for N) is 0 where the sizes do not pay for the planes. */
+int64_t b200_linear_f32_scratch_bytes(int64_t M, int64_t N, int64_t K);
+int b200_linear_f32(const float* A, const float* B, float* C, int64_t M, int64_t N, int64_t K, int64_t sAm,
+                    int64_t sAk, int64_t sBk, int64_t sBn, void* scratch, int64_t scratch_bytes,
+                    uint32_t* status, void* stream);
+int b200_gated_linear_f32(const float* x, const float* w, float* out, float* projections, int64_t M, int64_t N,
+                          int64_t K, int64_t sxm, int64_t sxk, int64_t swn, int64_t swk, int activation,
+                          void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream);
+
 /* The gate by itself (fp32, whose products come in several launches), and its gradient, for contiguous fp32
  * projections [M, 2 N] = [g | u]: out = act(g) * u;  grad_projections = [grad * u * act'(g) | grad * act(g)], grad and
  * grad_projections of any float dtype. */

@@ -128,6 +128,11 @@ def test_the_library_refuses_what_the_wrappers_would(monkeypatch):
     assert lib.b200_mm_int8_scratch_bytes(base, base, 4, 8, 64, 64, 1, 8, 1) >= 8 * 64
     m = lambda *a: lib.b200_mm_int8(None, None, None, None, None, None, *a, None, 0, None, None)
     assert m(4, 4, 131072, 4, 1, 4, 1, BF) == -1 and m(4, 4, 4, 4, 1, 4, 1, _abi.I32) == -2 and m(4, 0, 4, 4, 1, 4, 1, BF) == 0 and m(4, 4, 4, 4, 1, 4, 1, BF) == -1
+    f = lambda *a: lib.b200_linear_f32(None, None, None, *a, None, 0, None, None)
+    assert f(4, 4, 4, 4, 1, 4, 1) == -1 and f(0, 4, 4, 4, 1, 4, 1) == -1
+    assert lib.b200_linear_f32(base, base, base, 128, 128, 128, 128, 1, 128, 1, None, 0, None, None) == -4
+    assert lib.b200_gated_linear_f32(base, base, base, None, 128, 128, 128, 128, 1, 128, 1, 7, None, 0, None, None) == -1
+    assert lib.b200_linear_f32_scratch_bytes(64, 4096, 4096) == lib.b200_linear_f32_scratch_bytes(128, 128, 128) == lib.b200_linear_f32_scratch_bytes(0, 1, 1) == 0
     assert lib.b200_dropout(None, None, None, 4, 1.5, None, 0, BF, None) == -1 and lib.b200_dropout(None, None, None, 0, 0.5, None, 0, BF, None) == 0
     assert lib.b200_dropout(None, None, None, 4, 0.5, None, 0, _abi.I8, None) == -2 and lib.b200_dropout(None, None, None, 4, 0.5, None, 0, BF, None) == -1
     assert lib.b200_gate(None, None, 4, 4, 9, None) == -1 and lib.b200_gate_backward(None, None, None, 4, 4, 0, _abi.I32, None) == -2

@@ -90,7 +90,10 @@ def test_every_activation_with_large_and_small_gates(name, dtype):
     ref.assert_within(gw, dw, tw, "dw")
 
 
-@pytest.mark.parametrize("size", [(1, 64, 8), (3, 17, 5), (130, 1000, 520), (300, 260, 301), (1531, 1027, 205)], ids=str)
+F32_LARGE = [(65, 11008, 200), (100, 2048, 512), (200, 4096, 300), (129, 1030, 1001), (2048, 1024, 1104), (1000, 64, 4000), (1531, 1027, 1365), (3000, 200, 190), (66, 4100, 3001)]
+
+
+@pytest.mark.parametrize("size", [(1, 64, 8), (3, 17, 5), (130, 1000, 520), (300, 260, 301), (1531, 1027, 205)] + F32_LARGE, ids=str)
 @pytest.mark.parametrize("name", ["silu", "gelu"])
 def test_gated_linear_32_bits(size, name):
     M, k, F = size
@@ -99,10 +102,51 @@ def test_gated_linear_32_bits(size, name):
     ref.assert_within(K.gated_linear(x, w, name), h, th, "h")
     out, projections = K.gated_linear_train(x, w, name)
     ref.assert_within(projections, p, tp, "projections")
+    ref.assert_within(out, h, th, "h of the training form")
+
+
+@pytest.mark.parametrize("size", F32_LARGE, ids=str)
+def test_large_products_in_32_bits_are_as_exact_as_their_sums(size):
+    """Against 64 bits by the norm, where errors that always have one sign would show: two f16 planes are off by 2^-23 of an element or so,
+    a sum rounded to nearest slab by slab by 2^-24 of what it has reached, at random: 1e-6 holds an order of magnitude."""
+    M, k, F = size
+    x, w = _pair(M, k, F, F32)
+    x = x.abs()  # sums that grow all the way
+    out, projections = K.gated_linear_train(x, w)
+    h, _, p, _ = ref.gated(x, w, "silu", F32)
+    assert (projections.double() - p).norm() <= 1e-6 * p.norm() and (out.double() - h).norm() <= 2e-6 * h.norm()
+    dh = _randn(M, F, dtype=F32, seed=3)
+    dx, _, dw, _ = ref.gated_grads(dh, x, w, projections, "silu", F32)
+    gx, gw = K.gated_linear_backward(dh, x, w, projections)
+    assert (gx.double() - dx).norm() <= 1e-6 * dx.norm() and (gw.double() - dw).norm() <= 1e-6 * dw.norm()
+
+
+def test_rows_of_any_magnitude_in_32_bits():
+    """Rows and columns from the subnormals to the largest numbers, rows of zeros, one large element in a row; what is not finite spoils its
+    own row or column alone."""
+    M, k, F = 300, 512, 256
+    x, w = _pair(M, k, F, F32)
+    x *= torch.logspace(-38, 20, M, device=DEV, dtype=F32)[:, None]
+    w *= torch.logspace(-15, 10, 2 * F, device=DEV, dtype=F32)[torch.randperm(2 * F, device=DEV)][:, None]
+    x[5], x[6, 1:], w[7], x[8] = 0.0, 0.0, 0.0, 1e-42
+    x[9, 3], x[290] = 1e6 * x[9].abs().max(), 3.0e38 / 512**2
+    w[11, 5] *= 1e4
+    _, projections = K.gated_linear_train(x, w, "relu")
+    _, _, p, tp = ref.gated(x, w, "relu", F32)
+    fine = p.abs() < 3.0e38
+    ref.assert_within(projections[fine], p[fine], tp[fine] + 2.0**-149, "projections")
+    assert not projections[p.abs() > 3.5e38].isfinite().any()
+    x, w = _pair(M, k, F, F32)
+    _, clean = K.gated_linear_train(x, w)
+    x[20, 100], x[21, 7], w[30, 9] = float("nan"), -float("inf"), float("inf")
+    _, spoilt = K.gated_linear_train(x, w)
+    rows, cols = [i for i in range(M) if i not in (20, 21)], [i for i in range(2 * F) if i != 30]
+    assert not spoilt[[20, 21]].isfinite().any() and not spoilt[:, 30].isfinite().any()
+    assert bits_equal(spoilt[rows][:, cols], clean[rows][:, cols])
 
 
 @pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "f16", "f32"])
-@pytest.mark.parametrize("size", [(1, 64, 8), (3, 17, 5), (64, 256, 96), (200, 512, 136), (257, 130, 77), (1024, 768, 640)], ids=str)
+@pytest.mark.parametrize("size", [(1, 64, 8), (3, 17, 5), (64, 256, 96), (200, 512, 136), (257, 130, 77), (1024, 768, 640), (777, 520, 1001), (130, 4096, 300)], ids=str)
 def test_gated_linear_backward(size, dtype):
     M, k, F = size
     x, w = _pair(M, k, F, dtype)
@@ -128,11 +172,12 @@ def test_products_of_drawn_sizes(seed):
         if rng.random() < 0.5:
             k, F = (k + 15) // 16 * 16, (F + 7) // 8 * 8
         dtype, name = rng.choice((BF, F16)), rng.choice(ref.ACTS)
-        x, w = _pair(M, k, F, dtype)
-        h, th, p, tp = ref.gated(x, w, name, dtype)
-        out, projections = K.gated_linear_train(x, w, name)
-        ref.assert_within(out, h, th, f"{M} x {k} x {F}: h")
-        ref.assert_within(projections, p, tp, f"{M} x {k} x {F}: projections")
+        for dtype in (dtype, F32):
+            x, w = _pair(M, k, F, dtype)
+            h, th, p, tp = ref.gated(x, w, name, dtype)
+            out, projections = K.gated_linear_train(x, w, name)
+            ref.assert_within(out, h, th, f"{M} x {k} x {F}: h")
+            ref.assert_within(projections, p, tp, f"{M} x {k} x {F}: projections")
         a, b = _int8(M, k), _int8(F, k, seed=1)
         _check_int8(a, b.t(), rng.choice((BF, F16, F32)), what=f"{M} x {k} x {F}: 8 bits")
 
@@ -151,7 +196,7 @@ def _layouts(M, k, F, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
-@pytest.mark.parametrize("size", [(5, 64, 24), (150, 328, 72)], ids=str)
+@pytest.mark.parametrize("size", [(5, 64, 24), (150, 328, 72), (260, 520, 400)], ids=str)
 def test_gated_linear_of_any_layout(size, dtype):
     M, k, F = size
     for what, x, w in _layouts(M, k, F, dtype):
@@ -502,24 +547,25 @@ def _all_calls(x, w, q, w8, sa, sb, dh, state):
     return (K.gated_linear(x, w), h, projections, *K.gated_linear_backward(dh, x, w, projections), K.dropout(x, 0.1, state, x), *K.quantize_rows(x), K.mm_int8(q, w8.t(), sa, sb))
 
 
-def _all_args(M=70, k=136, F=72, odd=0):
+def _all_args(M=70, k=136, F=72, odd=0, dtype=BF):
     k += odd
-    x, w = _pair(M, k, F, BF)
-    return x, w, _int8(M, k), _int8(96, k), torch.rand(M, device=DEV), torch.rand(96, device=DEV), _randn(M, F, dtype=BF), _state(3, 4)
+    x, w = _pair(M, k, F, dtype)
+    return x, w, _int8(M, k), _int8(96, k), torch.rand(M, device=DEV), torch.rand(96, device=DEV), _randn(M, F, dtype=dtype), _state(3, 4)
 
 
 @pytest.mark.parametrize("odd", [0, 3])
 @pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "f16", "f32"])
-def test_native_calls_give_what_the_wrappers_give(dtype, odd, bands):
+@pytest.mark.parametrize("size", [(70, 136, 72), (300, 600, 200)], ids=str)
+def test_native_calls_give_what_the_wrappers_give(dtype, odd, size, bands):
     """With the bands' allocator in place every call goes through the wrappers; without it plain ones come from native code."""
-    M, k, F = 70, 136 + odd, 72
+    M, k, F = size[0], size[1] + odd, size[2]
     x, w = _pair(M, k, F, dtype)
     q, w8, sa, sb, bias = _int8(M, k), _int8(96, k), torch.rand(M, device=DEV), torch.rand(96, device=DEV), _randn(96, dtype=dtype)
     dh, s, r = _randn(M, F, dtype=dtype), _state(3, 4), _randn(M, k, dtype=dtype, seed=6)
     wide = _randn(M, k + 8, dtype=dtype)
 
     def calls():
-        for v in (x, wide[:, :k], x.t().contiguous().t(), x.view(2, 35, k)):
+        for v in (x, wide[:, :k], x.t().contiguous().t(), x.view(2, M // 2, k)):
             h, projections = K.gated_linear_train(v, w, "gelu")
             g = dh.view(h.shape)
             yield from (K.gated_linear(v, w), h, projections)
@@ -562,9 +608,9 @@ def test_refusals_come_back_as_the_wrappers_raise_them(bands):
             K.gated_linear(torch.autograd.forward_ad.make_dual(x, x), w)
 
 
-@pytest.mark.parametrize("odd", [0, 3])
-def test_calls_repeat_bit_for_bit_on_other_streams_and_side_by_side(odd):
-    args = _all_args(odd=odd)
+@pytest.mark.parametrize("args", [{}, {"odd": 3}, {"M": 300, "k": 1000, "F": 200, "dtype": F32}], ids=str)
+def test_calls_repeat_bit_for_bit_on_other_streams_and_side_by_side(args):
+    args = _all_args(**args)
     want = _all_calls(*args)
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(3)]
@@ -578,10 +624,10 @@ def test_calls_repeat_bit_for_bit_on_other_streams_and_side_by_side(odd):
 
 
 @without_bands
-@pytest.mark.parametrize("odd", [0, 3])
-def test_captured_calls_replay_with_new_contents(odd):
+@pytest.mark.parametrize("args", [{}, {"odd": 3}, {"M": 300, "k": 1000, "F": 200, "dtype": F32}], ids=str)
+def test_captured_calls_replay_with_new_contents(args):
     """Two graphs of the same calls, replayed in turn on two streams with new inputs and a new offset; each owns what its calls used."""
-    args = _all_args(odd=odd)
+    args = _all_args(**args)
     _all_calls(*args)
     torch.cuda.synchronize()
     graphs = []
@@ -591,7 +637,7 @@ def test_captured_calls_replay_with_new_contents(odd):
             out = _all_calls(*args)
         graphs.append((g, out, torch.cuda.Stream()))
     for step in range(3):
-        args[0].copy_(_randn(*args[0].shape, dtype=BF, seed=20 + step))
+        args[0].copy_(_randn(*args[0].shape, dtype=args[0].dtype, seed=20 + step))
         args[7][1] = 1000 * step
         torch.cuda.synchronize()
         for g, _, s in graphs:
