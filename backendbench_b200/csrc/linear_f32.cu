@@ -26,6 +26,10 @@ namespace {
 constexpr int kF32Cols = 128, kF32Accs = 4, kF32MaxStages = 8;
 constexpr size_t kF32Smem = static_cast<size_t>(kLinRing) + kLinEpiWarps * kLinEpiBytes + 1024 /*align*/ + 512 /*barriers*/;
 
+// The accumulator is handed back through tensor memory's own fence; nothing in memory goes with it, so the arrival is ordered within
+// the CTA alone. (With a release to the cluster each of these waited for a memory barrier: a slab took four times as long.)
+__device__ __forceinline__ void mbar_arrive_of_pair(uint32_t bar_cluster) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory"); }
+
 struct F32Params {
   int64_t M, N, kp;       // outputs; K rounded up to whole slabs of 64: planes are kp apart
   int a_rows;             // rows of the A box
@@ -40,21 +44,34 @@ __device__ __forceinline__ int scale_exponent(uint32_t bits) {
   const int e = static_cast<int>(bits >> 23);
   return bits == 0u ? 0 : (e == 255 ? 254 : e) - 141;  // 2^-exponent brings the largest magnitude to [2^14, 2^15)
 }
-// v * 2^e for e beyond what one factor can hold; rounded once
-__device__ __forceinline__ float times_two_to(float v, int e) {
-  int h = e >> 1, l = e - h;
-  h = h < -126 ? -126 : h > 127 ? 127 : h;
-  l = l < -126 ? -126 : l > 127 ? 127 : l;
-  return v * __int_as_float((h + 127) << 23) * __int_as_float((l + 127) << 23);
+// 2^exponent of a row or column as two factors, its halves (one cannot hold all of them); of row and column the halves are multiplied
+// with each other first: powers of two, so that a sum is rounded once at most, where the result itself is subnormal
+__device__ __forceinline__ float2 halves_of(uint32_t bits) {
+  const int e = scale_exponent(bits), h = e >> 1;
+  return make_float2(__int_as_float((h + 127) << 23), __int_as_float((e - h + 127) << 23));
+}
+__device__ __forceinline__ float scaled(float v, float2 row, float2 col) { return v * (row.x * col.x) * (row.y * col.y); }
+
+// The gate of eight outputs: a call, since the exact activations are long and a tile's 32 to a thread would not fit the instruction cache
+struct Eight {
+  float v[8];
+};
+__device__ __noinline__ Eight gate_eight(int act, Eight g, Eight u) {
+  gate_act_each(act, [&](auto a) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g.v[e] = a.exact(g.v[e]) * u.v[e];
+  });
+  return g;
 }
 
 template <bool GATED> __device__ __forceinline__ void f32_out(const F32Params& p, float* out, int64_t m, int64_t n, const float* first, const float* second, bool vec) {
-  const int left = p.N - n < 4 ? static_cast<int>(p.N - n) : 4, ea = scale_exponent(p.a_max[m]);
+  const int left = p.N - n < 4 ? static_cast<int>(p.N - n) : 4;
+  const float2 row = halves_of(p.a_max[m]);
   float g[4], u[4], v[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    g[e] = e < left ? times_two_to(first[e], ea + scale_exponent(p.b_max[n + e])) : 0.f;
-    if constexpr (GATED) u[e] = e < left ? times_two_to(second[e], ea + scale_exponent(p.b_max[p.N + n + e])) : 0.f;
+    g[e] = e < left ? scaled(first[e], row, halves_of(p.b_max[n + e])) : 0.f;
+    if constexpr (GATED) u[e] = e < left ? scaled(second[e], row, halves_of(p.b_max[p.N + n + e])) : 0.f;
     v[e] = g[e];
   }
   auto put = [&](float* to, const float* f) {
@@ -257,8 +274,8 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_f32(const __grid_consta
       const int64_t mr0 = static_cast<int64_t>(mb) * kTileM + static_cast<int64_t>(cta_rank) * 128 + q * 32, n0 = static_cast<int64_t>(nb) * kW;
       const int nrows = p.M - mr0 < 32 ? static_cast<int>(p.M - mr0) : 32;
       const int64_t na = n0 + (GATED ? half * 32 : half * 64), nbb = GATED ? na : na + 32;  // first output columns of the two chunks
-      const int ea = lane < nrows ? scale_exponent(p.a_max[mr0 + lane]) : 0;
-      const int e0 = na + lane < p.N ? scale_exponent(p.b_max[na + lane]) : 0, e1 = nbb + lane < p.N ? scale_exponent(p.b_max[(GATED ? p.N : 0) + nbb + lane]) : 0;
+      const float2 row = halves_of(lane < nrows ? p.a_max[mr0 + lane] : 0u);
+      const float2 c0 = halves_of(na + lane < p.N ? p.b_max[na + lane] : 0u), c1 = halves_of(nbb + lane < p.N ? p.b_max[(GATED ? p.N : 0) + nbb + lane] : 0u);
       float sum[64];
 #pragma unroll
       for (int e = 0; e < 64; ++e) sum[e] = 0.f;
@@ -277,7 +294,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_f32(const __grid_consta
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if (kPair) mbar_arrive_cluster(tempty_target + 8u * acc);
+          if (kPair) mbar_arrive_of_pair(tempty_target + 8u * acc);
           else mbar_arrive(tempty_bar(acc));
         }
 #pragma unroll
@@ -297,14 +314,18 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_f32(const __grid_consta
         }
         break;
       }
-      // the columns' exponents, one to a lane so far, to every lane by way of the staging buffer
-      int* shared = reinterpret_cast<int*>(mine);
+      // the columns' factors, one to a lane so far, to every lane by way of the staging buffer
+      float2* shared = reinterpret_cast<float2*>(mine);
       __syncwarp();
-      shared[lane] = e0;
-      shared[32 + lane] = e1;
+      shared[lane] = c0;
+      shared[32 + lane] = c1;
       __syncwarp();
 #pragma unroll
-      for (int e = 0; e < 64; ++e) sum[e] = times_two_to(sum[e], ea + shared[e]);
+      for (int e = 0; e < 64; e += 2) {
+        const float4 c = *reinterpret_cast<const float4*>(shared + e);
+        sum[e] = scaled(sum[e], row, make_float2(c.x, c.y));
+        sum[e + 1] = scaled(sum[e + 1], row, make_float2(c.z, c.w));
+      }
       if (nrows <= 0) continue;
       const int wide0 = p.N - na < 32 ? static_cast<int>(p.N - na) : 32, wide1 = p.N - nbb < 32 ? static_cast<int>(p.N - nbb) : 32;
       if constexpr (GATED) {
@@ -314,10 +335,18 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_f32(const __grid_consta
           lin_store<float>(sum, mine, side, 2 * p.N, nrows, wide0, vec, lane);
           lin_store<float>(sum + 32, mine, side + p.N, 2 * p.N, nrows, wide0, vec, lane);
         }
-        gate_act_each(p.act, [&](auto act) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) sum[e] = act.exact(sum[e]) * sum[32 + e];
-        });
+        for (int e = 0; e < 32; e += 8) {
+          Eight g, u;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            g.v[i] = sum[e + i];
+            u.v[i] = sum[32 + e + i];
+          }
+          g = gate_eight(p.act, g, u);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[e + i] = g.v[i];
+        }
         lin_store<float>(sum, mine, out + mr0 * p.N + na, p.N, nrows, wide0, vec, lane);
       } else {
         if (wide0 > 0) lin_store<float>(sum, mine, out + mr0 * p.N + na, p.N, nrows, wide0, vec, lane);
@@ -382,37 +411,48 @@ struct F32Operand {
   uint32_t* most;         // [rows]
   int64_t rows, K, kp, s_r, s_k;
 };
-__device__ __forceinline__ void planes_of(float x, int e, __half& h, __half& l) {
-  const float y = times_two_to(x, -e);
-  h = __float2half_rn(y);
-  l = __float2half_rn(y - __half2float(h));
+// 2^-exponent as two factors (one cannot hold all of them)
+struct ToScale {
+  float a, b;
+  __device__ __forceinline__ explicit ToScale(uint32_t most) {
+    const int e = -scale_exponent(most), h = e >> 1;
+    a = __int_as_float((h + 127) << 23);
+    b = __int_as_float((e - h + 127) << 23);
+  }
+};
+__device__ __forceinline__ void planes_of(float x0, float x1, const ToScale& s, __half2& h, __half2& l) {
+  const float y0 = x0 * s.a * s.b, y1 = x1 * s.a * s.b;
+  h = __floats2half2_rn(y0, y1);
+  const float2 f = __half22float2(h);
+  l = __floats2half2_rn(y0 - f.x, y1 - f.y);
 }
 
 // Rows along K: a CTA to a row, read once where it fits into registers (NV pairs of elements to a thread), twice else (NV = 0). Both
-// operands in one launch, the first `rows0` CTAs taking the one.
-template <int NV> __global__ void __launch_bounds__(256) split_rows(F32Operand A, F32Operand B, unsigned rows0) {
+// operands in one launch, the first `rows0` CTAs taking the one. UNIT: the elements of every row are contiguous.
+template <int NV, bool UNIT> __global__ void __launch_bounds__(256) split_rows(F32Operand A, F32Operand B, unsigned rows0) {
   __shared__ uint32_t part[8];
-  next_grid_may_start();  // (the product's CTAs set themselves up meanwhile)
+  next_grid_may_start();
+  after_grids_before();
   const bool second = blockIdx.x >= rows0;
   const F32Operand& P = second ? B : A;
-  const int64_t r = second ? blockIdx.x - rows0 : blockIdx.x, K = P.K, kp = P.kp;
+  const int64_t r = second ? blockIdx.x - rows0 : blockIdx.x, s_k = UNIT ? 1 : P.s_k;
+  const int K = static_cast<int>(P.K), kp = static_cast<int>(P.kp), first = 2 * static_cast<int>(threadIdx.x);
   const float* x = P.x + r * P.s_r;
-  const int64_t s_k = P.s_k;
-  __half* to = P.to + r * 2 * kp;
+  __half* to = P.to + r * 2 * P.kp;
   float v[NV ? NV : 1][2];
   uint32_t m = 0u;
-  auto fetch = [&](int64_t j, float* f) {
+  auto fetch = [&](int j, float* f) {
     f[0] = j < K ? x[j * s_k] : 0.f;
     f[1] = j + 1 < K ? x[(j + 1) * s_k] : 0.f;
   };
   auto look = [&](const float* f) { m = max(m, max(__float_as_uint(f[0]) & 0x7fffffffu, __float_as_uint(f[1]) & 0x7fffffffu)); };
   if constexpr (NV) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) fetch(2 * (threadIdx.x + k * 256), v[k]);
+    for (int k = 0; k < NV; ++k) fetch(first + k * 512, v[k]);
 #pragma unroll
     for (int k = 0; k < NV; ++k) look(v[k]);
   } else {
-    for (int64_t j = 2 * threadIdx.x; j < K; j += 512) {
+    for (int j = first; j < K; j += 512) {
       fetch(j, v[0]);
       look(v[0]);
     }
@@ -422,22 +462,19 @@ template <int NV> __global__ void __launch_bounds__(256) split_rows(F32Operand A
   __syncthreads();
   m = __reduce_max_sync(0xffffffffu, part[threadIdx.x & 7]);
   if (threadIdx.x == 0) P.most[r] = m;
-  const int e = scale_exponent(m);
-  auto store = [&](int64_t j, const float* f) {
+  const ToScale scale(m);
+  auto store = [&](int j, const float* f) {
     __half2 h, l;
-    planes_of(f[0], e, h.x, l.x);
-    planes_of(f[1], e, h.y, l.y);
+    planes_of(f[0], f[1], scale, h, l);
     *reinterpret_cast<__half2*>(to + j) = h;
     *reinterpret_cast<__half2*>(to + kp + j) = l;
   };
   if constexpr (NV) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int64_t j = 2 * (threadIdx.x + k * 256);
-      if (j < kp) store(j, v[k]);
-    }
+    for (int k = 0; k < NV; ++k)
+      if (first + k * 512 < kp) store(first + k * 512, v[k]);
   } else {
-    for (int64_t j = 2 * threadIdx.x; j < kp; j += 512) {
+    for (int j = first; j < kp; j += 512) {
       fetch(j, v[0]);
       store(j, v[0]);
     }
@@ -446,20 +483,26 @@ template <int NV> __global__ void __launch_bounds__(256) split_rows(F32Operand A
 
 // Operands whose rows are contiguous across K: the largest magnitudes first (most[] is zero before; a maximum does not
 // depend on its order), then tiles of 32 rows by 64 k turned in shared memory.
+constexpr int kLookRows = 128;
 __global__ void __launch_bounds__(256) largest_of_columns(F32Operand A, F32Operand B, unsigned blocks0) {
   __shared__ uint32_t part[8][32];
+  next_grid_may_start();
+  after_grids_before();
   const bool second = blockIdx.x >= blocks0;
   const F32Operand& P = second ? B : A;
-  const int64_t across = (P.rows + 31) / 32, block = second ? blockIdx.x - blocks0 : blockIdx.x;
+  const uint32_t across = static_cast<uint32_t>((P.rows + 31) / 32), block = second ? blockIdx.x - blocks0 : blockIdx.x;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int64_t r = block % across * 32 + tx, k0 = block / across * 256;
+  const int64_t r = static_cast<int64_t>(block % across) * 32 + tx, k0 = static_cast<int64_t>(block / across) * kLookRows + ty;
   uint32_t m = 0u;
   if (r < P.rows) {
-#pragma unroll 8
-    for (int i = 0; i < 32; ++i) {
-      const int64_t k = k0 + ty + 8 * i;
-      if (k < P.K) m = max(m, __float_as_uint(P.x[r * P.s_r + k * P.s_k]) & 0x7fffffffu);
-    }
+    const float* x = P.x + r * P.s_r + k0 * P.s_k;
+    const int64_t step = 8 * P.s_k;
+    const int left = static_cast<int>(P.K - k0 < kLookRows ? P.K - k0 : kLookRows);
+    float v[kLookRows / 8];
+#pragma unroll
+    for (int i = 0; i < kLookRows / 8; ++i, x += step) v[i] = 8 * i < left ? *x : 0.f;
+#pragma unroll
+    for (int i = 0; i < kLookRows / 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
   }
   part[ty][tx] = m;
   __syncthreads();
@@ -472,24 +515,25 @@ __global__ void __launch_bounds__(256) largest_of_columns(F32Operand A, F32Opera
 __global__ void __launch_bounds__(256) split_columns(F32Operand A, F32Operand B, unsigned blocks0) {
   __shared__ float tile[64][33];
   next_grid_may_start();
+  after_grids_before();
   const bool second = blockIdx.x >= blocks0;
   const F32Operand& P = second ? B : A;
-  const int64_t across = (P.rows + 31) / 32, block = second ? blockIdx.x - blocks0 : blockIdx.x;
-  const int64_t r0 = block % across * 32, k0 = block / across * 64;
+  const uint32_t across = static_cast<uint32_t>((P.rows + 31) / 32), block = second ? blockIdx.x - blocks0 : blockIdx.x;
+  const int64_t r0 = static_cast<int64_t>(block % across) * 32, k0 = static_cast<int64_t>(block / across) * 64;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t left = P.K - k0 - ty;  // of K, from this thread's first row on
+  const float* x = P.x + (r0 + tx) * P.s_r + (k0 + ty) * P.s_k;
+  const bool in = r0 + tx < P.rows;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = r0 + tx, k = k0 + ty + 8 * i;
-    tile[ty + 8 * i][tx] = r < P.rows && k < P.K ? P.x[r * P.s_r + k * P.s_k] : 0.f;
-  }
+  for (int i = 0; i < 8; ++i, x += 8 * P.s_k) tile[ty + 8 * i][tx] = in && 8 * i < left ? *x : 0.f;
   __syncthreads();
   const int c = threadIdx.x >> 3, kk = (threadIdx.x & 7) * 8;
   const int64_t r = r0 + c;
   if (r >= P.rows) return;
-  const int e = scale_exponent(P.most[r]);
-  __half h[8], l[8];
+  const ToScale scale(P.most[r]);
+  __half2 h[4], l[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) planes_of(tile[kk + i][c], e, h[i], l[i]);
+  for (int i = 0; i < 4; ++i) planes_of(tile[kk + 2 * i][c], tile[kk + 2 * i + 1][c], scale, h[i], l[i]);
   __half* to = P.to + r * 2 * P.kp + k0 + kk;  // (kp is a multiple of 64)
   *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(h);
   *reinterpret_cast<uint4*>(to + P.kp) = *reinterpret_cast<const uint4*>(l);
@@ -571,6 +615,7 @@ int run_f32(const float* A, const float* B, float* out, int64_t M, int64_t N, in
   // rows that lie along K, and those that lie across it
   F32Operand along[2], across[2];
   int n_along = 0, n_across = 0, launches = 1;
+  cudaError_t le = cudaSuccess;
   for (const F32Operand* o : {&a, &b}) {
     if (o->s_k == 1 || (o->s_r != 1 && o->rows > 1)) along[n_along++] = *o;
     else across[n_across++] = *o;
@@ -580,18 +625,23 @@ int run_f32(const float* A, const float* B, float* out, int64_t M, int64_t N, in
     if (e != cudaSuccess) { set_last_cuda_error(e); return B200_ELAUNCH; }
     if (n_across == 1) across[1] = F32Operand{};
     auto blocks = [&](int i, int64_t step, int64_t k) { return i < n_across ? (across[i].rows + 31) / 32 * ((k + step - 1) / step) : 0; };
-    largest_of_columns<<<static_cast<unsigned>(blocks(0, 256, K) + blocks(1, 256, K)), 256, 0, st>>>(across[0], across[1], static_cast<unsigned>(blocks(0, 256, K)));
-    split_columns<<<static_cast<unsigned>(blocks(0, 64, kp) + blocks(1, 64, kp)), 256, 0, st>>>(across[0], across[1], static_cast<unsigned>(blocks(0, 64, kp)));
+    le = launch_after(largest_of_columns, blocks(0, kLookRows, K) + blocks(1, kLookRows, K), 256, 0, st, across[0], across[1], static_cast<unsigned>(blocks(0, kLookRows, K)));
+    if (le == cudaSuccess) le = launch_after(split_columns, blocks(0, 64, kp) + blocks(1, 64, kp), 256, 0, st, across[0], across[1], static_cast<unsigned>(blocks(0, 64, kp)));
     launches += 2;
   }
   if (n_along) {
     if (n_along == 1) along[1] = F32Operand{};
     const unsigned grid = static_cast<unsigned>(along[0].rows + along[1].rows), rows0 = static_cast<unsigned>(along[0].rows);
-    if (kp <= 1024) split_rows<2><<<grid, 256, 0, st>>>(along[0], along[1], rows0);
-    else if (kp <= 4096) split_rows<8><<<grid, 256, 0, st>>>(along[0], along[1], rows0);
-    else split_rows<0><<<grid, 256, 0, st>>>(along[0], along[1], rows0);
+    const bool unit = along[0].s_k == 1 && (n_along == 1 || along[1].s_k == 1);
+    auto go = [&](auto kernel) {
+      if (le == cudaSuccess) le = launch_after(kernel, grid, 256, 0, st, along[0], along[1], rows0);
+    };
+    if (kp <= 1024) unit ? go(split_rows<2, true>) : go(split_rows<2, false>);
+    else if (kp <= 4096) unit ? go(split_rows<8, true>) : go(split_rows<8, false>);
+    else unit ? go(split_rows<0, true>) : go(split_rows<0, false>);
     ++launches;
   }
+  if (le != cudaSuccess) { set_last_cuda_error(le); return B200_ELAUNCH; }
   F32Params p{};
   p.M = M;
   p.N = N;
