@@ -697,7 +697,7 @@ using namespace b200;
 // (below, the package's other fp32 products take the call).
 extern "C" int64_t b200_linear_f32_scratch_bytes(int64_t M, int64_t N, int64_t K) {
   if (!f32_sizes(M, N, K) || !encode_fn()) return 0;
-  if (M <= 64 || N <= 64 || K < 32 || static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K) < 67108864.) return 0;
+  if (M <= 32 || N <= 32 || K < 32 || static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K) < 67108864.) return 0;
   return f32_scratch(M, N, K);
 }
 

@@ -480,7 +480,8 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
 }
 
 // ------------------------------------------------------------------ operands off the grid
-// A matrix [rows, K] of any strides into rows along K with a pitch that is a multiple of 16 bytes, for the copy engine.
+// A matrix [rows, K] of any strides into rows along K for the copy engine, which wants a pitch that is a multiple of 16 bytes, and is
+// faster where no slab of a row lies across two lines.
 //
 // Rows that lie along K, off the 16-byte grid: a thread to 16 bytes of the result, from the one or two aligned blocks that its bytes
 // lie in, shifted into place. A block holds a byte of the matrix or is not read, so that no load leaves the
@@ -489,8 +490,8 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
 struct PackRows {
   const unsigned char* x;
   unsigned char* to;
-  int64_t rows, row_bytes, s_bytes;
-  uint32_t pieces;  // of sixteen bytes to a row of the result
+  int64_t rows, row_bytes, s_bytes, pitch;  // (the last: bytes)
+  uint32_t pieces;  // of sixteen bytes that a row's elements take
 };
 __global__ void __launch_bounds__(256) pack_rows_shifted(PackRows A, PackRows B, unsigned blocks0) {
   next_grid_may_start();  // (the product's CTAs set themselves up meanwhile)
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(256) pack_rows_shifted(PackRows A, PackRows B,
       const uint32_t a = skip & 1u ? w[k + 1 < 8 ? k + 1 : 7] : w[k], b = skip & 1u ? w[k + 3 < 8 ? k + 3 : 7] : w[k + 2 < 8 ? k + 2 : 7];
       v[k] = skip & 2u ? b : a;
     }
-    *reinterpret_cast<uint4*>(to + i * 16) = make_uint4(__funnelshift_r(v[0], v[1], bits), __funnelshift_r(v[1], v[2], bits), __funnelshift_r(v[2], v[3], bits), __funnelshift_r(v[3], v[4], bits));
+    *reinterpret_cast<uint4*>(to + r * P.pitch + j * 16) = make_uint4(__funnelshift_r(v[0], v[1], bits), __funnelshift_r(v[1], v[2], bits), __funnelshift_r(v[2], v[3], bits), __funnelshift_r(v[3], v[4], bits));
   }
 }
 
@@ -547,10 +548,21 @@ struct LinOperand {
   const void* base;
   int64_t rows, K, s_r, s_k;
   int esize;
-  bool ready() const {  // as the copy engine takes it
-    return aligned16(base) && (s_k == 1 || K == 1) && (rows == 1 || (s_r >= K && s_r * esize % 16 == 0));
+  int64_t reads;  // how many tiles read a row
+  bool ready() const {  // as the copy engine takes it, and a copy would not pay
+    return aligned16(base) && (s_k == 1 || K == 1) && (rows == 1 || (s_r >= K && s_r * esize % 16 == 0)) && !better_copied();
   }
-  int64_t pitch() const { return (K * esize + 15) / 16 * 16 / esize; }
+  // Rows on the 16-byte grid but across lines of 128: every slab of a row that a tile reads takes a second line, 4.5 ps of the whole device
+  // each time (2.9 to 6.7 over nine sizes); a copy takes 3e-5 us a slab once, more where it does not fit into L2, and a launch. bf16 gated 8192 x 4088 x 11008:
+  // 1345 us as they are, 1046 copied, 914 with rows on lines; 512 x 4088 x 11008 107, 87 with the input alone copied, 76; 128 x 2040 x 5504 stays at 17 (14), where copies
+  // would make it 29.
+  bool better_copied() const {
+    const bool lines = (reinterpret_cast<uintptr_t>(base) & 127u) == 0 && (rows == 1 || s_r * esize % 128 == 0);
+    if (lines || rows == 1 || K * esize <= 128) return false;
+    const double slabs = static_cast<double>(rows) * static_cast<double>((K * esize + kSlabBytes - 1) / kSlabBytes);
+    return slabs * (4.5e-6 * static_cast<double>(reads) - (slabs * kSlabBytes > 64e6 ? 4.5e-5 : 3e-5)) > 1.5;
+  }
+  int64_t pitch() const { return K * esize > 128 ? (K * esize + 127) / 128 * 128 / esize : (K * esize + 15) / 16 * 16 / esize; }
   int64_t packed_bytes() const { return ready() ? 0 : (rows * pitch() * esize + 255) / 256 * 256; }
 };
 
@@ -567,8 +579,8 @@ void pack(LinOperand& a, LinOperand& b, unsigned char* at, cudaStream_t st, int&
     }
     const int64_t pitch = o->pitch(), bytes = o->packed_bytes();
     if (o->s_k == 1 || o->K == 1) {
-      const int64_t pieces = pitch * o->esize / 16, needed = (o->rows * pieces + 255) / 256;
-      rows[n] = PackRows{static_cast<const unsigned char*>(o->base), at, o->rows, o->K * o->esize, o->s_r * o->esize, static_cast<uint32_t>(pieces)};
+      const int64_t pieces = (o->K * o->esize + 15) / 16, needed = (o->rows * pieces + 255) / 256;
+      rows[n] = PackRows{static_cast<const unsigned char*>(o->base), at, o->rows, o->K * o->esize, o->s_r * o->esize, pitch * o->esize, static_cast<uint32_t>(pieces)};
       blocks[n++] = static_cast<unsigned>(needed < most ? needed : most);
     } else {
       const int64_t tiles = ((o->rows + 31) / 32) * ((o->K + 31) / 32);
@@ -701,11 +713,25 @@ int launch_linear(int cluster, int64_t ctas, cudaStream_t st, const CUtensorMap&
   return B200_OK;
 }
 
+struct LinOperands {
+  LinOperand a, b;
+  LinPlan plan;
+  // a is [M, K], b [per N, K]
+  LinOperands(const void* A, const void* B, int64_t M, int64_t N, int64_t K, int64_t sAm, int64_t sAk, int64_t sBn, int64_t sBk, int per, int esize)
+      : a{A, M, K, sAm, sAk, esize, 0}, b{B, per * N, K, sBn, sBk, esize, 0}, plan(plan_linear(M, N, K, per, kSlabBytes / esize)) {
+    const int tile_m = plan.share == kPaired ? 256 : 128;
+    a.reads = (N + plan.w - 1) / plan.w;
+    b.reads = (M + tile_m - 1) / tile_m;
+  }
+  int64_t packed_bytes() const { return a.packed_bytes() + b.packed_bytes(); }
+};
+
 template <int MODE>
-int run_linear(LinOperand a, LinOperand b, void* out, int64_t M, int64_t N, int64_t K, int dtype_out, bool is_bf16, LinParams& p, void* scratch, int64_t scratch_bytes, uint32_t* status, cudaStream_t st) {
+int run_linear(LinOperands ops, void* out, int64_t M, int64_t N, int64_t K, int dtype_out, bool is_bf16, LinParams& p, void* scratch, int64_t scratch_bytes, uint32_t* status, cudaStream_t st) {
   constexpr int per = MODE == kGated ? 2 : 1;
+  LinOperand &a = ops.a, &b = ops.b;
   if (!encode_fn()) return B200_EDRIVER;
-  const int64_t need = a.packed_bytes() + b.packed_bytes();
+  const int64_t need = ops.packed_bytes();
   if (need && (!scratch || scratch_bytes < need + 256)) return B200_ESCRATCH;
   unsigned char* at = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(scratch) + 255) & ~static_cast<uintptr_t>(255));
   int launches = 1;
@@ -751,9 +777,8 @@ int run_linear(LinOperand a, LinOperand b, void* out, int64_t M, int64_t N, int6
     if constexpr (MODE == kInt8) return go(static_cast<float*>(out));
     return B200_EDTYPE;
   };
-  const LinPlan plan = plan_linear(M, N, K, per, p.k_step);
-  int rc = run(plan);
-  if (rc == B200_ELAUNCH && plan.share != kSingle) {
+  int rc = run(ops.plan);
+  if (rc == B200_ELAUNCH && ops.plan.share != kSingle) {
     // the cluster launch was refused (a device or a partition without thread-block clusters): the same on single CTAs
     (void)cudaGetLastError();
     rc = run(LinPlan{kSingle, 256 / per, M >= 128 ? 128 : static_cast<int>((M + 7) / 8 * 8), 1});
@@ -777,7 +802,7 @@ using namespace b200;
 
 extern "C" int64_t b200_gated_linear_scratch_bytes(const void* x, const void* w, int64_t M, int64_t N, int64_t K, int64_t sxm, int64_t sxk, int64_t swn, int64_t swk) {
   if (M < 1 || N < 1 || K < 1) return 0;
-  const int64_t need = LinOperand{x, M, K, sxm, sxk, 2}.packed_bytes() + LinOperand{w, 2 * N, K, swn, swk, 2}.packed_bytes();
+  const int64_t need = LinOperands(x, w, M, N, K, sxm, sxk, swn, swk, 2, 2).packed_bytes();
   return need ? need + 256 : 0;
 }
 
@@ -798,12 +823,12 @@ extern "C" int b200_gated_linear(const void* x, const void* w, void* out, float*
   LinParams p{};
   p.act = activation;
   p.side = projections;
-  return run_linear<kGated>(LinOperand{x, M, K, sxm, sxk, 2}, LinOperand{w, 2 * N, K, swn, swk, 2}, out, M, N, K, dtype, dtype == B200_BF16, p, scratch, scratch_bytes, status, st);
+  return run_linear<kGated>(LinOperands(x, w, M, N, K, sxm, sxk, swn, swk, 2, 2), out, M, N, K, dtype, dtype == B200_BF16, p, scratch, scratch_bytes, status, st);
 }
 
 extern "C" int64_t b200_mm_int8_scratch_bytes(const void* A, const void* B, int64_t M, int64_t N, int64_t K, int64_t sAm, int64_t sAk, int64_t sBk, int64_t sBn) {
   if (M < 1 || N < 1 || K < 1) return 0;
-  const int64_t need = LinOperand{A, M, K, sAm, sAk, 1}.packed_bytes() + LinOperand{B, N, K, sBn, sBk, 1}.packed_bytes();
+  const int64_t need = LinOperands(A, B, M, N, K, sAm, sAk, sBn, sBk, 1, 1).packed_bytes();
   return need ? need + 256 : 0;
 }
 
@@ -826,5 +851,5 @@ extern "C" int b200_mm_int8(const void* A, const void* B, const float* a_scale, 
   p.a_scale = a_scale;
   p.b_scale = b_scale;
   p.bias = bias;
-  return run_linear<kInt8>(LinOperand{A, M, K, sAm, sAk, 1}, LinOperand{B, N, K, sBn, sBk, 1}, out, M, N, K, dtype_out, false, p, scratch, scratch_bytes, status, st);
+  return run_linear<kInt8>(LinOperands(A, B, M, N, K, sAm, sAk, sBn, sBk, 1, 1), out, M, N, K, dtype_out, false, p, scratch, scratch_bytes, status, st);
 }

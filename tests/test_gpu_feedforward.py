@@ -690,3 +690,85 @@ def test_offsets_beyond_32_bits():
     out = K.mm_int8(q, w8.t(), s, torch.ones(8, device=DEV), out_dtype=F32)
     want = (q[-130:].double() @ w8.double().t()) * s[-130:].double()[:, None]
     ref.assert_within(out[-130:], want, 2.0**-22 * want.abs() + 1e-30, "int8")
+
+
+# ------------------------------------------------------------------ rows that lie across lines, threads, captured gradients
+def _on_lines(t, offset):
+    """The values of t in rows a multiple of 128 bytes apart, the first `offset` bytes behind a line."""
+    size = t.element_size()
+    wide = torch.empty(t.shape[0], (t.shape[1] * size + offset + 127) // 128 * 128 // size, dtype=t.dtype, device=t.device)
+    return wide[:, offset // size : offset // size + t.shape[1]].copy_(t)
+
+
+@pytest.mark.parametrize("size", [(4000, 1000, 2500), (1000, 1000, 6000), (8000, 1000, 520), (300, 200, 96)], ids=["both", "input", "weight", "neither"])
+def test_rows_across_lines_of_memory(size):
+    """Rows on the 16-byte grid that start anywhere in a line are copied where many tiles read them: the same bits either way."""
+    M, k, F = size
+    x, w = _pair(M, k, F, BF)
+    h, th, _, _ = ref.gated(x[-200:], w, "silu", BF)
+    want = K.gated_linear(_on_lines(x, 0), _on_lines(w, 0))
+    ref.assert_within(want[-200:], h, th, "h")
+    assert bits_equal(K.gated_linear(x, w), want)
+    assert bits_equal(K.gated_linear(_on_lines(x, 16), _on_lines(w, 48)), want)
+    k8 = 2 * k + 16  # 2016 and 416 bytes
+    a, b, sa, sb = _int8(M, k8), _int8(2 * F, k8), torch.rand(M, device=DEV) + 0.5, torch.rand(2 * F, device=DEV) + 0.5
+    want = K.mm_int8(_on_lines(a, 0), _on_lines(b, 0).t(), sa, sb, out_dtype=F32)
+    exact = (a[-200:].double() @ b.double().t()) * sa[-200:].double()[:, None] * sb.double()
+    ref.assert_within(want[-200:], exact, 2.0**-22 * exact.abs() + 1e-30, "int8")  # three roundings of 2^-24
+    assert bits_equal(K.mm_int8(a, b.t(), sa, sb, out_dtype=F32), want)
+    assert bits_equal(K.mm_int8(_on_lines(a, 16), _on_lines(b, 112).t(), sa, sb, out_dtype=F32), want)
+
+
+@without_bands
+def test_calls_of_several_threads_at_once():
+    """Four threads, each on a stream of its own, with calls that need scratch and calls of other sizes in between."""
+    import threading
+
+    cases = [_all_args(odd=3), _all_args(), _all_args(M=300, k=1000, F=200, dtype=F32), _all_args(M=70, k=264, F=88)]
+    wants = [_all_calls(*args) for args in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(first):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got = [(i % 4, _all_calls(*cases[i % 4])) for i in range(first, first + 12)]
+                torch.cuda.current_stream().synchronize()
+            wrong.extend(i for i, g in got if not all(bits_equal(a, b) for a, b in zip(g, wants[i])))
+        except Exception as e:
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@without_bands
+def test_gradients_captured_through_autograd():
+    """A forward and backward pass through the autograd formulas in one graph, replayed with new contents."""
+    x, w = _pair(96, 128, 48, BF)
+    x.requires_grad_(), w.requires_grad_()
+    state, dy = _state(3, 0), _randn(96, 48, dtype=BF, seed=5)
+
+    def step():
+        y = K.dropout(K.gated_linear(x, w), 0.25, state)
+        return (y, *torch.autograd.grad(y, (x, w), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(2):
+        with torch.no_grad():
+            x.copy_(_randn(96, 128, dtype=BF, seed=30 + seed))
+        state[1] = 1000 * seed
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(bits_equal(a, b) for a, b in zip(out, step())), seed
