@@ -485,7 +485,70 @@ template <int NV, bool UNIT> __global__ void __launch_bounds__(256) split_rows(F
   }
 }
 
-// Operands whose rows are contiguous across K: the largest magnitudes first (most[] is zero before; a maximum does not
+// Operands whose rows are contiguous across K, read once: a cluster to 32 rows, each of its CTAs with a range of `slabs` times 64 k in
+// shared memory, where the largest magnitudes are found, exchanged, and the planes written from.
+constexpr int kOncePitch = 33, kOnceMost = 26;  // slabs of 64 x 33 values that fit into an SM's shared memory
+__global__ void __launch_bounds__(256) split_columns_once(F32Operand A, F32Operand B, unsigned tiles0, int ctas, int slabs) {
+  extern __shared__ float once_tile[];
+  __shared__ uint32_t part[8][32], largest[32];
+  next_grid_may_start();
+  after_grids_before();
+  const unsigned t = blockIdx.x / static_cast<unsigned>(ctas), rank = blockIdx.x % static_cast<unsigned>(ctas);
+  const bool second = t >= tiles0;
+  const F32Operand& P = second ? B : A;
+  const int64_t r0 = static_cast<int64_t>(second ? t - tiles0 : t) * 32, k0 = static_cast<int64_t>(rank) * slabs * 64;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int count = static_cast<int>(P.kp - k0 < slabs * 64 ? P.kp - k0 : slabs * 64);  // (a multiple of 64; 0 or less: none)
+  const int64_t left = r0 + tx < P.rows ? P.K - k0 : 0;
+  const float* x = P.x + (r0 + tx) * P.s_r + (k0 + ty) * P.s_k;
+  uint32_t m = 0u;
+  for (int base = ty; base < count; base += 128) {
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i, x += 8 * P.s_k) v[i] = base + 8 * i < left && base + 8 * i < count ? *x : 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+      if (base + 8 * i < count) once_tile[(base + 8 * i) * kOncePitch + tx] = v[i];
+    }
+  }
+  part[ty][tx] = m;
+  __syncthreads();
+  if (ty == 0) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = max(m, part[i][tx]);
+    largest[tx] = m;
+  }
+  const int c = threadIdx.x >> 3;
+  const int64_t r = r0 + c;
+  if (ctas > 1) {
+    cluster_sync_all();
+    m = 0u;
+    for (int i = 0; i < ctas; ++i) {
+      uint32_t of;
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(of) : "r"(map_to_cta(smem_u32(&largest[c]), static_cast<uint32_t>(i))) : "memory");
+      m = max(m, of);
+    }
+  } else {
+    __syncthreads();
+    m = largest[c];
+  }
+  if (r < P.rows) {
+    if (rank == 0 && (threadIdx.x & 7) == 0) P.most[r] = m;
+    const ToScale scale(m);
+    __half* to = P.to + r * 2 * P.kp + k0;
+    for (int kk = (threadIdx.x & 7) * 8; kk < count; kk += 64) {
+      __half2 h[4], l[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) planes_of(once_tile[(kk + 2 * i) * kOncePitch + c], once_tile[(kk + 2 * i + 1) * kOncePitch + c], scale, h[i], l[i]);
+      *reinterpret_cast<uint4*>(to + kk) = *reinterpret_cast<const uint4*>(h);
+      *reinterpret_cast<uint4*>(to + P.kp + kk) = *reinterpret_cast<const uint4*>(l);
+    }
+  }
+  if (ctas > 1) cluster_sync_all();  // nobody leaves while another reads its largest
+}
+
+// Longer ones, read twice: the largest magnitudes first (most[] is zero before; a maximum does not
 // depend on its order), then tiles of 32 rows by 64 k turned in shared memory.
 constexpr int kLookRows = 128;
 __global__ void __launch_bounds__(256) largest_of_columns(F32Operand A, F32Operand B, unsigned blocks0) {
@@ -610,6 +673,43 @@ int launch_f32(int cluster, int64_t ctas, cudaStream_t st, const CUtensorMap& ma
   return B200_OK;
 }
 
+// Eight slabs to a CTA, or fewer where that makes fewer than two CTAs to an SM. `done` stays false where the columns are too long for a
+// cluster, or the cluster is refused.
+cudaError_t launch_once(const F32Operand* across, int64_t tiles0, int64_t tiles, int64_t slabs, cudaStream_t st, bool& done) {
+  int64_t ctas = (slabs + 7) / 8;
+  if (tiles * ctas < 2 * kNumSMs) ctas = (2 * kNumSMs + tiles - 1) / tiles;
+  ctas = ctas < slabs ? ctas : slabs;
+  ctas = ctas < 8 ? ctas : 8;
+  const int64_t each = (slabs + ctas - 1) / ctas;
+  if (each > kOnceMost || tiles * ctas > 0x7fffffff) return cudaSuccess;
+  static std::atomic<uint64_t> allowed{0};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (e == cudaSuccess && !(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(split_columns_once, cudaFuncAttributeMaxDynamicSharedMemorySize, kOnceMost * 64 * kOncePitch * 4);
+    if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * ctas));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = static_cast<size_t>(each) * 64 * kOncePitch * 4;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // (see launch_after)
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 2 : 1;
+  done = cudaLaunchKernelEx(&cfg, split_columns_once, across[0], across[1], static_cast<unsigned>(tiles0), static_cast<int>(ctas), static_cast<int>(each)) == cudaSuccess;
+  if (!done) (void)cudaGetLastError();
+  return cudaSuccess;
+}
+
 template <bool GATED>
 int run_f32(const float* A, const float* B, float* out, int64_t M, int64_t N, int64_t K, int64_t sAm, int64_t sAk, int64_t sBn, int64_t sBk, int act, float* side, void* scratch, uint32_t* status, cudaStream_t st) {
   if (!encode_fn()) return B200_EDRIVER;
@@ -626,10 +726,17 @@ int run_f32(const float* A, const float* B, float* out, int64_t M, int64_t N, in
     if (o->s_k == 1 || (o->s_r != 1 && o->rows > 1)) along[n_along++] = *o;
     else across[n_across++] = *o;
   }
+  bool once = false;
   if (n_across) {
+    if (n_across == 1) across[1] = F32Operand{};
+    const int64_t tiles0 = (across[0].rows + 31) / 32, tiles = tiles0 + (across[1].rows + 31) / 32;
+    const cudaError_t e = launch_once(across, tiles0, tiles, kp / 64, st, once);
+    if (e != cudaSuccess) { set_last_cuda_error(e); return B200_ELAUNCH; }
+    if (once) ++launches;
+  }
+  if (n_across && !once) {
     const cudaError_t e = cudaMemsetAsync(across[0].most, 0, static_cast<size_t>((n_across == 2 ? M + rows_b : across[0].rows) * 4), st);
     if (e != cudaSuccess) { set_last_cuda_error(e); return B200_ELAUNCH; }
-    if (n_across == 1) across[1] = F32Operand{};
     auto blocks = [&](int i, int64_t step, int64_t k) { return i < n_across ? (across[i].rows + 31) / 32 * ((k + step - 1) / step) : 0; };
     le = launch_after(largest_of_columns, blocks(0, kLookRows, K) + blocks(1, kLookRows, K), 256, 0, st, across[0], across[1], static_cast<unsigned>(blocks(0, kLookRows, K)));
     if (le == cudaSuccess) le = launch_after(split_columns, blocks(0, 64, kp) + blocks(1, 64, kp), 256, 0, st, across[0], across[1], static_cast<unsigned>(blocks(0, 64, kp)));
@@ -643,6 +750,7 @@ int run_f32(const float* A, const float* B, float* out, int64_t M, int64_t N, in
       if (le == cudaSuccess) le = launch_after(kernel, grid, 256, 0, st, along[0], along[1], rows0);
     };
     if (kp <= 1024) unit ? go(split_rows<2, true>) : go(split_rows<2, false>);
+    else if (kp <= 2048) unit ? go(split_rows<4, true>) : go(split_rows<4, false>);
     else if (kp <= 4096) unit ? go(split_rows<8, true>) : go(split_rows<8, false>);
     else unit ? go(split_rows<0, true>) : go(split_rows<0, false>);
     ++launches;
