@@ -14,7 +14,7 @@ constexpr int kFfThreads = 256;
 // ------------------------------------------------------------------ the gate
 // h = act(g) * u of fp32 projections P = [g | u] (M x 2 N). fp32 products come in two steps (their sums are
 // put together from six plane products over several launches), so the gate has a kernel of its own there.
-// Backward: dP = [dh * u * act'(g) | dh * act(g)], rounded to the type of the operands it is multiplied by next.
+// Backward: dP = [dh * u * act'(g) | dh * act(g)], rounded to the type of the operands it is multiplied by next, in rows of any pitch.
 template <int N> __device__ __forceinline__ void load_f32(const float* p, float* v) {
 #pragma unroll
   for (int e = 0; e < N; e += 4) widen<float>(ld_stream(p + e), v + e);
@@ -25,12 +25,11 @@ __device__ __forceinline__ int64_t row_of(int64_t i, int64_t per_row, int64_t to
 
 // Rows off the grid: four single elements to a thread, a CTA's width apart and all on their way together (fp32 1531 x 1365 11.1 us
 // with one).
-// Where element span + offset of a matrix of N columns is in P, when element `span` is in row m0 and column c0: past the row's
+// The row of element span + offset of a matrix of N columns, when element `span` is in row m0 and column c0: past the row's
 // end a wide matrix has one more row to go, a narrow one takes a division of small numbers.
-__device__ __forceinline__ int64_t in_pair(int64_t span, int offset, int64_t m0, int64_t c0, int64_t N) {
+__device__ __forceinline__ int64_t row_behind(int offset, int64_t m0, int64_t c0, int64_t N) {
   const int64_t past = c0 + offset;
-  const int64_t rows = N >= 4 * kFfThreads ? (past >= N ? 1 : 0) : static_cast<uint32_t>(past) / static_cast<uint32_t>(N);
-  return span + offset + (m0 + rows) * N;
+  return m0 + (N >= 4 * kFfThreads ? (past >= N ? 1 : 0) : static_cast<uint32_t>(past) / static_cast<uint32_t>(N));
 }
 
 template <typename ACT, bool VECTOR>
@@ -54,7 +53,7 @@ __global__ void __launch_bounds__(kFfThreads) gate_forward(const float* p, float
       float g[4], u[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int64_t i = i0 + e * kFfThreads, at = in_pair(span, static_cast<int>(threadIdx.x) + e * kFfThreads, m0, c0, N);
+        const int64_t i = i0 + e * kFfThreads, at = i + row_behind(static_cast<int>(threadIdx.x) + e * kFfThreads, m0, c0, N) * N;  // (m rows of 2 N, not N, lie before)
         g[e] = i < total ? p[at] : 0.f;
         u[e] = i < total ? p[at + N] : 0.f;
       }
@@ -66,7 +65,7 @@ __global__ void __launch_bounds__(kFfThreads) gate_forward(const float* p, float
 }
 
 template <typename T, typename ACT, bool VECTOR>
-__global__ void __launch_bounds__(kFfThreads) gate_backward(const T* dh, const float* p, T* __restrict__ dp, int64_t M, int64_t N) {
+__global__ void __launch_bounds__(kFfThreads) gate_backward(const T* dh, const float* p, T* __restrict__ dp, int64_t M, int64_t N, int64_t pitch) {
   constexpr int kVec = VECTOR ? 16 / static_cast<int>(sizeof(T)) : 4;
   auto slope = [](float& d, float& g, float& u) {
     float a, s;
@@ -78,34 +77,34 @@ __global__ void __launch_bounds__(kFfThreads) gate_backward(const T* dh, const f
   if constexpr (VECTOR) {
     const int64_t per_row = N / kVec, total = M * per_row;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kFfThreads) {
-      const int64_t at = i * kVec + row_of(i, per_row, total) * N;
+      const int64_t m = row_of(i, per_row, total), at = i * kVec + m * N, to = i * kVec + m * (pitch - N);
       widen<T>(ld_stream(dh + i * kVec), d);
       load_f32<kVec>(p + at, g);
       load_f32<kVec>(p + at + N, u);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) slope(d[e], g[e], u[e]);
-      *reinterpret_cast<uint4*>(dp + at) = narrow<T>(g);  // (both products read it next: not streamed past L2)
-      *reinterpret_cast<uint4*>(dp + at + N) = narrow<T>(u);
+      *reinterpret_cast<uint4*>(dp + to) = narrow<T>(g);  // (both products read it next: not streamed past L2)
+      *reinterpret_cast<uint4*>(dp + to + N) = narrow<T>(u);
     }
   } else {
     const int64_t total = M * N;
     for (int64_t span = static_cast<int64_t>(blockIdx.x) * (4 * kFfThreads); span < total; span += static_cast<int64_t>(gridDim.x) * (4 * kFfThreads)) {
       const int64_t m0 = row_of(span, N, total), c0 = span - m0 * N, i0 = span + threadIdx.x;
-      int64_t at[4];
+      int64_t to[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int64_t i = i0 + e * kFfThreads;
-        at[e] = in_pair(span, static_cast<int>(threadIdx.x) + e * kFfThreads, m0, c0, N);
+        const int64_t i = i0 + e * kFfThreads, m = row_behind(static_cast<int>(threadIdx.x) + e * kFfThreads, m0, c0, N), at = i + m * N;
+        to[e] = i + m * (pitch - N);
         d[e] = i < total ? to_f32(dh[i]) : 0.f;
-        g[e] = i < total ? p[at[e]] : 0.f;
-        u[e] = i < total ? p[at[e] + N] : 0.f;
+        g[e] = i < total ? p[at] : 0.f;
+        u[e] = i < total ? p[at + N] : 0.f;
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (i0 + e * kFfThreads >= total) break;
         slope(d[e], g[e], u[e]);
-        dp[at[e]] = from_f32<T>(g[e]);
-        dp[at[e] + N] = from_f32<T>(u[e]);
+        dp[to[e]] = from_f32<T>(g[e]);
+        dp[to[e] + N] = from_f32<T>(u[e]);
       }
     }
   }
@@ -126,13 +125,13 @@ int launch_gate(const float* p, float* out, int64_t M, int64_t N, int act, cudaS
   return check_launch();
 }
 
-template <typename T> int launch_gate_backward(const void* dh, const float* p, void* out, int64_t M, int64_t N, int act, cudaStream_t st) {
+template <typename T> int launch_gate_backward(const void* dh, const float* p, void* out, int64_t M, int64_t N, int64_t pitch, int act, cudaStream_t st) {
   constexpr int kVec = 16 / sizeof(T);
-  const bool vec = N % kVec == 0 && aligned16(p) && aligned16(out) && aligned16(dh);
+  const bool vec = N % kVec == 0 && pitch % kVec == 0 && aligned16(p) && aligned16(out) && aligned16(dh);
   const int grid = ff_grid(M * N / (vec ? kVec : 4));
   gate_act_each(act, [&](auto a) {
-    if (vec) gate_backward<T, decltype(a), true><<<grid, kFfThreads, 0, st>>>(static_cast<const T*>(dh), p, static_cast<T*>(out), M, N);
-    else gate_backward<T, decltype(a), false><<<grid, kFfThreads, 0, st>>>(static_cast<const T*>(dh), p, static_cast<T*>(out), M, N);
+    if (vec) gate_backward<T, decltype(a), true><<<grid, kFfThreads, 0, st>>>(static_cast<const T*>(dh), p, static_cast<T*>(out), M, N, pitch);
+    else gate_backward<T, decltype(a), false><<<grid, kFfThreads, 0, st>>>(static_cast<const T*>(dh), p, static_cast<T*>(out), M, N, pitch);
   });
   return check_launch();
 }
@@ -527,17 +526,21 @@ extern "C" int b200_gate(const float* projections, float* out, int64_t M, int64_
   return launch_gate(projections, out, M, N, activation, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int b200_gate_backward(const void* grad, const float* projections, void* grad_projections, int64_t M, int64_t N, int activation, int dtype, void* stream) {
-  if (M < 0 || N < 0 || activation < 0 || activation >= B200_ACT_COUNT) return B200_EINVAL;
+extern "C" int b200_gate_backward_rows(const void* grad, const float* projections, void* grad_projections, int64_t row_stride, int64_t M, int64_t N, int activation, int dtype, void* stream) {
+  if (M < 0 || N < 0 || row_stride < 2 * N || activation < 0 || activation >= B200_ACT_COUNT) return B200_EINVAL;
   if (!is_float_dtype(dtype)) return B200_EDTYPE;
   if (M == 0 || N == 0) return B200_OK;
   if (!grad || !projections || !grad_projections) return B200_EINVAL;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case B200_F32: return launch_gate_backward<float>(grad, projections, grad_projections, M, N, activation, st);
-    case B200_BF16: return launch_gate_backward<__nv_bfloat16>(grad, projections, grad_projections, M, N, activation, st);
-    default: return launch_gate_backward<__half>(grad, projections, grad_projections, M, N, activation, st);
+    case B200_F32: return launch_gate_backward<float>(grad, projections, grad_projections, M, N, row_stride, activation, st);
+    case B200_BF16: return launch_gate_backward<__nv_bfloat16>(grad, projections, grad_projections, M, N, row_stride, activation, st);
+    default: return launch_gate_backward<__half>(grad, projections, grad_projections, M, N, row_stride, activation, st);
   }
+}
+
+extern "C" int b200_gate_backward(const void* grad, const float* projections, void* grad_projections, int64_t M, int64_t N, int activation, int dtype, void* stream) {
+  return b200_gate_backward_rows(grad, projections, grad_projections, N < 0 ? 0 : 2 * N, M, N, activation, dtype, stream);
 }
 
 extern "C" int b200_dropout(const void* x, const void* residual, void* out, int64_t n, double p, const int64_t* state, int64_t subsequence, int dtype, void* stream) {

@@ -155,6 +155,9 @@ Tensor ff_product(const Operand& a, const Operand& b, int64_t M, int64_t N, int6
   return taken(r);
 }
 
+// The pitch of dP's rows: on lines of 128 bytes for the copy engine (fp32 ones are split into planes from anywhere)
+int64_t gradient_pitch(int64_t cols, const Tensor& like) { return dt(like) == B200_F32 || cols % 64 == 0 ? cols : cols > 64 ? (cols + 63) / 64 * 64 : (cols + 7) / 8 * 8; }
+
 // (output, projections); an undefined output: the wrapper has to take the call
 std::tuple<Tensor, Tensor> gated_direct(const Tensor& x, const Tensor& w, c10::string_view activation, bool keep) {
   Rows r;
@@ -213,11 +216,27 @@ std::tuple<TensorOpt, TensorOpt> ff_gated_linear_backward(const Tensor& g, const
     const int64_t F = w.size(0) / 2;
     if (r.M && F && r.K && w.scalar_type() == x.scalar_type() && g.scalar_type() == x.scalar_type() && p.scalar_type() == at::kFloat && g.is_contiguous() && p.is_contiguous() &&
         g.sizes() == at::IntArrayRef(with_last(x, F)) && p.sizes() == at::IntArrayRef(with_last(x, 2 * F))) {
-      Tensor dp = new_tensor({r.M, 2 * F}, x.scalar_type(), x);
-      ff_launched(launched("b200_gate_backward", [&, st = stream()] { return api.b200_gate_backward(ptr(g), static_cast<const float*>(ptr(p)), ptr(dp), r.M, F, act, dt(x), st); }));
+      const int64_t pitch = gradient_pitch(2 * F, x);
+      Tensor dp = new_tensor({r.M, pitch}, x.scalar_type(), x);
+      ff_launched(launched("b200_gate_backward_rows", [&, st = stream()] { return api.b200_gate_backward_rows(ptr(g), static_cast<const float*>(ptr(p)), ptr(dp), pitch, r.M, F, act, dt(x), st); }));
       std::tuple<TensorOpt, TensorOpt> out;
-      if (mask[0]) std::get<0>(out) = ff_product(Operand{dp, 0, 2 * F, 1}, Operand{w, 0, w.stride(0), w.stride(1)}, r.M, r.K, 2 * F, x.sizes());
-      if (mask[1]) std::get<1>(out) = ff_product(Operand{dp, 0, 1, 2 * F}, Operand{x, 0, r.s_m, r.s_k}, 2 * F, r.K, r.M, w.sizes());
+      const int64_t ws0 = w.stride(0), ws1 = w.stride(1);
+      const int64_t need = dt(x) != B200_F32 ? api.b200_linear_grads_scratch_bytes(ptr(dp), ptr(x), ptr(w), r.M, 2 * F, r.K, pitch, r.s_m, r.s_k, ws0, ws1) : -1;
+      if (need >= 0) {
+        Tensor dx, dw;
+        if (mask[0]) dx = new_tensor(x.sizes(), x.scalar_type(), x);
+        if (mask[1]) dw = new_tensor({2 * F, r.K}, x.scalar_type(), x);
+        const Tensor s = ff_scratch(x, need);
+        const int rc = api.b200_linear_grads(ptr(dp), ptr(x), ptr(w), ptr(dx), ptr(dw), r.M, 2 * F, r.K, pitch, r.s_m, ws0, dt(x), ptr(s), need, ff_status(x), stream());
+        if (rc != B200_ELAUNCH) {  // (a refused cluster launch: one product after the other)
+          ff_check(rc, "b200_linear_grads");
+          if (mask[0]) std::get<0>(out) = dx;
+          if (mask[1]) std::get<1>(out) = dw;
+          return out;
+        }
+      }
+      if (mask[0]) std::get<0>(out) = ff_product(Operand{dp, 0, pitch, 1}, Operand{w, 0, w.stride(0), w.stride(1)}, r.M, r.K, 2 * F, x.sizes());
+      if (mask[1]) std::get<1>(out) = ff_product(Operand{dp, 0, 1, pitch}, Operand{x, 0, r.s_m, r.s_k}, 2 * F, r.K, r.M, w.sizes());
       return out;
     }
   }

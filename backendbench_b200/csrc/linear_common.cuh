@@ -89,4 +89,29 @@ __device__ __forceinline__ void lin_store(const float* v, unsigned char* mine, T
   }
 }
 
+// An operand [rows, K] that the copy engine reads along K
+struct LinOperand {
+  const void* base;
+  int64_t rows, K, s_r, s_k;
+  int esize;
+  int64_t reads;  // how many tiles read a row
+  bool ready() const {  // as the copy engine takes it, and a copy would not pay
+    return aligned16(base) && (s_k == 1 || K == 1) && (rows == 1 || (s_r >= K && s_r * esize % 16 == 0)) && !better_copied();
+  }
+  // Rows on the 16-byte grid but across lines of 128: every slab of a row that a tile reads takes a second line, 4.5 ps of the whole device
+  // each time (2.9 to 6.7 over nine sizes); a copy takes 3e-5 us a slab once, more where it does not fit into L2, and a launch. bf16 gated 8192 x 4088 x 11008:
+  // 1345 us as they are, 1046 copied, 914 with rows on lines; 512 x 4088 x 11008 107, 87 with the input alone copied, 76; 128 x 2040 x 5504 stays at 17 (14), where copies
+  // would make it 29.
+  bool better_copied() const {
+    const bool lines = (reinterpret_cast<uintptr_t>(base) & 127u) == 0 && (rows == 1 || s_r * esize % 128 == 0);
+    if (lines || rows == 1 || K * esize <= 128) return false;
+    const double slabs = static_cast<double>(rows) * static_cast<double>((K * esize + kSlabBytes - 1) / kSlabBytes);
+    return slabs * (4.5e-6 * static_cast<double>(reads) - (slabs * kSlabBytes > 64e6 ? 4.5e-5 : 3e-5)) > 1.5;
+  }
+  int64_t pitch() const { return K * esize > 128 ? (K * esize + 127) / 128 * 128 / esize : (K * esize + 15) / 16 * 16 / esize; }
+  int64_t packed_bytes() const { return ready() ? 0 : (rows * pitch() * esize + 255) / 256 * 256; }
+};
+// The operands that are not ready are copied behind `at`, and become their copies.
+void lin_pack(LinOperand& a, LinOperand& b, unsigned char* at, cudaStream_t st, int& launches);
+
 }  // namespace b200

@@ -23,6 +23,7 @@ from . import ops
 from ._abi import check, lib
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}  # B200_ACT_*
+ELAUNCH = -3  # B200_ELAUNCH
 INT8_MAX_K = 131071  # B200_INT8_MAX_K: |sum| <= K * 128 * 128 < 2^31
 
 
@@ -150,7 +151,8 @@ def gated_linear_train(input: torch.Tensor, weight: torch.Tensor, activation: st
 def gated_linear_backward(grad_output: torch.Tensor, input: torch.Tensor, weight: torch.Tensor, projections: torch.Tensor, activation: str = "silu", output_mask=(True, True)):
     """(grad_input, grad_weight) of gated_linear, None where `output_mask` is False. With P = [g | u] the
     projections: dP = [grad u act'(g) | grad act(g)] (rounded to the type of the operands: it is one of the two
-    products that follow), grad_input = dP @ weight, grad_weight = dP^T @ input."""
+    products that follow), grad_input = dP @ weight, grad_weight = dP^T @ input, in one launch where one product after the other
+    would leave SMs idle."""
     ops._require_cuda(grad_output, input, weight, projections)
     act = _activation(activation)
     F, K = _pair_args(input, weight, "gated_linear_backward")
@@ -163,12 +165,30 @@ def gated_linear_backward(grad_output: torch.Tensor, input: torch.Tensor, weight
     if not (want_dx or want_dw):
         return None, None
     M = ops._prod(lead)
-    dp = ops._new((M, 2 * F), input.dtype, input.device)
+    J = 2 * F
+    # rows on lines of 128 bytes for the copy engine (fp32 ones are split into planes from anywhere)
+    pitch = J if input.dtype == torch.float32 or J % 64 == 0 else (J + 63) // 64 * 64 if J > 64 else (J + 7) // 8 * 8
+    dp = ops._new((M, pitch), input.dtype, input.device)[:, :J]
     if dp.numel():
         g, p = ops._contig(grad_output), ops._contig(projections)
-        check(lib().b200_gate_backward(g.data_ptr(), p.data_ptr(), dp.data_ptr(), M, F, act, ops._dt(g.dtype), ops._stream_handle()), "b200_gate_backward")
+        check(lib().b200_gate_backward_rows(g.data_ptr(), p.data_ptr(), dp.data_ptr(), pitch, M, F, act, ops._dt(g.dtype), ops._stream_handle()), "b200_gate_backward_rows")
+    x = _as_rows(input)
+    if dp.numel() and dp.dtype != torch.float32:
+        strides = (pitch, x.stride(0), x.stride(1), weight.stride(0), weight.stride(1))
+        need = int(lib().b200_linear_grads_scratch_bytes(dp.data_ptr(), x.data_ptr(), weight.data_ptr(), M, J, K, *strides))
+        if need >= 0:
+            dx = ops._new(input.shape, input.dtype, input.device) if want_dx else None
+            dw = ops._new((J, K), input.dtype, input.device) if want_dw else None
+            scratch = ops._scratch(dp.device, need) if need else None
+            rc = lib().b200_linear_grads(
+                dp.data_ptr(), x.data_ptr(), weight.data_ptr(), dx.data_ptr() if want_dx else None, dw.data_ptr() if want_dw else None, M, J, K, pitch, strides[1], strides[3], ops._dt(dp.dtype),
+                scratch.data_ptr() if need else None, need, ops._status(dp.device).data_ptr(), ops._stream_handle(),
+            )
+            if rc != ELAUNCH:  # (a refused cluster launch: one product after the other)
+                check(rc, "b200_linear_grads")
+                return dx, dw
     dx = _product(dp, weight).view(input.shape) if want_dx else None
-    dw = _product(dp.t(), _as_rows(input)) if want_dw else None
+    dw = _product(dp.t(), x) if want_dw else None
     return dx, dw
 
 

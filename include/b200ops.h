@@ -377,12 +377,23 @@ int b200_gated_linear_f32(const float* x, const float* w, float* out, float* pro
                           int64_t K, int64_t sxm, int64_t sxk, int64_t swn, int64_t swk, int activation,
                           void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream);
 
+/* Both gradients of y = x w^T in one launch (bf16, f16): dx [M, K] = g w and dw [J, K] = g^T x, contiguous, of g [M, J] with rows on the
+ * 16-byte grid, x [M, K] and w [J, K] with rows along K; dx or dw may be NULL, and the other is the same then. b200_linear_grads_scratch_bytes is -1 where one product after the other is the
+ * better way (few tiles with a long contraction, or small matrices) or an operand lies otherwise. */
+int64_t b200_linear_grads_scratch_bytes(const void* g, const void* x, const void* w, int64_t M, int64_t J, int64_t K,
+                                        int64_t sgm, int64_t sxm, int64_t sxk, int64_t swj, int64_t swk);
+int b200_linear_grads(const void* g, const void* x, const void* w, void* dx, void* dw, int64_t M, int64_t J,
+                      int64_t K, int64_t sgm, int64_t sxm, int64_t swj, int dtype, void* scratch,
+                      int64_t scratch_bytes, uint32_t* status, void* stream);
+
 /* The gate by itself (fp32, whose products come in several launches), and its gradient, for contiguous fp32
  * projections [M, 2 N] = [g | u]: out = act(g) * u;  grad_projections = [grad * u * act'(g) | grad * act(g)], grad and
- * grad_projections of any float dtype. */
+ * grad_projections of any float dtype; the last form with rows of grad_projections row_stride elements apart. */
 int b200_gate(const float* projections, float* out, int64_t M, int64_t N, int activation, void* stream);
 int b200_gate_backward(const void* grad, const float* projections, void* grad_projections, int64_t M,
                        int64_t N, int activation, int dtype, void* stream);
+int b200_gate_backward_rows(const void* grad, const float* projections, void* grad_projections,
+                            int64_t row_stride, int64_t M, int64_t N, int activation, int dtype, void* stream);
 
 /* out[i] = residual[i] + (word(i) >= round(p 2^32) ? x[i] / (1 - p) : 0) for n contiguous elements (residual
  * may be NULL). word(i) is word i % 4 of Philox-4x32 with ten rounds for the counter (state[1] + i / 4, subsequence)

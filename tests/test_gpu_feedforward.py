@@ -772,3 +772,49 @@ def test_gradients_captured_through_autograd():
         graph.replay()
         torch.cuda.synchronize()
         assert all(bits_equal(a, b) for a, b in zip(out, step())), seed
+
+
+# ------------------------------------------------------------------ both gradients in one launch
+def _takes(M, F, x, w):
+    J, k = 2 * F, x.shape[1]
+    dp = torch.empty(M, (J + 63) // 64 * 64, dtype=x.dtype, device=DEV)
+    return feedforward.lib().b200_linear_grads_scratch_bytes(dp.data_ptr(), x.data_ptr(), w.data_ptr(), M, J, k, dp.stride(0), x.stride(0), x.stride(1), w.stride(0), w.stride(1)) >= 0
+
+
+@pytest.mark.parametrize("dtype", [BF, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("size", [(129, 72, 68), (130, 1000, 520), (256, 256, 128), (300, 267, 1000), (777, 520, 1003), (2500, 512, 300), (2000, 1000, 400), (513, 4096, 2752), (2752, 2048, 1280), (1536, 2048, 2048)], ids=str)
+def test_both_gradients_in_one_launch(size, dtype):
+    """dx and dW against 64 bits, sizes whose tiles are ragged, of one part alone, with the longer contraction on either side."""
+    M, k, F = size
+    x, w = _pair(M, k, F, dtype)
+    if k % 2 == 0:
+        x, w = _on_lines(x, 0), _on_lines(w, 16)  # (an odd K is copied to the grid)
+    dh = _randn(M, F, dtype=dtype, seed=3)
+    _, projections = K.gated_linear_train(x, w)
+    dx, tx, dw, tw = ref.gated_grads(dh, x, w, projections, "silu", dtype)
+    assert _takes(M, F, x, w)
+    gx, gw = K.gated_linear_backward(dh, x, w, projections)
+    ref.assert_within(gx, dx, tx, "dx")
+    ref.assert_within(gw, dw, tw, "dW")
+    again = K.gated_linear_backward(dh, x, w, projections)
+    assert bits_equal(gx, again[0]) and bits_equal(gw, again[1])
+    # one gradient at a time is the same; operands that the launch does not take have products of their own
+    one, other = K.gated_linear_backward(dh, x, w, projections, "silu", [True, False])[0], K.gated_linear_backward(dh, x, w, projections, "silu", [False, True])[1]
+    assert bits_equal(one, gx) and bits_equal(other, gw)
+    wt = w.t().contiguous().t()
+    assert not _takes(M, F, x, wt)
+    ref.assert_within(K.gated_linear_backward(dh, x, wt, projections)[0], dx, tx, "dx of a turned weight")
+
+
+def test_gradients_that_are_not_finite_stay_in_their_rows():
+    M, k, F = 400, 264, 304
+    x, w = _pair(M, k, F, BF)
+    dh = _randn(M, F, dtype=BF, seed=3)
+    _, projections = K.gated_linear_train(x, w)
+    assert _takes(M, F, x, w)
+    cx, cw = K.gated_linear_backward(dh, x, w, projections)
+    dh[33, 20] = float("nan")
+    gx, gw = K.gated_linear_backward(dh, x, w, projections)
+    rows, ups = [i for i in range(M) if i != 33], [i for i in range(2 * F) if i not in (20, F + 20)]
+    assert gx[33].isnan().all() and bits_equal(gx[rows], cx[rows])
+    assert gw[[20, F + 20]].isnan().all() and bits_equal(gw[ups], cw[ups])
