@@ -23,8 +23,8 @@ __device__ __forceinline__ int64_t row_of(int64_t i, int64_t per_row, int64_t to
   return total <= 0xffff0000ll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(per_row) : i / per_row;  // (i may run past total, by less than four CTAs' worth)
 }
 
-// Rows off the grid: four single elements to a thread, a CTA's width apart and all on their way together (fp32 1531 x 1365 11.1 us
-// with one).
+// Rows off the grid: four single elements to a thread, a CTA's width apart and all on their way together (backward, bf16 4096 x 5501:
+// 64 us, 48 for 5504 columns).
 // The row of element span + offset of a matrix of N columns, when element `span` is in row m0 and column c0: past the row's
 // end a wide matrix has one more row to go, a narrow one takes a division of small numbers.
 __device__ __forceinline__ int64_t row_behind(int offset, int64_t m0, int64_t c0, int64_t N) {
@@ -64,32 +64,56 @@ __global__ void __launch_bounds__(kFfThreads) gate_forward(const float* p, float
   }
 }
 
+// Four elements of a row on the grid of four
+template <typename T> __device__ __forceinline__ void load_four_floats(const T* p, float* v) {
+  if constexpr (sizeof(T) == 4) {
+    widen<float>(ld_stream(p), v);
+  } else {
+    uint2 w;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "l"(p));
+    float out[8];
+    widen<T>(make_uint4(w.x, w.y, 0u, 0u), out);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = out[e];
+  }
+}
+template <typename T> __device__ __forceinline__ void store_four(T* p, const float* v) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<uint4*>(p) = narrow<float>(v);
+  } else {
+    const float w[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
+    const uint4 r = narrow<T>(w);
+    *reinterpret_cast<uint2*>(p) = make_uint2(r.x, r.y);
+  }
+}
 template <typename T, typename ACT, bool VECTOR>
 __global__ void __launch_bounds__(kFfThreads) gate_backward(const T* dh, const float* p, T* __restrict__ dp, int64_t M, int64_t N, int64_t pitch) {
-  constexpr int kVec = VECTOR ? 16 / static_cast<int>(sizeof(T)) : 4;
   auto slope = [](float& d, float& g, float& u) {
     float a, s;
     ACT::template both<sizeof(T) == 2>(g, a, s);
     g = d * u * s;
     u = d * a;
   };
-  float d[kVec], g[kVec], u[kVec];
   if constexpr (VECTOR) {
-    const int64_t per_row = N / kVec, total = M * per_row;
+    // Four elements to a thread whatever the type: 16 bytes of a projection, so that a warp's loads are whole lines (bf16 4096 x 11008: 133 us with
+    // eight, whose loads are every second 16 bytes, 96 so: the memory's own time).
+    const int64_t per_row = N / 4, total = M * per_row;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFfThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kFfThreads) {
-      const int64_t m = row_of(i, per_row, total), at = i * kVec + m * N, to = i * kVec + m * (pitch - N);
-      widen<T>(ld_stream(dh + i * kVec), d);
-      load_f32<kVec>(p + at, g);
-      load_f32<kVec>(p + at + N, u);
+      const int64_t m = row_of(i, per_row, total), at = i * 4 + m * N, to = i * 4 + m * (pitch - N);
+      float d[4], g[4], u[4];
+      load_four_floats<T>(dh + i * 4, d);
+      load_f32<4>(p + at, g);
+      load_f32<4>(p + at + N, u);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) slope(d[e], g[e], u[e]);
-      *reinterpret_cast<uint4*>(dp + to) = narrow<T>(g);  // (both products read it next: not streamed past L2)
-      *reinterpret_cast<uint4*>(dp + to + N) = narrow<T>(u);
+      for (int e = 0; e < 4; ++e) slope(d[e], g[e], u[e]);
+      store_four<T>(dp + to, g);  // (both products read it next: not streamed past L2)
+      store_four<T>(dp + to + N, u);
     }
   } else {
     const int64_t total = M * N;
     for (int64_t span = static_cast<int64_t>(blockIdx.x) * (4 * kFfThreads); span < total; span += static_cast<int64_t>(gridDim.x) * (4 * kFfThreads)) {
       const int64_t m0 = row_of(span, N, total), c0 = span - m0 * N, i0 = span + threadIdx.x;
+      float d[4], g[4], u[4];
       int64_t to[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -111,7 +135,7 @@ __global__ void __launch_bounds__(kFfThreads) gate_backward(const T* dh, const f
 }
 
 inline int ff_grid(int64_t items) {
-  const int64_t b = (items + kFfThreads - 1) / kFfThreads, most = kNumSMs * 16LL;
+  const int64_t b = (items + kFfThreads - 1) / kFfThreads, most = kNumSMs * 64LL;
   return static_cast<int>(b < 1 ? 1 : b < most ? b : most);
 }
 
@@ -126,9 +150,8 @@ int launch_gate(const float* p, float* out, int64_t M, int64_t N, int act, cudaS
 }
 
 template <typename T> int launch_gate_backward(const void* dh, const float* p, void* out, int64_t M, int64_t N, int64_t pitch, int act, cudaStream_t st) {
-  constexpr int kVec = 16 / sizeof(T);
-  const bool vec = N % kVec == 0 && pitch % kVec == 0 && aligned16(p) && aligned16(out) && aligned16(dh);
-  const int grid = ff_grid(M * N / (vec ? kVec : 4));
+  const bool vec = N % 4 == 0 && pitch % 4 == 0 && aligned16(p) && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(dh)) & (4 * sizeof(T) - 1)) == 0;
+  const int grid = ff_grid(M * N / 4);
   gate_act_each(act, [&](auto a) {
     if (vec) gate_backward<T, decltype(a), true><<<grid, kFfThreads, 0, st>>>(static_cast<const T*>(dh), p, static_cast<T*>(out), M, N, pitch);
     else gate_backward<T, decltype(a), false><<<grid, kFfThreads, 0, st>>>(static_cast<const T*>(dh), p, static_cast<T*>(out), M, N, pitch);
