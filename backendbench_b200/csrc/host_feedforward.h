@@ -221,13 +221,16 @@ std::tuple<TensorOpt, TensorOpt> ff_gated_linear_backward(const Tensor& g, const
       ff_launched(launched("b200_gate_backward_rows", [&, st = stream()] { return api.b200_gate_backward_rows(ptr(g), static_cast<const float*>(ptr(p)), ptr(dp), pitch, r.M, F, act, dt(x), st); }));
       std::tuple<TensorOpt, TensorOpt> out;
       const int64_t ws0 = w.stride(0), ws1 = w.stride(1);
-      const int64_t need = dt(x) != B200_F32 ? api.b200_linear_grads_scratch_bytes(ptr(dp), ptr(x), ptr(w), r.M, 2 * F, r.K, pitch, r.s_m, r.s_k, ws0, ws1) : -1;
+      const bool fp32 = dt(x) == B200_F32;
+      const int64_t need = fp32 ? api.b200_linear_f32_grads_scratch_bytes(r.M, 2 * F, r.K) : api.b200_linear_grads_scratch_bytes(ptr(dp), ptr(x), ptr(w), r.M, 2 * F, r.K, pitch, r.s_m, r.s_k, ws0, ws1);
       if (need >= 0) {
         Tensor dx, dw;
         if (mask[0]) dx = new_tensor(x.sizes(), x.scalar_type(), x);
         if (mask[1]) dw = new_tensor({2 * F, r.K}, x.scalar_type(), x);
         const Tensor s = ff_scratch(x, need);
-        const int rc = api.b200_linear_grads(ptr(dp), ptr(x), ptr(w), ptr(dx), ptr(dw), r.M, 2 * F, r.K, pitch, r.s_m, ws0, dt(x), ptr(s), need, ff_status(x), stream());
+        auto f = [](const Tensor& t) { return static_cast<float*>(ptr(t)); };
+        const int rc = fp32 ? api.b200_linear_f32_grads(f(dp), f(x), f(w), f(dx), f(dw), r.M, 2 * F, r.K, pitch, 1, r.s_m, r.s_k, ws0, ws1, ptr(s), need, ff_status(x), stream())
+                            : api.b200_linear_grads(ptr(dp), ptr(x), ptr(w), ptr(dx), ptr(dw), r.M, 2 * F, r.K, pitch, r.s_m, ws0, dt(x), ptr(s), need, ff_status(x), stream());
         if (rc != B200_ELAUNCH) {  // (a refused cluster launch: one product after the other)
           ff_check(rc, "b200_linear_grads");
           if (mask[0]) std::get<0>(out) = dx;

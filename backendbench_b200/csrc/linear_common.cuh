@@ -33,6 +33,54 @@ __device__ __forceinline__ void lin_tile(int64_t t, int64_t mt, int64_t nt, int 
   nb = static_cast<int>(in_g / gm);
 }
 
+// Two products in one launch, dealt to pairs of CTAs. The tiles of the one with the longer contraction (`first`, 0 or 1) go round; the pairs that
+// have one less (all but the first `late`) take `head` tiles of the other each meanwhile, and the rest of its `tiles` goes round again, so that
+// pairs at work at one time have neighbouring tiles.
+struct TwoParts {
+  int pairs, first, rounds, late, head, tiles;
+};
+__device__ __forceinline__ bool two_parts_tile(const TwoParts& p, int pair, int n, int& part, int& tile) {  // the n-th of a pair
+  const int mine = p.rounds + (pair < p.late ? 1 : 0), early = p.late ? p.pairs - p.late : 0;
+  if (n < mine) {
+    part = p.first;
+    tile = n * p.pairs + pair;
+    return true;
+  }
+  part = 1 - p.first;
+  n -= mine;
+  if (early && pair >= p.late) {
+    if (n < p.head) {
+      tile = n * early + (pair - p.late);
+      return tile < p.tiles;
+    }
+    n -= p.head;
+  }
+  tile = p.head * early + n * p.pairs + pair;
+  return tile < p.tiles;
+}
+// us, by what a tile of each takes: the one with the longer tiles by itself; both dealt out evenly
+struct TwoTimes {
+  int64_t tiles[2];
+  double tile[2], longest, even;
+  int first;
+  TwoTimes(int64_t tiles0, int64_t tiles1, double tile0, double tile1) : tiles{tiles0, tiles1}, tile{tile0, tile1}, first(tile1 > tile0 ? 1 : 0) {
+    const int pairs = kNumSMs / 2;
+    longest = static_cast<double>((tiles[first] + pairs - 1) / pairs) * tile[first];
+    even = (static_cast<double>(tiles[0]) * tile[0] + static_cast<double>(tiles[1]) * tile[1]) / pairs;
+  }
+};
+inline TwoParts two_parts(int first, int64_t tiles0, int64_t tiles1, const double* tile) {
+  TwoParts p{};
+  const int64_t tiles[2] = {tiles0, tiles1};
+  p.pairs = kNumSMs / 2;
+  p.first = first;
+  p.rounds = static_cast<int>(tiles[first] / p.pairs);
+  p.late = static_cast<int>(tiles[first] % p.pairs);
+  p.head = p.late ? static_cast<int>(tile[first] / tile[1 - first] + 0.5) : 0;
+  p.tiles = static_cast<int>(tiles[1 - first]);
+  return p;
+}
+
 // 16 bytes of a cluster CTA's shared memory
 template <typename V> __device__ __forceinline__ V ld_cluster(uint32_t from) {
   uint4 v;

@@ -100,9 +100,11 @@ template <bool GATED> __device__ __forceinline__ void f32_out(const F32Params& p
   put(out + m * p.N + n, v);
 }
 
+constexpr int kTwo = 3;  // pairs, with two products to deal out (part 1: map_a1, map_b1, out1, p1)
 template <bool GATED, int SHARE>
-__global__ void __launch_bounds__(kLinThreads, 1) linear_f32(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, float* __restrict__ out, F32Params p, uint32_t* __restrict__ status) {
-  constexpr bool kPair = SHARE == kPaired;
+__device__ __forceinline__ void linear_f32_body(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap& map_a1, const CUtensorMap& map_b1, float* __restrict__ out, float* __restrict__ out1,
+                                                F32Params p, F32Params p1, const TwoParts& two, uint32_t* __restrict__ status) {
+  constexpr bool kPair = SHARE == kPaired || SHARE == kTwo;
   constexpr int kTileM = kPair ? 256 : 128, kW = GATED ? kF32Cols / 2 : kF32Cols;  // output columns of a tile
   constexpr uint32_t kBPlane = (kPair ? kF32Cols / 2 : kF32Cols) * kSlabBytes;      // of B in this CTA
   extern __shared__ unsigned char smem_raw[];
@@ -155,10 +157,33 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_f32(const __grid_consta
   after_grids_before();
   p.a_max = waited(p.a_max);
   p.b_max = waited(p.b_max);
+  p1.a_max = waited(p1.a_max);
+  p1.b_max = waited(p1.b_max);
 
   const int64_t mt = (p.M + kTileM - 1) / kTileM, nt = (p.N + kW - 1) / kW, tiles = mt * nt;
   const int64_t tile_first = kPair ? (blockIdx.x >> 1) : SHARE == kSplit ? blockIdx.x / p.splits : blockIdx.x, tile_step = kPair ? (gridDim.x >> 1) : SHARE == kSplit ? tiles : gridDim.x;
   const int all_slabs = static_cast<int>(p.kp / 64);
+  const int slabs1 = static_cast<int>(p1.kp / 64);
+  const int64_t mt1 = (p1.M + kTileM - 1) / kTileM, nt1 = (p1.N + kW - 1) / kW;
+  // this CTA's (pair's) n-th tile
+  auto next_tile = [&](int n, int& part, int64_t& t) {
+    if constexpr (SHARE == kTwo) {
+      int tile = 0;
+      const bool is = two_parts_tile(two, static_cast<int>(blockIdx.x >> 1), n, part, tile);
+      t = tile;
+      return is;
+    } else {
+      part = 0;
+      t = tile_first + n * tile_step;
+      return t < tiles;
+    }
+  };
+  auto block_of = [&](int part, int64_t t, int& mb, int& nb) {
+    if (SHARE == kTwo && part) lin_tile(t, mt1, nt1, p1.group_m, mb, nb);
+    else lin_tile(t, mt, nt, p.group_m, mb, nb);
+  };
+  int part = 0;
+  int64_t t = 0;
   const int slab0 = SHARE == kSplit ? static_cast<int>(static_cast<int64_t>(all_slabs) * rank / p.splits) : 0;
   const int slabs = SHARE == kSplit ? static_cast<int>(static_cast<int64_t>(all_slabs) * (rank + 1) / p.splits) - slab0 : all_slabs;
 
@@ -168,24 +193,27 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_f32(const __grid_consta
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int64_t t = tile_first; t < tiles && ok; t += tile_step) {
+      for (int n = 0; ok && next_tile(n, part, t); ++n) {
         int mb, nb;
-        lin_tile(t, mt, nt, p.group_m, mb, nb);
+        block_of(part, t, mb, nb);
+        const bool other = SHARE == kTwo && part;
+        const CUtensorMap *ma = other ? &map_a1 : &map_a, *mapb = other ? &map_b1 : &map_b;
+        const int plane = static_cast<int>(other ? p1.kp : p.kp), tile_slabs = other ? slabs1 : slabs;
         const int m0 = mb * kTileM + static_cast<int>(cta_rank) * 128;
         int n0 = nb * kW;
         const int n1 = n0 + static_cast<int>(p.N);  // gated: the up rows
         if (kPair && cta_rank == 1u) n0 = GATED ? n1 : n0 + kF32Cols / 2;
-        for (int kb = 0; kb < slabs; ++kb) {
+        for (int kb = 0; kb < tile_slabs; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, kLinWaitNs)) { ok = false; break; }
           const uint32_t a_dst = smem_base + stage * stage_bytes, b_dst = a_dst + 2 * a_plane;
           const uint32_t bar = kPair ? map_to_cta(full_bar(stage), 0u) : full_bar(stage);
           if (!kPair) mbar_expect_tx(full_bar(stage), stage_bytes);
           else if (cta_rank == 0u) mbar_expect_tx(full_bar(stage), 2 * stage_bytes);
           for (int q = 0; q < 2; ++q) {
-            const int k = (slab0 + kb) * 64 + q * static_cast<int>(p.kp);
+            const int k = (slab0 + kb) * 64 + q * plane;
             if (kPair) {
-              tma_load_3d_pair(a_dst + q * a_plane, &map_a, bar, k, m0, 0);
-              tma_load_3d_pair(b_dst + q * kBPlane, &map_b, bar, k, n0, 0);
+              tma_load_3d_pair(a_dst + q * a_plane, ma, bar, k, m0, 0);
+              tma_load_3d_pair(b_dst + q * kBPlane, mapb, bar, k, n0, 0);
             } else {
               tma_load_3d(a_dst + q * a_plane, &map_a, bar, k, m0, 0);
               tma_load_3d(b_dst + q * kBPlane, &map_b, bar, k, n0, 0);
@@ -215,8 +243,9 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_f32(const __grid_consta
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int64_t t = tile_first; t < tiles && ok; t += tile_step) {
-        for (int kb = 0; kb < slabs; ++kb) {
+      for (int n = 0; ok && next_tile(n, part, t); ++n) {
+        const int tile_slabs = SHARE == kTwo && part ? slabs1 : slabs;
+        for (int kb = 0; kb < tile_slabs; ++kb) {
           if (!warp_wait(tempty_bar(acc), acc_phase ^ 1u) || !warp_wait(full_bar(stage), phase)) { ok = false; break; }
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kF32Cols);
@@ -267,24 +296,29 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_f32(const __grid_consta
     const int q = warp & 3, half = (warp - 2) >> 2;
     const uint32_t col0 = static_cast<uint32_t>(GATED ? half * 32 : half * 64), col1 = static_cast<uint32_t>(GATED ? 64 + half * 32 : half * 64 + 32);
     unsigned char* mine = epi_stage + (warp - 2) * kLinEpiBytes;
-    const bool vec = p.N % 4 == 0 && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(p.side)) & 15u) == 0;
     const uint32_t tempty_target = kPair ? map_to_cta(tempty_bar(0), 0u) : 0u;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int64_t t = tile_first; t < tiles && ok; t += tile_step) {
+    for (int n = 0; ok && next_tile(n, part, t); ++n) {
       int mb, nb;
-      lin_tile(t, mt, nt, p.group_m, mb, nb);
+      block_of(part, t, mb, nb);
+      const bool other = SHARE == kTwo && part;
+      const int64_t M = other ? p1.M : p.M, N = other ? p1.N : p.N;
+      float* to = other ? out1 : out;
+      const uint32_t *a_max = other ? p1.a_max : p.a_max, *b_max = other ? p1.b_max : p.b_max;
+      const int tile_slabs = other ? slabs1 : slabs;
+      const bool vec = N % 4 == 0 && ((reinterpret_cast<uintptr_t>(to) | reinterpret_cast<uintptr_t>(p.side)) & 15u) == 0;
       const int64_t mr0 = static_cast<int64_t>(mb) * kTileM + static_cast<int64_t>(cta_rank) * 128 + q * 32, n0 = static_cast<int64_t>(nb) * kW;
-      const int nrows = p.M - mr0 < 32 ? static_cast<int>(p.M - mr0) : 32;
+      const int nrows = M - mr0 < 32 ? static_cast<int>(M - mr0) : 32;
       const int64_t na = n0 + (GATED ? half * 32 : half * 64), nbb = GATED ? na : na + 32;  // first output columns of the two chunks
-      const float2 row = halves_of(lane < nrows ? p.a_max[mr0 + lane] : 0u);
-      const float2 c0 = halves_of(na + lane < p.N ? p.b_max[na + lane] : 0u), c1 = halves_of(nbb + lane < p.N ? p.b_max[(GATED ? p.N : 0) + nbb + lane] : 0u);
+      const float2 row = halves_of(lane < nrows ? a_max[mr0 + lane] : 0u);
+      const float2 c0 = halves_of(na + lane < N ? b_max[na + lane] : 0u), c1 = halves_of(nbb + lane < N ? b_max[(GATED ? N : 0) + nbb + lane] : 0u);
       float sum[64];
 #pragma unroll
       for (int e = 0; e < 64; ++e) sum[e] = 0.f;
 #pragma unroll 1
-      for (int kb = 0; kb < slabs; ++kb) {
+      for (int kb = 0; kb < tile_slabs; ++kb) {
         int got = 0;
         if (lane == 0) got = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, kLinWaitNs) ? 1 : 0;
         got = __shfl_sync(0xffffffffu, got, 0);
@@ -331,13 +365,13 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_f32(const __grid_consta
         sum[e + 1] = scaled(sum[e + 1], row, make_float2(c.z, c.w));
       }
       if (nrows <= 0) continue;
-      const int wide0 = p.N - na < 32 ? static_cast<int>(p.N - na) : 32, wide1 = p.N - nbb < 32 ? static_cast<int>(p.N - nbb) : 32;
+      const int wide0 = N - na < 32 ? static_cast<int>(N - na) : 32, wide1 = N - nbb < 32 ? static_cast<int>(N - nbb) : 32;
       if constexpr (GATED) {
         if (wide0 <= 0) continue;
         if (p.side) {
-          float* side = p.side + mr0 * (2 * p.N) + na;
-          lin_store<float>(sum, mine, side, 2 * p.N, nrows, wide0, vec, lane);
-          lin_store<float>(sum + 32, mine, side + p.N, 2 * p.N, nrows, wide0, vec, lane);
+          float* side = p.side + mr0 * (2 * N) + na;
+          lin_store<float>(sum, mine, side, 2 * N, nrows, wide0, vec, lane);
+          lin_store<float>(sum + 32, mine, side + N, 2 * N, nrows, wide0, vec, lane);
         }
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
@@ -351,10 +385,10 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_f32(const __grid_consta
 #pragma unroll
           for (int i = 0; i < 8; ++i) sum[e + i] = g.v[i];
         }
-        lin_store<float>(sum, mine, out + mr0 * p.N + na, p.N, nrows, wide0, vec, lane);
+        lin_store<float>(sum, mine, to + mr0 * N + na, N, nrows, wide0, vec, lane);
       } else {
-        if (wide0 > 0) lin_store<float>(sum, mine, out + mr0 * p.N + na, p.N, nrows, wide0, vec, lane);
-        if (wide1 > 0) lin_store<float>(sum + 32, mine, out + mr0 * p.N + nbb, p.N, nrows, wide1, vec, lane);
+        if (wide0 > 0) lin_store<float>(sum, mine, to + mr0 * N + na, N, nrows, wide0, vec, lane);
+        if (wide1 > 0) lin_store<float>(sum + 32, mine, to + mr0 * N + nbb, N, nrows, wide1, vec, lane);
       }
     }
     if (!ok && lane == 0) {
@@ -406,6 +440,17 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_f32(const __grid_consta
     if (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kF32Accs * kF32Cols) : "memory");
     else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kF32Accs * kF32Cols) : "memory");
   }
+}
+
+template <bool GATED, int SHARE>
+__global__ void __launch_bounds__(kLinThreads, 1) linear_f32(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, float* __restrict__ out, F32Params p, uint32_t* __restrict__ status) {
+  linear_f32_body<GATED, SHARE>(map_a, map_b, map_a, map_b, out, out, p, p, TwoParts{}, status);
+}
+// Two products in one launch: C = A B and C1 = A1 B1
+__global__ void __launch_bounds__(kLinThreads, 1)
+linear_f32_two(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
+               float* __restrict__ out, float* __restrict__ out1, F32Params p, F32Params p1, TwoParts two, uint32_t* __restrict__ status) {
+  linear_f32_body<false, kTwo>(map_a, map_b, map_a1, map_b1, out, out1, p, p1, two, status);
 }
 
 // ------------------------------------------------------------------ planes
@@ -610,15 +655,16 @@ __global__ void __launch_bounds__(256) split_columns(F32Operand A, F32Operand B,
 int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 struct F32Plan {
   int share, splits;
+  double us;
 };
 // us: splitting and starting 9, a slab 0.62 in a pair and 0.88 on a CTA of its own. Pairs or ranges, both measured: 500 x 2000 x 700 31.8 in pairs, 28.7 in two
 // ranges; 1024 x 1024 x 1024 22.1 in pairs, 25.6 on single CTAs; 200 x 4096 x 300 43.7, 63.6, 19.0 in eight ranges.
 F32Plan plan_f32(int64_t M, int64_t N, int64_t kp, bool gated) {
   const int64_t w = gated ? kF32Cols / 2 : kF32Cols, nt = (N + w - 1) / w, slabs = kp / 64;
-  F32Plan best{kSingle, 1};
+  F32Plan best{kSingle, 1, 0.};
   double least = 1e30;
   auto offer = [&](int share, int splits, double t) {
-    if (t < least) { least = t; best = F32Plan{share, splits}; }
+    if (t < least) { least = t; best = F32Plan{share, splits, t}; }
   };
   if (M > 128) {
     const int64_t tiles = (M + 255) / 256 * nt, rounds = (tiles + kNumSMs / 2 - 1) / (kNumSMs / 2);
@@ -710,17 +756,12 @@ cudaError_t launch_once(const F32Operand* across, int64_t tiles0, int64_t tiles,
   return cudaSuccess;
 }
 
-template <bool GATED>
-int run_f32(const float* A, const float* B, float* out, int64_t M, int64_t N, int64_t K, int64_t sAm, int64_t sAk, int64_t sBn, int64_t sBk, int act, float* side, void* scratch, uint32_t* status, cudaStream_t st) {
-  if (!encode_fn()) return B200_EDRIVER;
-  const int64_t rows_b = GATED ? 2 * N : N, kp = up_to(K, 64);
-  unsigned char* at = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(scratch) + 255) & ~static_cast<uintptr_t>(255));
-  uint32_t* most = reinterpret_cast<uint32_t*>(at);
-  __half* planes = reinterpret_cast<__half*>(at + up_to((M + rows_b) * 4, 256));
-  const F32Operand a{A, planes, most, M, K, kp, sAm, sAk}, b{B, planes + M * 2 * kp, most + M, rows_b, K, kp, sBn, sBk};
+// The planes of both operands of a product, whose magnitudes lie side by side
+int make_planes(const F32Operand& a, const F32Operand& b, cudaStream_t st, int& launches) {
   // rows that lie along K, and those that lie across it
   F32Operand along[2], across[2];
-  int n_along = 0, n_across = 0, launches = 1;
+  int n_along = 0, n_across = 0;
+  const int64_t K = a.K, kp = a.kp;
   cudaError_t le = cudaSuccess;
   for (const F32Operand* o : {&a, &b}) {
     if (o->s_k == 1 || (o->s_r != 1 && o->rows > 1)) along[n_along++] = *o;
@@ -735,7 +776,7 @@ int run_f32(const float* A, const float* B, float* out, int64_t M, int64_t N, in
     if (once) ++launches;
   }
   if (n_across && !once) {
-    const cudaError_t e = cudaMemsetAsync(across[0].most, 0, static_cast<size_t>((n_across == 2 ? M + rows_b : across[0].rows) * 4), st);
+    const cudaError_t e = cudaMemsetAsync(across[0].most, 0, static_cast<size_t>((n_across == 2 ? a.rows + b.rows : across[0].rows) * 4), st);
     if (e != cudaSuccess) { set_last_cuda_error(e); return B200_ELAUNCH; }
     auto blocks = [&](int i, int64_t step, int64_t k) { return i < n_across ? (across[i].rows + 31) / 32 * ((k + step - 1) / step) : 0; };
     le = launch_after(largest_of_columns, blocks(0, kLookRows, K) + blocks(1, kLookRows, K), 256, 0, st, across[0], across[1], static_cast<unsigned>(blocks(0, kLookRows, K)));
@@ -756,6 +797,20 @@ int run_f32(const float* A, const float* B, float* out, int64_t M, int64_t N, in
     ++launches;
   }
   if (le != cudaSuccess) { set_last_cuda_error(le); return B200_ELAUNCH; }
+  return B200_OK;
+}
+
+template <bool GATED>
+int run_f32(const float* A, const float* B, float* out, int64_t M, int64_t N, int64_t K, int64_t sAm, int64_t sAk, int64_t sBn, int64_t sBk, int act, float* side, void* scratch, uint32_t* status, cudaStream_t st) {
+  if (!encode_fn()) return B200_EDRIVER;
+  const int64_t rows_b = GATED ? 2 * N : N, kp = up_to(K, 64);
+  unsigned char* at = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(scratch) + 255) & ~static_cast<uintptr_t>(255));
+  uint32_t* most = reinterpret_cast<uint32_t*>(at);
+  __half* planes = reinterpret_cast<__half*>(at + up_to((M + rows_b) * 4, 256));
+  const F32Operand a{A, planes, most, M, K, kp, sAm, sAk}, b{B, planes + M * 2 * kp, most + M, rows_b, K, kp, sBn, sBk};
+  int launches = 1;
+  const int planes_rc = make_planes(a, b, st, launches);
+  if (planes_rc) return planes_rc;
   F32Params p{};
   p.M = M;
   p.N = N;
@@ -786,7 +841,7 @@ int run_f32(const float* A, const float* B, float* out, int64_t M, int64_t N, in
   int rc = run(plan);
   if (rc == B200_ELAUNCH && plan.share != kSingle) {  // the cluster launch was refused: the same on single CTAs
     (void)cudaGetLastError();
-    rc = run(F32Plan{kSingle, 1});
+    rc = run(F32Plan{kSingle, 1, 0.});
   }
   if (rc) return rc;
   return check_launch(launches);
@@ -794,6 +849,88 @@ int run_f32(const float* A, const float* B, float* out, int64_t M, int64_t N, in
 
 int64_t f32_scratch(int64_t M, int64_t rows_b, int64_t K) { return 256 + up_to((M + rows_b) * 4, 256) + (M + rows_b) * up_to(K, 64) * 4; }
 bool f32_sizes(int64_t M, int64_t rows_b, int64_t K) { return M >= 1 && rows_b >= 1 && K >= 1 && M <= 0x7fffffff && rows_b <= 0x7fffffff && K <= (1ll << 29) && M + rows_b <= 0x7fffffff; }
+
+// Both gradients of y = x w^T, dx = g w and dw = g^T x: four sets of planes (g's rows for the one are its columns for the other), one launch for the
+// products (see TwoParts; fp32 1531 x 2730 x 1027: 54 tiles of 43 slabs and 99 of 24).
+bool grads_pay(int64_t M, int64_t J, int64_t K) {
+  if (!f32_sizes(M, K, J) || !f32_sizes(J, K, M) || M <= 128 || J <= 128) return false;
+  const int64_t kx = up_to(J, 64), kw = up_to(M, 64), nt = (K + kF32Cols - 1) / kF32Cols;
+  const TwoTimes t((M + 255) / 256 * nt, (J + 255) / 256 * nt, 1. + 0.62 * static_cast<double>(kx / 64), 1. + 0.62 * static_cast<double>(kw / 64));
+  if (t.tiles[0] > (1 << 29) || t.tiles[1] > (1 << 29)) return false;  // (they are counted in 32 bits)
+  const double shorter = t.tile[1 - t.first], together = 9. + (t.longest > t.even + 0.5 * shorter ? t.longest : t.even + 0.5 * shorter);
+  // (0.8: a slab takes longer where every pair is at work. 206 sizes that this lets through: 16 % faster on average, 4 % slower at most)
+  return together < 0.8 * (plan_f32(M, K, kx, false).us + plan_f32(J, K, kw, false).us);
+}
+int run_grads(const float* g, const float* x, const float* w, float* dx, float* dw, int64_t M, int64_t J, int64_t K, const int64_t* s, void* scratch, uint32_t* status, cudaStream_t st) {
+  if (!encode_fn()) return B200_EDRIVER;
+  unsigned char* at = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(scratch) + 255) & ~static_cast<uintptr_t>(255));
+  int launches = 1;
+  alignas(64) CUtensorMap maps[4];
+  F32Params p[2] = {};
+  for (int i = 0; i < 2; ++i) {
+    const int64_t rows = i ? J : M, contraction = i ? M : J, kp = up_to(contraction, 64);
+    p[i].M = rows;
+    p[i].N = K;
+    p[i].kp = kp;
+    p[i].a_rows = 128;
+    p[i].splits = 1;
+    const int64_t group = (32ll << 20) / (4 * kp) / 256 * 256;  // (see run_f32)
+    p[i].group_m = static_cast<int>((group < 2048 ? 2048 : group > 65536 ? 65536 : group) / 256);
+    p[i].stages = kLinRing / (2 * (128 + kF32Cols / 2) * kSlabBytes);
+    p[i].idesc = (1u << 4) | (static_cast<uint32_t>(kF32Cols >> 3) << 17) | (16u << 24);  // f16 operands, fp32 sums
+    if (!(i ? dw : dx)) continue;
+    uint32_t* most = reinterpret_cast<uint32_t*>(at);
+    __half* planes = reinterpret_cast<__half*>(at + up_to((rows + K) * 4, 256));
+    const F32Operand a{g, planes, most, rows, contraction, kp, i ? s[1] : s[0], i ? s[0] : s[1]};
+    const F32Operand b{i ? x : w, planes + rows * 2 * kp, most + rows, K, contraction, kp, i ? s[3] : s[5], i ? s[2] : s[4]};
+    const int rc = make_planes(a, b, st, launches);
+    if (rc) return rc;
+    if (!encode_planes(&maps[2 * i], a.to, rows, kp, 128) || !encode_planes(&maps[2 * i + 1], b.to, K, kp, kF32Cols / 2)) return B200_EDRIVER;
+    p[i].a_max = a.most;
+    p[i].b_max = b.most;
+    at += up_to(f32_scratch(rows, K, contraction) - 256, 256);
+  }
+  for (int i = 0; i < 2; ++i) {  // a gradient that nobody wants has no tiles
+    if (i ? dw : dx) continue;
+    maps[2 * i] = maps[2 - 2 * i];
+    maps[2 * i + 1] = maps[3 - 2 * i];
+    p[i].a_max = p[1 - i].a_max;
+    p[i].b_max = p[1 - i].b_max;
+  }
+  const int64_t nt = (K + kF32Cols - 1) / kF32Cols;
+  const double tile[2] = {1. + 0.62 * static_cast<double>(p[0].kp / 64), 1. + 0.62 * static_cast<double>(p[1].kp / 64)};
+  const TwoParts two = two_parts(tile[1] > tile[0] ? 1 : 0, dx ? (M + 255) / 256 * nt : 0, dw ? (J + 255) / 256 * nt : 0, tile);
+  static std::atomic<uint64_t> allowed{0};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (e == cudaSuccess && !(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(linear_f32_two, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kF32Smem));
+    if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) { set_last_cuda_error(e); return B200_ELAUNCH; }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * two.pairs), 1, 1);
+  cfg.blockDim = dim3(kLinThreads, 1, 1);
+  cfg.dynamicSmemBytes = kF32Smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // (see launch_after)
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  e = cudaLaunchKernelEx(&cfg, linear_f32_two, maps[0], maps[1], maps[2], maps[3], dx, dw, p[0], p[1], two, status);
+  if (e != cudaSuccess) {  // (a refused cluster launch: the caller has other products)
+    set_last_cuda_error(e);
+    (void)cudaGetLastError();
+    return B200_ELAUNCH;
+  }
+  return check_launch(launches);
+}
 
 }  // namespace
 
@@ -821,4 +958,18 @@ extern "C" int b200_gated_linear_f32(const float* x, const float* w, float* out,
   if (N < 1 || N > 0x3fffffff || !f32_sizes(M, 2 * N, K) || activation < 0 || activation >= B200_ACT_COUNT || !x || !w || !out) return B200_EINVAL;
   if (!scratch || scratch_bytes < f32_scratch(M, 2 * N, K)) return B200_ESCRATCH;
   return run_f32<true>(x, w, out, M, N, K, sxm, sxk, swn, swk, activation, projections, scratch, status, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int64_t b200_linear_f32_grads_scratch_bytes(int64_t M, int64_t J, int64_t K) {
+  if (M < 1 || J < 1 || K < 1 || b200_linear_f32_scratch_bytes(M, K, J) <= 0 || b200_linear_f32_scratch_bytes(J, K, M) <= 0 || !grads_pay(M, J, K)) return -1;
+  return f32_scratch(M, K, J) + 256 + f32_scratch(J, K, M);
+}
+
+extern "C" int b200_linear_f32_grads(const float* g, const float* x, const float* w, float* dx, float* dw, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sgj, int64_t sxm, int64_t sxk, int64_t swj,
+                                     int64_t swk, void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream) {
+  if (!g || !x || !w || (!dx && !dw)) return B200_EINVAL;
+  const int64_t need = b200_linear_f32_grads_scratch_bytes(M, J, K), s[6] = {sgm, sgj, sxm, sxk, swj, swk};
+  if (need < 0) return B200_EINVAL;
+  if (!scratch || scratch_bytes < need) return B200_ESCRATCH;
+  return run_grads(g, x, w, dx, dw, M, J, K, s, scratch, status, static_cast<cudaStream_t>(stream));
 }

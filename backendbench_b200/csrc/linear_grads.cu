@@ -27,32 +27,9 @@ constexpr size_t kGradSmem = static_cast<size_t>(kLinRing) + kLinEpiWarps * kLin
 struct GradParams {
   int64_t M, J, K;
   int nt;                       // tiles across
-  int pairs, first, rounds, late, head, tiles;  // (see grad_tile; part 0 is dx, 1 is dw)
+  TwoParts two;                 // 0 is dx, 1 is dw
   int group_m;
 };
-
-// The n-th tile of a pair. Those of the part with the longer contraction (`first`) go round; the pairs that have one less (all but the
-// first `late`) take `head` tiles of the other part each meanwhile, and the rest of its `tiles` goes round again, so that pairs at work at one
-// time have neighbouring tiles.
-__device__ __forceinline__ bool grad_tile(const GradParams& p, int pair, int n, int& part, int& tile) {
-  const int mine = p.rounds + (pair < p.late ? 1 : 0), early = p.late ? p.pairs - p.late : 0;
-  if (n < mine) {
-    part = p.first;
-    tile = n * p.pairs + pair;
-    return true;
-  }
-  part = 1 - p.first;
-  n -= mine;
-  if (early && pair >= p.late) {
-    if (n < p.head) {
-      tile = n * early + (pair - p.late);
-      return tile < p.tiles;
-    }
-    n -= p.head;
-  }
-  tile = p.head * early + n * p.pairs + pair;
-  return tile < p.tiles;
-}
 
 // Groups of row blocks, the row block fastest inside one
 __device__ __forceinline__ void grad_block(const GradParams& p, int part, int t, int& mb, int& nb) {
@@ -116,7 +93,7 @@ linear_grads(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ 
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int n = 0; ok && grad_tile(p, pair, n, part, tile); ++n) {
+      for (int n = 0; ok && two_parts_tile(p.two, pair, n, part, tile); ++n) {
         int mb, nb;
         grad_block(p, part, tile, mb, nb);
         const int slabs = part ? slabs_m : slabs_j;
@@ -160,7 +137,7 @@ linear_grads(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ 
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int n = 0; ok && grad_tile(p, pair, n, part, tile); ++n) {
+      for (int n = 0; ok && two_parts_tile(p.two, pair, n, part, tile); ++n) {
         if (!warp_wait(tempty_bar(acc), acc_phase ^ 1u)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * 256), idesc = part ? idesc0 | 1u << 15 : idesc0;
@@ -209,7 +186,7 @@ linear_grads(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ 
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int n = 0; ok && grad_tile(p, pair, n, part, tile); ++n) {
+    for (int n = 0; ok && two_parts_tile(p.two, pair, n, part, tile); ++n) {
       T* out = part ? dw : dx;
       int mb, nb;
       grad_block(p, part, tile, mb, nb);
@@ -301,22 +278,10 @@ bool encode_grad(CUtensorMap* map, const void* base, int64_t rows, int64_t cols,
 // x and w as the copy engine takes them; every tile of the other part's rows reads them once
 LinOperand grad_operand(const void* base, int64_t rows, int64_t others, int64_t K, int64_t s_r) { return LinOperand{base, rows, K, s_r, 1, 2, (others + 255) / 256}; }
 
-// us: a tile; the part with the longer contraction by itself; both parts dealt out evenly
-struct GradTimes {
-  double tile[2], longest, even;
-  int64_t tiles[2];
-  int first;
-  GradTimes(int64_t M, int64_t J, int64_t K) {
-    const int64_t nt = (K + 255) / 256;
-    tiles[0] = (M + 255) / 256 * nt;
-    tiles[1] = (J + 255) / 256 * nt;
-    tile[0] = 1.5 + static_cast<double>((J + 63) / 64) * 0.31;
-    tile[1] = 1.5 + static_cast<double>((M + 63) / 64) * 0.31;
-    first = M > J ? 1 : 0;
-    const int pairs = kNumSMs / 2;
-    longest = static_cast<double>((tiles[first] + pairs - 1) / pairs) * tile[first];
-    even = (static_cast<double>(tiles[0]) * tile[0] + static_cast<double>(tiles[1]) * tile[1]) / pairs;
-  }
+// us: a tile of 256 x 256, a start and its slabs
+struct GradTimes : TwoTimes {
+  GradTimes(int64_t M, int64_t J, int64_t K)
+      : TwoTimes((M + 255) / 256 * ((K + 255) / 256), (J + 255) / 256 * ((K + 255) / 256), 1.5 + static_cast<double>((J + 63) / 64) * 0.31, 1.5 + static_cast<double>((M + 63) / 64) * 0.31) {}
 };
 
 template <typename T>
@@ -332,7 +297,7 @@ int launch_grads(const CUtensorMap* maps, void* dx, void* dw, const GradParams& 
   }
   if (e != cudaSuccess) { set_last_cuda_error(e); return B200_ELAUNCH; }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(2 * p.pairs), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * p.two.pairs), 1, 1);
   cfg.blockDim = dim3(kLinThreads, 1, 1);
   cfg.dynamicSmemBytes = kGradSmem;
   cfg.stream = st;
@@ -361,13 +326,14 @@ int launch_grads(const CUtensorMap* maps, void* dx, void* dw, const GradParams& 
 using namespace b200;
 
 extern "C" int64_t b200_linear_grads_scratch_bytes(const void* g, const void* x, const void* w, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sxm, int64_t sxk, int64_t swj, int64_t swk) {
-  if (M <= 128 || J <= 128 || K <= 64 || M > 0x7ffffeffLL || J > 0x7ffffeffLL || K > 0x7ffffeffLL || !encode_fn()) return -1;
+  if (M < 1 || J <= 128 || K <= 64 || M > 0x7ffffeffLL || J > 0x7ffffeffLL || K > 0x7ffffeffLL || !encode_fn()) return -1;
   if (sxk != 1 || swk != 1 || !aligned16(g) || sgm < J || sgm % 8) return -1;
   const GradTimes t(M, J, K);
   if (t.tiles[0] > (1 << 29) || t.tiles[1] > (1 << 29)) return -1;  // (they are counted in 32 bits)
-  // 1,062 sizes (136 to 8192 rows, J 256 to 28672, K 136 to 8192): 19 % faster than one product after the other on average, slower by more than 3 % for 38 of those
-  // that this lets through (2.5 to 5 times slower for some that it does not: one tile of 28672 to a pair, where a product by itself shares it)
-  if (t.longest > 1.75 * t.even && t.longest >= 20.) return -1;
+  // One tile to a pair is a poor way through a long contraction (28672: 140 us, where a product by itself shares it and takes 25). 1,062 sizes of 136 to 8192
+  // rows that this lets through: 19 % faster than one product after the other on average, slower by more than 3 % for 38; up to 128 rows, which are half a
+  // tile, 27 to 39 % faster for J up to 1400, even at 2048.
+  if (M <= 128 ? t.longest >= 10. : t.longest > 1.75 * t.even && t.longest >= 20.) return -1;
   const int64_t need = grad_operand(x, M, J, K, sxm).packed_bytes() + grad_operand(w, J, M, K, swj).packed_bytes();
   return need ? need + 256 : 0;
 }
@@ -398,14 +364,8 @@ extern "C" int b200_linear_grads(const void* g, const void* x, const void* w, vo
   p.J = J;
   p.K = K;
   p.nt = static_cast<int>((K + 255) / 256);
-  p.pairs = kNumSMs / 2;
   p.group_m = 8;
   const GradTimes t(M, J, K);
-  const int64_t tiles[2] = {dx ? t.tiles[0] : 0, dw ? t.tiles[1] : 0};
-  p.first = t.first;
-  p.rounds = static_cast<int>(tiles[t.first] / p.pairs);
-  p.late = static_cast<int>(tiles[t.first] % p.pairs);
-  p.head = p.late ? static_cast<int>(t.tile[t.first] / t.tile[1 - t.first] + 0.5) : 0;
-  p.tiles = static_cast<int>(tiles[1 - t.first]);
+  p.two = two_parts(t.first, dx ? t.tiles[0] : 0, dw ? t.tiles[1] : 0, t.tile);
   return bf16 ? launch_grads<__nv_bfloat16>(maps, dx, dw, p, launches, status, st) : launch_grads<__half>(maps, dx, dw, p, launches, status, st);
 }

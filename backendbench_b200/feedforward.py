@@ -173,17 +173,21 @@ def gated_linear_backward(grad_output: torch.Tensor, input: torch.Tensor, weight
         g, p = ops._contig(grad_output), ops._contig(projections)
         check(lib().b200_gate_backward_rows(g.data_ptr(), p.data_ptr(), dp.data_ptr(), pitch, M, F, act, ops._dt(g.dtype), ops._stream_handle()), "b200_gate_backward_rows")
     x = _as_rows(input)
-    if dp.numel() and dp.dtype != torch.float32:
-        strides = (pitch, x.stride(0), x.stride(1), weight.stride(0), weight.stride(1))
-        need = int(lib().b200_linear_grads_scratch_bytes(dp.data_ptr(), x.data_ptr(), weight.data_ptr(), M, J, K, *strides))
+    if dp.numel():
+        fp32 = dp.dtype == torch.float32
+        xs, ws = (x.stride(0), x.stride(1)), (weight.stride(0), weight.stride(1))
+        operands = (dp.data_ptr(), x.data_ptr(), weight.data_ptr())
+        need = int(lib().b200_linear_f32_grads_scratch_bytes(M, J, K) if fp32 else lib().b200_linear_grads_scratch_bytes(*operands, M, J, K, pitch, *xs, *ws))
         if need >= 0:
             dx = ops._new(input.shape, input.dtype, input.device) if want_dx else None
             dw = ops._new((J, K), input.dtype, input.device) if want_dw else None
             scratch = ops._scratch(dp.device, need) if need else None
-            rc = lib().b200_linear_grads(
-                dp.data_ptr(), x.data_ptr(), weight.data_ptr(), dx.data_ptr() if want_dx else None, dw.data_ptr() if want_dw else None, M, J, K, pitch, strides[1], strides[3], ops._dt(dp.dtype),
-                scratch.data_ptr() if need else None, need, ops._status(dp.device).data_ptr(), ops._stream_handle(),
-            )
+            results = (dx.data_ptr() if want_dx else None, dw.data_ptr() if want_dw else None)
+            behind = (scratch.data_ptr() if need else None, need, ops._status(dp.device).data_ptr(), ops._stream_handle())
+            if fp32:
+                rc = lib().b200_linear_f32_grads(*operands, *results, M, J, K, pitch, 1, *xs, *ws, *behind)
+            else:
+                rc = lib().b200_linear_grads(*operands, *results, M, J, K, pitch, xs[0], ws[0], ops._dt(dp.dtype), *behind)
             if rc != ELAUNCH:  # (a refused cluster launch: one product after the other)
                 check(rc, "b200_linear_grads")
                 return dx, dw

@@ -379,12 +379,17 @@ int b200_gated_linear_f32(const float* x, const float* w, float* out, float* pro
 
 /* Both gradients of y = x w^T in one launch (bf16, f16): dx [M, K] = g w and dw [J, K] = g^T x, contiguous, of g [M, J] with rows on the
  * 16-byte grid, x [M, K] and w [J, K] with rows along K; dx or dw may be NULL, and the other is the same then. b200_linear_grads_scratch_bytes is -1 where one product after the other is the
- * better way (few tiles with a long contraction, or small matrices) or an operand lies otherwise. */
+ * better way (few tiles with a long contraction, or J up to 128 or K up to 64) or an operand lies otherwise. */
 int64_t b200_linear_grads_scratch_bytes(const void* g, const void* x, const void* w, int64_t M, int64_t J, int64_t K,
                                         int64_t sgm, int64_t sxm, int64_t sxk, int64_t swj, int64_t swk);
 int b200_linear_grads(const void* g, const void* x, const void* w, void* dx, void* dw, int64_t M, int64_t J,
                       int64_t K, int64_t sgm, int64_t sxm, int64_t swj, int dtype, void* scratch,
                       int64_t scratch_bytes, uint32_t* status, void* stream);
+/* The same in fp32, by planes like b200_linear_f32, operands of any strides */
+int64_t b200_linear_f32_grads_scratch_bytes(int64_t M, int64_t J, int64_t K);
+int b200_linear_f32_grads(const float* g, const float* x, const float* w, float* dx, float* dw, int64_t M,
+                          int64_t J, int64_t K, int64_t sgm, int64_t sgj, int64_t sxm, int64_t sxk, int64_t swj,
+                          int64_t swk, void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream);
 
 /* The gate by itself (fp32, whose products come in several launches), and its gradient, for contiguous fp32
  * projections [M, 2 N] = [g | u]: out = act(g) * u;  grad_projections = [grad * u * act'(g) | grad * act(g)], grad and

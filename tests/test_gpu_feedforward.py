@@ -818,3 +818,35 @@ def test_gradients_that_are_not_finite_stay_in_their_rows():
     rows, ups = [i for i in range(M) if i != 33], [i for i in range(2 * F) if i not in (20, F + 20)]
     assert gx[33].isnan().all() and bits_equal(gx[rows], cx[rows])
     assert gw[[20, F + 20]].isnan().all() and bits_equal(gw[ups], cw[ups])
+
+
+@pytest.mark.parametrize("size", [(200, 512, 300), (300, 700, 333), (777, 520, 1003), (1531, 1027, 1365), (2752, 640, 400), (513, 2048, 2752)], ids=str)
+def test_both_gradients_of_fp32_in_one_launch(size):
+    M, k, F = size
+    x, w = _pair(M, k, F, F32)
+    dh = _randn(M, F, dtype=F32, seed=3)
+    _, projections = K.gated_linear_train(x, w)
+    dx, tx, dw, tw = ref.gated_grads(dh, x, w, projections, "silu", F32)
+    gx, gw = K.gated_linear_backward(dh, x, w, projections)
+    ref.assert_within(gx, dx, tx, "dx")
+    ref.assert_within(gw, dw, tw, "dW")
+    assert (gx.double() - dx).norm() <= 1e-6 * dx.norm() and (gw.double() - dw).norm() <= 1e-6 * dw.norm()
+    one, other = K.gated_linear_backward(dh, x, w, projections, "silu", [True, False])[0], K.gated_linear_backward(dh, x, w, projections, "silu", [False, True])[1]
+    assert bits_equal(one, gx) and bits_equal(other, gw)
+    turned = K.gated_linear_backward(dh, x.t().contiguous().t(), w.t().contiguous().t(), projections)
+    assert bits_equal(turned[0], gx) and bits_equal(turned[1], gw)
+
+
+@pytest.mark.parametrize("size", [(1, 72, 68), (1, 1000, 500), (17, 520, 333), (64, 2048, 700), (128, 300, 512)], ids=str)
+def test_both_gradients_of_few_rows_in_one_launch(size):
+    M, k, F = size
+    x, w = _pair(M, k, F, BF)
+    dh = _randn(M, F, dtype=BF, seed=3)
+    _, projections = K.gated_linear_train(x, w)
+    dx, tx, dw, tw = ref.gated_grads(dh, x, w, projections, "silu", BF)
+    assert _takes(M, F, x, w)
+    gx, gw = K.gated_linear_backward(dh, x, w, projections)
+    ref.assert_within(gx, dx, tx, "dx")
+    ref.assert_within(gw, dw, tw, "dW")
+    one, other = K.gated_linear_backward(dh, x, w, projections, "silu", [True, False])[0], K.gated_linear_backward(dh, x, w, projections, "silu", [False, True])[1]
+    assert bits_equal(one, gx) and bits_equal(other, gw)
