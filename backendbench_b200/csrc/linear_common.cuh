@@ -1,5 +1,5 @@
-// What the kernels of linear_tc.cu and linear_f32.cu share: sizes, the order of tiles, stores of 32 x 32 values, shared memory of a
-// cluster.
+// What the kernels of linear_tc.cu, linear_f32.cu and linear_grads.cu share: sizes, the order of tiles, two products in one launch, stores of
+// 32 x 32 values, shared memory of a cluster, operands copied to lines.
 #pragma once
 
 #include <cuda.h>

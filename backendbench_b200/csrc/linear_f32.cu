@@ -15,7 +15,8 @@
 // kind each. Clusters share a tile's K where tiles are few. An operand whose K elements are not contiguous is turned on its way into the planes.
 //
 // 1531 x 1027 x 1365 gated: 43 us with the split (10), 2.9e-7 of the norm off 64 bits; three bf16 planes and a gate of its own took 74, 2.8e-6 off.
-// The training step of that size 236 -> 145 (of which planes 28: operands across K read once 18, twice 27). What bounds it: shared memory, which a product of 128 columns waits for (the
+// The training step of that size 236 -> 142 (operands across K read once, not twice: 9 less; both gradients' products in one launch: 10 less, 3 of them left when
+// inputs come from memory). What bounds it: shared memory, which a product of 128 columns waits for (the
 // tensor pipe is 43 % busy), and 256 columns would want 128 sums to a thread.
 #include <atomic>
 #include <utility>

@@ -10,6 +10,9 @@
 // A pair of CTAs to a tile of 256 x 256 (tcgen05.mma, cta_group::2, fp32 sums in tensor memory, one rounding), loads, products
 // and stores as in the other kernels here. No operand is turned: g lies along the contraction for dx and across it for dw, x and w lie across it,
 // and the descriptors say so.
+//
+// bf16 2048 x 8192 x 4096: 158 us, 1.74 PFLOP/s, the tensor pipe 85 % busy, which is what bounds it; 4096 x 22016 x 4096 in a loop 1073 (under the power cap),
+// one product after the other 1178; 512 x 2048 x 1024 15.3 and 24.5.
 #include <cuda.h>
 
 #include <atomic>
@@ -84,6 +87,7 @@ linear_grads(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ 
   tc_fence_after();
   const uint32_t tmem_base = *tmem_base_slot;
   after_grids_before();
+  T *const to_dx = waited(dx), *const to_dw = waited(dw);  // (the copy engine reads, and nothing is written before)
 
   const int slabs_j = static_cast<int>((p.J + 63) / 64), slabs_m = static_cast<int>((p.M + 63) / 64);
   int part, tile;
@@ -181,13 +185,13 @@ linear_grads(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ 
     // ------------------------------------------------------------ epilogue: 64 columns at a time, two warps to a lane quarter
     const int q = warp & 3, half = (warp - 2) >> 2;
     unsigned char* mine = epi_stage + (warp - 2) * kLinEpiBytes;
-    const bool vec = p.K % 8 == 0 && ((reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw)) & 15u) == 0;
+    const bool vec = p.K % 8 == 0 && ((reinterpret_cast<uintptr_t>(to_dx) | reinterpret_cast<uintptr_t>(to_dw)) & 15u) == 0;
     const uint32_t tempty_target = map_to_cta(tempty_bar(0), 0u);
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
     for (int n = 0; ok && two_parts_tile(p.two, pair, n, part, tile); ++n) {
-      T* out = part ? dw : dx;
+      T* out = part ? to_dw : to_dx;
       int mb, nb;
       grad_block(p, part, tile, mb, nb);
       const int64_t r0 = static_cast<int64_t>(mb) * 256 + static_cast<int64_t>(rank) * 128 + q * 32, n0 = static_cast<int64_t>(nb) * 256 + half * 128, rows = part ? p.J : p.M;
