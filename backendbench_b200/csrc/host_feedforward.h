@@ -155,6 +155,16 @@ Tensor ff_product(const Operand& a, const Operand& b, int64_t M, int64_t N, int6
   return taken(r);
 }
 
+// a @ b as feedforward._scaled_product forms it
+Tensor ff_scaled_product(const Operand& a, const Tensor& most, int64_t first, const Operand& b, int64_t M, int64_t N, int64_t K, at::IntArrayRef shape) {
+  Tensor out = new_tensor(shape, a.t.scalar_type(), a.t);
+  const int64_t need = api.b200_linear_scaled_scratch_bytes(ptr(a.t), ptr(b.t), M, N, K, a.row, a.col, b.row, b.col);
+  const Tensor s = ff_scratch(a.t, need);
+  ff_check(api.b200_linear_scaled(ptr(a.t), static_cast<const uint32_t*>(ptr(most)) + first, ptr(b.t), ptr(out), M, N, K, a.row, a.col, b.row, b.col, ptr(s), need, ff_status(a.t), stream()),
+           "b200_linear_scaled");
+  return out;
+}
+
 // The pitch of dP's rows: on lines of 128 bytes for the copy engine (fp32 ones are split into planes from anywhere)
 int64_t gradient_pitch(int64_t cols, const Tensor& like) { return dt(like) == B200_F32 || cols % 64 == 0 ? cols : cols > 64 ? (cols + 63) / 64 * 64 : (cols + 7) / 8 * 8; }
 
@@ -217,12 +227,20 @@ std::tuple<TensorOpt, TensorOpt> ff_gated_linear_backward(const Tensor& g, const
     if (r.M && F && r.K && w.scalar_type() == x.scalar_type() && g.scalar_type() == x.scalar_type() && p.scalar_type() == at::kFloat && g.is_contiguous() && p.is_contiguous() &&
         g.sizes() == at::IntArrayRef(with_last(x, F)) && p.sizes() == at::IntArrayRef(with_last(x, 2 * F))) {
       const int64_t pitch = gradient_pitch(2 * F, x);
-      Tensor dp = new_tensor({r.M, pitch}, x.scalar_type(), x);
-      ff_launched(launched("b200_gate_backward_rows", [&, st = stream()] { return api.b200_gate_backward_rows(ptr(g), static_cast<const float*>(ptr(p)), ptr(dp), pitch, r.M, F, act, dt(x), st); }));
+      const bool scaled = dt(x) == B200_F16;
+      Tensor dp = new_tensor({r.M, pitch}, x.scalar_type(), x), dp_columns = dp, most;
+      if (scaled) {
+        if (mask[0] && mask[1]) dp_columns = new_tensor({r.M, pitch}, x.scalar_type(), x);
+        most = new_tensor({r.M + 2 * F}, at::kInt, x);
+        ff_launched(launched("b200_gate_backward_scaled", [&, st = stream()] {
+          return api.b200_gate_backward_scaled(ptr(g), static_cast<const float*>(ptr(p)), mask[0] ? ptr(dp) : nullptr, mask[1] ? ptr(dp_columns) : nullptr, static_cast<uint32_t*>(ptr(most)), pitch, r.M, F,
+                                               act, st);
+        }));
+      } else ff_launched(launched("b200_gate_backward_rows", [&, st = stream()] { return api.b200_gate_backward_rows(ptr(g), static_cast<const float*>(ptr(p)), ptr(dp), pitch, r.M, F, act, dt(x), st); }));
       std::tuple<TensorOpt, TensorOpt> out;
       const int64_t ws0 = w.stride(0), ws1 = w.stride(1);
       const bool fp32 = dt(x) == B200_F32;
-      const int64_t need = fp32 ? api.b200_linear_f32_grads_scratch_bytes(r.M, 2 * F, r.K) : api.b200_linear_grads_scratch_bytes(ptr(dp), ptr(x), ptr(w), r.M, 2 * F, r.K, pitch, r.s_m, r.s_k, ws0, ws1);
+      const int64_t need = fp32 ? api.b200_linear_f32_grads_scratch_bytes(r.M, 2 * F, r.K) : (scaled ? api.b200_linear_grads_scaled_scratch_bytes : api.b200_linear_grads_scratch_bytes)(ptr(dp), ptr(x), ptr(w), r.M, 2 * F, r.K, pitch, r.s_m, r.s_k, ws0, ws1);
       if (need >= 0) {
         Tensor dx, dw;
         if (mask[0]) dx = new_tensor(x.sizes(), x.scalar_type(), x);
@@ -230,13 +248,18 @@ std::tuple<TensorOpt, TensorOpt> ff_gated_linear_backward(const Tensor& g, const
         const Tensor s = ff_scratch(x, need);
         auto f = [](const Tensor& t) { return static_cast<float*>(ptr(t)); };
         const int rc = fp32 ? api.b200_linear_f32_grads(f(dp), f(x), f(w), f(dx), f(dw), r.M, 2 * F, r.K, pitch, 1, r.s_m, r.s_k, ws0, ws1, ptr(s), need, ff_status(x), stream())
-                            : api.b200_linear_grads(ptr(dp), ptr(x), ptr(w), ptr(dx), ptr(dw), r.M, 2 * F, r.K, pitch, r.s_m, ws0, dt(x), ptr(s), need, ff_status(x), stream());
+                            : api.b200_linear_grads(ptr(dp), ptr(dp_columns), static_cast<const uint32_t*>(ptr(most)), ptr(x), ptr(w), ptr(dx), ptr(dw), r.M, 2 * F, r.K, pitch, r.s_m, ws0, dt(x), ptr(s), need, ff_status(x), stream());
         if (rc != B200_ELAUNCH) {  // (a refused cluster launch: one product after the other)
           ff_check(rc, "b200_linear_grads");
           if (mask[0]) std::get<0>(out) = dx;
           if (mask[1]) std::get<1>(out) = dw;
           return out;
         }
+      }
+      if (scaled) {
+        if (mask[0]) std::get<0>(out) = ff_scaled_product(Operand{dp, 0, pitch, 1}, most, 0, Operand{w, 0, ws0, ws1}, r.M, r.K, 2 * F, x.sizes());
+        if (mask[1]) std::get<1>(out) = ff_scaled_product(Operand{dp_columns, 0, 1, pitch}, most, r.M, Operand{x, 0, r.s_m, r.s_k}, 2 * F, r.K, r.M, w.sizes());
+        return out;
       }
       if (mask[0]) std::get<0>(out) = ff_product(Operand{dp, 0, pitch, 1}, Operand{w, 0, w.stride(0), w.stride(1)}, r.M, r.K, 2 * F, x.sizes());
       if (mask[1]) std::get<1>(out) = ff_product(Operand{dp, 0, 1, pitch}, Operand{x, 0, r.s_m, r.s_k}, 2 * F, r.K, r.M, w.sizes());

@@ -81,6 +81,17 @@ inline TwoParts two_parts(int first, int64_t tiles0, int64_t tiles1, const doubl
   return p;
 }
 
+// Rows scaled by a power of two for f16, so that their largest magnitude (as fp32 bits) lies in [2^14, 2^15): its exponent, 2^-exponent being the scale
+__device__ __forceinline__ int scale_exponent(uint32_t bits) {
+  const int e = static_cast<int>(bits >> 23);
+  return bits == 0u ? 0 : (e == 255 ? 254 : e) - 141;
+}
+// 2^exponent, and 2^-exponent, in one float each: exponents below -100 count as that, which takes rows whose largest is below 2^-86 (times f16
+// operands they make no f16 result but zero)
+__device__ __forceinline__ int bounded_exponent(uint32_t bits) { return max(scale_exponent(bits), -100); }
+__device__ __forceinline__ float row_factor(uint32_t bits) { return __int_as_float((127 + bounded_exponent(bits)) << 23); }
+__device__ __forceinline__ float row_scale(uint32_t bits) { return __int_as_float((127 - bounded_exponent(bits)) << 23); }
+
 // 16 bytes of a cluster CTA's shared memory
 template <typename V> __device__ __forceinline__ V ld_cluster(uint32_t from) {
   uint4 v;

@@ -45,10 +45,6 @@ struct F32Params {
   const uint32_t *a_max, *b_max;  // largest magnitude of every row, as fp32 bits
 };
 
-__device__ __forceinline__ int scale_exponent(uint32_t bits) {
-  const int e = static_cast<int>(bits >> 23);
-  return bits == 0u ? 0 : (e == 255 ? 254 : e) - 141;  // 2^-exponent brings the largest magnitude to [2^14, 2^15)
-}
 // 2^exponent of a row or column as two factors, its halves (one cannot hold all of them); of row and column the halves are multiplied
 // with each other first: powers of two, so that a sum is rounded once at most, where the result itself is subnormal
 __device__ __forceinline__ float2 halves_of(uint32_t bits) {

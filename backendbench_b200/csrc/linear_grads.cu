@@ -11,6 +11,9 @@
 // and stores as in the other kernels here. No operand is turned: g lies along the contraction for dx and across it for dw, x and w lie across it,
 // and the descriptors say so.
 //
+// f16 holds 2^-24 to 65504, which a gradient of the projections need not keep to although dx and dw do: there g comes twice, its rows scaled by powers
+// of two for dx and its columns for dw, and the sums take the factors back before they are rounded.
+//
 // bf16 2048 x 8192 x 4096: 158 us, 1.74 PFLOP/s, the tensor pipe 85 % busy, which is what bounds it; 4096 x 22016 x 4096 in a loop 1073 (under the power cap),
 // one product after the other 1178; 512 x 2048 x 1024 15.3 and 24.5.
 #include <cuda.h>
@@ -31,6 +34,7 @@ struct GradParams {
   int64_t M, J, K;
   int nt;                       // tiles across
   TwoParts two;                 // 0 is dx, 1 is dw
+  const uint32_t* most[2];      // f16: largest magnitudes of g's rows and columns before they were scaled, as fp32 bits
   int group_m;
 };
 
@@ -87,6 +91,8 @@ linear_grads(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ 
   tc_fence_after();
   const uint32_t tmem_base = *tmem_base_slot;
   after_grids_before();
+  constexpr bool kScaledRows = std::is_same<T, __half>::value;
+  const uint32_t *const most_dx = waited(p.most[0]), *const most_dw = waited(p.most[1]);
   T *const to_dx = waited(dx), *const to_dw = waited(dw);  // (the copy engine reads, and nothing is written before)
 
   const int slabs_j = static_cast<int>((p.J + 63) / 64), slabs_m = static_cast<int>((p.M + 63) / 64);
@@ -197,6 +203,7 @@ linear_grads(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ 
       const int64_t r0 = static_cast<int64_t>(mb) * 256 + static_cast<int64_t>(rank) * 128 + q * 32, n0 = static_cast<int64_t>(nb) * 256 + half * 128, rows = part ? p.J : p.M;
       const int left = p.K - n0 < 128 ? static_cast<int>(p.K - n0) : 128, nrows = rows - r0 < 32 ? static_cast<int>(rows - r0) : 32;  // (0 or less: none)
       const int count = (left + 63) / 64;
+      const float factor = kScaledRows && lane < nrows ? row_factor((part ? most_dw : most_dx)[r0 + lane]) : 0.f;
       int got = 0;
       if (lane == 0) got = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, kLinWaitNs) ? 1 : 0;
       got = __shfl_sync(0xffffffffu, got, 0);
@@ -225,8 +232,12 @@ linear_grads(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ 
 #pragma unroll 1
       for (int i = 0; i < count; ++i, to += 64) {
         const int ncols = left - i * 64 < 64 ? left - i * 64 : 64;
-        const float* v = reinterpret_cast<const float*>(r);
+        float* v = reinterpret_cast<float*>(r);
         tc_ld_wait();
+        if constexpr (kScaledRows) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) v[e] *= factor;
+        }
         if (vec) {
           __syncwarp();  // what was staged has been read out
 #pragma unroll
@@ -329,7 +340,8 @@ int launch_grads(const CUtensorMap* maps, void* dx, void* dw, const GradParams& 
 
 using namespace b200;
 
-extern "C" int64_t b200_linear_grads_scratch_bytes(const void* g, const void* x, const void* w, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sxm, int64_t sxk, int64_t swj, int64_t swk) {
+namespace {
+int64_t grads_need(const void* g, const void* x, const void* w, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sxm, int64_t sxk, int64_t swj, int64_t swk, bool f16) {
   if (M < 1 || J <= 128 || K <= 64 || M > 0x7ffffeffLL || J > 0x7ffffeffLL || K > 0x7ffffeffLL || !encode_fn()) return -1;
   if (sxk != 1 || swk != 1 || !aligned16(g) || sgm < J || sgm % 8) return -1;
   const GradTimes t(M, J, K);
@@ -337,16 +349,32 @@ extern "C" int64_t b200_linear_grads_scratch_bytes(const void* g, const void* x,
   // One tile to a pair is a poor way through a long contraction (28672: 140 us, where a product by itself shares it and takes 25). 1,062 sizes of 136 to 8192
   // rows that this lets through: 19 % faster than one product after the other on average, slower by more than 3 % for 38; up to 128 rows, which are half a
   // tile, 27 to 39 % faster for J up to 1400, even at 2048.
-  if (M <= 128 ? t.longest >= 10. : t.longest > 1.75 * t.even && t.longest >= 20.) return -1;
+  // f16 has other products to weigh against (b200_linear_scaled), which turn dP, x and w first, 2.6e-6 us an element: 17 x 22016 x 4096 363 us with
+  // them, 135 here; 1024 x 4096 x 1024 95 and 53.
+  const double turned = 2.6e-6 * (static_cast<double>(J) * static_cast<double>(K) + static_cast<double>(M) * static_cast<double>(J + K));
+  const double most = f16 ? 20. + turned : M <= 128 ? 10. : 20.;
+  if (t.longest >= most && ((M <= 128 && !f16) || t.longest > 1.75 * t.even)) return -1;
   const int64_t need = grad_operand(x, M, J, K, sxm).packed_bytes() + grad_operand(w, J, M, K, swj).packed_bytes();
   return need ? need + 256 : 0;
 }
+}  // namespace
 
-extern "C" int b200_linear_grads(const void* g, const void* x, const void* w, void* dx, void* dw, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sxm, int64_t swj, int dtype, void* scratch,
-                                 int64_t scratch_bytes, uint32_t* status, void* stream) {
+extern "C" int64_t b200_linear_grads_scratch_bytes(const void* g, const void* x, const void* w, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sxm, int64_t sxk, int64_t swj, int64_t swk) {
+  return grads_need(g, x, w, M, J, K, sgm, sxm, sxk, swj, swk, false);
+}
+extern "C" int64_t b200_linear_grads_scaled_scratch_bytes(const void* g, const void* x, const void* w, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sxm, int64_t sxk, int64_t swj, int64_t swk) {
+  return grads_need(g, x, w, M, J, K, sgm, sxm, sxk, swj, swk, true);
+}
+
+extern "C" int b200_linear_grads(const void* g, const void* g_columns, const uint32_t* most, const void* x, const void* w, void* dx, void* dw, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sxm,
+                                 int64_t swj, int dtype, void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream) {
   if (dtype != B200_BF16 && dtype != B200_F16) return B200_EDTYPE;
-  if (!g || !x || !w || (!dx && !dw)) return B200_EINVAL;
-  const int64_t need = b200_linear_grads_scratch_bytes(g, x, w, M, J, K, sgm, sxm, 1, swj, 1);
+  if (dtype == B200_BF16) g_columns = g;
+  else if (!most) return B200_EINVAL;
+  if (!dx) g = g_columns;  // (the one that nobody wants need not be there)
+  if (!dw) g_columns = g;
+  if (!g || !g_columns || !aligned16(g_columns) || !x || !w || (!dx && !dw)) return B200_EINVAL;
+  const int64_t need = grads_need(g, x, w, M, J, K, sgm, sxm, 1, swj, 1, dtype == B200_F16);
   if (need < 0) return B200_EINVAL;
   if (need && (!scratch || scratch_bytes < need)) return B200_ESCRATCH;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -359,7 +387,7 @@ extern "C" int b200_linear_grads(const void* g, const void* x, const void* w, vo
   lin_pack(ox, ow, reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(scratch) + 255) & ~static_cast<uintptr_t>(255)), st, launches);
   const bool bf16 = dtype == B200_BF16;
   alignas(64) CUtensorMap maps[4];
-  if (!encode_grad(&maps[0], g, M, J, sgm, bf16, 128) || !encode_grad(&maps[2], g, M, J, sgm, bf16, 64)) return B200_EDRIVER;
+  if (!encode_grad(&maps[0], g, M, J, sgm, bf16, 128) || !encode_grad(&maps[2], g_columns, M, J, sgm, bf16, 64)) return B200_EDRIVER;
   maps[1] = maps[3] = maps[2];
   if ((dx && !encode_grad(&maps[1], ow.base, J, K, ow.s_r, bf16, 64)) || (dw && !encode_grad(&maps[3], ox.base, M, K, ox.s_r, bf16, 64)))
     return B200_EDRIVER;
@@ -369,6 +397,8 @@ extern "C" int b200_linear_grads(const void* g, const void* x, const void* w, vo
   p.K = K;
   p.nt = static_cast<int>((K + 255) / 256);
   p.group_m = 8;
+  p.most[0] = most;
+  p.most[1] = most ? most + M : nullptr;
   const GradTimes t(M, J, K);
   p.two = two_parts(t.first, dx ? t.tiles[0] : 0, dw ? t.tiles[1] : 0, t.tile);
   return bf16 ? launch_grads<__nv_bfloat16>(maps, dx, dw, p, launches, status, st) : launch_grads<__half>(maps, dx, dw, p, launches, status, st);

@@ -2,8 +2,9 @@
 //
 //   gated   h[m, n] = act(g[m, n]) * u[m, n],  g = x Wg^T, u = x Wu^T   (bf16 / f16, W = [Wg; Wu], 2 N x K)
 //   int8    y[m, n] = (sum_k a[m, k] b[n, k]) * sa[m] * sb[n] + bias[n]   (int8 operands, exact 32-bit sums)
+//   scaled  y[m, n] = (sum_k a[m, k] b[n, k]) * 2^e[m]                    (f16, rows of a scaled by powers of two: see row_factor)
 //
-// Both read operands whose rows lie along K, in slabs of 128 bytes, and both need the whole accumulator of a tile
+// All read operands whose rows lie along K, in slabs of 128 bytes, and all need the whole accumulator of a tile
 // before anything is written, so they share one kernel: a TMA producer warp, a warp that issues tcgen05.mma
 // (kind::f16 or kind::i8, four steps of 32 bytes of K to a slab), two accumulators of 256 columns in tensor memory and eight
 // epilogue warps that empty one while the other fills.
@@ -37,7 +38,7 @@ constexpr int kLinAccs = 2;  // at most
 constexpr int kLinHalfRing = 108 * 1024;                // two CTAs to an SM: 110 KB each (and never three, which would be more tensor memory than there is)
 constexpr size_t lin_smem(int ring) { return static_cast<size_t>(ring) + (ring == kLinRing ? kLinEpiWarps * kLinEpiBytes : 0) + 1024 /*align*/ + 512 /*barriers*/; }
 
-enum : int { kGated = 0, kInt8 = 1 };
+enum : int { kGated = 0, kInt8 = 1, kScaled = 2 };
 
 struct LinParams {
   int64_t M, N, K;        // outputs M x N; K in elements
@@ -56,6 +57,7 @@ struct LinParams {
   const float* a_scale;   // int8
   const float* b_scale;
   const void* bias;       // int8: [N] of the output type, or NULL
+  const uint32_t* a_most; // scaled: largest magnitude of every row of a before it was scaled, as fp32 bits
 };
 
 __device__ __forceinline__ void lin_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, bool i8) {
@@ -80,7 +82,7 @@ __device__ __forceinline__ void lin_mma_pair(uint32_t d, uint64_t a, uint64_t b,
 
 // Four outputs of a row, from sums (gated: of both projections), and where they go
 template <int MODE, typename TO>
-__device__ __forceinline__ void lin_out(const LinParams& p, TO* out, const float* a_scale, const float* b_scale, const TO* bias, int64_t m, int64_t n, const float* g, const float* u, bool vec) {
+__device__ __forceinline__ void lin_out(const LinParams& p, TO* out, const float* a_scale, const float* b_scale, const TO* bias, const uint32_t* a_most, int64_t m, int64_t n, const float* g, const float* u, bool vec) {
   float v[4];
   const int left = p.N - n < 4 ? static_cast<int>(p.N - n) : 4;
   if constexpr (MODE == kInt8) {
@@ -90,6 +92,10 @@ __device__ __forceinline__ void lin_out(const LinParams& p, TO* out, const float
       v[e] = e < left ? g[e] * sa * b_scale[n + e] : 0.f;
       if (bias && e < left) v[e] += to_f32(bias[n + e]);
     }
+  } else if constexpr (MODE == kScaled) {
+    const float factor = row_factor(a_most[m]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = g[e] * factor;
   } else {
     gate_act_each(p.act, [&](auto act) {
 #pragma unroll
@@ -128,7 +134,7 @@ __device__ __forceinline__ void lin_out(const LinParams& p, TO* out, const float
 
 template <int MODE, typename TO, int SHARE>
 __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, TO* __restrict__ out, LinParams p, uint32_t* __restrict__ status) {
-  constexpr bool kI8 = MODE == kInt8, kPair = SHARE == kPaired;
+  constexpr bool kI8 = MODE == kInt8, kTwice = MODE == kGated /* two accumulators' columns to an output */, kPair = SHARE == kPaired;
   constexpr int kTileM = kPair ? 256 : 128;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -191,13 +197,14 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
       lin_tile(t, mt, nt, p.group_m, mb, nb);
       for (int s = 0; s < p.ahead && k0 + s < k1; ++s) {
         prefetch_l2_3d(&map_b, (k0 + s) * p.k_step, nb * p.w, 0);
-        if (!kI8) prefetch_l2_3d(&map_b, (k0 + s) * p.k_step, nb * p.w + static_cast<int>(p.N), 0);
+        if (kTwice) prefetch_l2_3d(&map_b, (k0 + s) * p.k_step, nb * p.w + static_cast<int>(p.N), 0);
       }
     }
   }
   after_grids_before();
   const float *a_scale = waited(p.a_scale), *b_scale = waited(p.b_scale);
   const TO* bias = waited(static_cast<const TO*>(p.bias));
+  const uint32_t* a_most = waited(p.a_most);
 
   const int64_t mt = (p.M + kTileM - 1) / kTileM, nt = (p.N + p.w - 1) / p.w, tiles = mt * nt;
   const int64_t tile_first = kPair ? (blockIdx.x >> 1) : SHARE == kSplit ? blockIdx.x / p.splits : blockIdx.x, tile_step = kPair ? (gridDim.x >> 1) : SHARE == kSplit ? tiles : gridDim.x;
@@ -217,7 +224,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
         const int m0 = mb * kTileM + static_cast<int>(cta_rank) * 128;
         // gated: the gate rows n0.., then the up rows N + n0..; a pair has a box of B to each CTA
         int n0 = nb * p.w, n1 = n0 + static_cast<int>(p.N);
-        if (kPair && cta_rank == 1u) n0 = kI8 ? n0 + p.b_rows : n1;
+        if (kPair && cta_rank == 1u) n0 = kTwice ? n1 : n0 + p.b_rows;
         for (int kb = 0; kb < slabs; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, kLinWaitNs)) { ok = false; break; }
           const uint32_t a_dst = smem_base + stage * stage_bytes, b_dst = a_dst + a_bytes;
@@ -230,7 +237,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
           } else {
             mbar_expect_tx(full_bar(stage), stage_bytes);
             tma_load_3d(b_dst, &map_b, full_bar(stage), k, n0, 0);
-            if (!kI8) tma_load_3d(b_dst + b_bytes, &map_b, full_bar(stage), k, n1, 0);
+            if (kTwice) tma_load_3d(b_dst + b_bytes, &map_b, full_bar(stage), k, n1, 0);
             tma_load_3d(a_dst, &map_a, full_bar(stage), k, m0, 0);
           }
           if (++stage == stages) { stage = 0; phase ^= 1u; }
@@ -310,7 +317,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
     // ------------------------------------------------------------ epilogue: 32 columns at a time, two warps to a lane quarter
     const int q = warp & 3, half = (warp - 2) >> 2;
     unsigned char* mine = epi_stage + (warp - 2) * kLinEpiBytes;
-    constexpr int kPer = 16 / static_cast<int>(sizeof(TO)), kRegs = kI8 ? 32 : 64;
+    constexpr int kPer = 16 / static_cast<int>(sizeof(TO)), kRegs = kTwice ? 64 : 32;
     const bool vec = p.N % kPer == 0 && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(p.side)) & 15u) == 0;
     const uint32_t tempty_target = kPair ? map_to_cta(tempty_bar(0), 0u) : 0u;
     int acc = 0;
@@ -331,7 +338,8 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
         }
       };
       ahead(n0 + half * 32, wide - half * 32);
-      const float sa = kI8 && lane < nrows ? a_scale[mr0 + lane] : 0.f;
+      float sa = 0.f;
+      if (!kTwice && lane < nrows) sa = kI8 ? a_scale[mr0 + lane] : row_factor(a_most[mr0 + lane]);
       int got = 0;
       if (lane == 0) got = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, kLinWaitNs) ? 1 : 0;
       got = __shfl_sync(0xffffffffu, got, 0);
@@ -340,7 +348,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
       const uint32_t t_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * p.acc_cols);
       if constexpr (SHARE == kSplit) {
         // this CTA's sums to its own shared memory (everything that was in the ring has been multiplied), a row to a lane
-        const int columns = p.w * (kI8 ? 1 : 2);
+        const int columns = p.w * (kTwice ? 2 : 1);
         if (q * 32 < p.a_rows) {
           for (int c = half * 32; c < columns; c += 64) {
             uint32_t r[32];
@@ -360,7 +368,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
       auto fetch = [&](int i) {
         const uint32_t col = static_cast<uint32_t>((half + 2 * i) * 32);
         tc_ld_32x32(t_base + col, r);
-        if constexpr (!kI8) tc_ld_32x32(t_base + static_cast<uint32_t>(p.w) + col, r + 32);
+        if constexpr (kTwice) tc_ld_32x32(t_base + static_cast<uint32_t>(p.w) + col, r + 32);
       };
       // the chunk's values are in `v`: the next chunk is on its way while they are rounded and stored, or, behind the last,
       // the accumulator goes back to the MMA warp
@@ -403,6 +411,10 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
             v[e + 2] = v[e + 2] * b.z + c.z;
             v[e + 3] = v[e + 3] * b.w + c.w;
           }
+        } else if constexpr (MODE == kScaled) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * sa;
+          next(i);
         } else {
           const float *g = reinterpret_cast<const float*>(r), *u = reinterpret_cast<const float*>(r + 32);
           if (p.side && nrows > 0) {
@@ -431,7 +443,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
     // Every CTA of the cluster puts together its share of the tile: four columns to a thread, the CTAs' sums added in the order of
     // their ranges of K.
     cluster_sync_all();
-    const int columns = p.w * (kI8 ? 1 : 2), quads = p.w / 4;
+    const int columns = p.w * (kTwice ? 2 : 1), quads = p.w / 4;
     const uint32_t pitch = static_cast<uint32_t>(columns) * 4 + 16;
     int mb, nb;
     lin_tile(tile_first, mt, nt, p.group_m, mb, nb);
@@ -449,9 +461,12 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
           const int4 v = ld_cluster<int4>(from);
           s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
         } else {
-          const float4 v = ld_cluster<float4>(from), w = ld_cluster<float4>(from + static_cast<uint32_t>(p.w) * 4);
+          const float4 v = ld_cluster<float4>(from);
           g[0] += v.x; g[1] += v.y; g[2] += v.z; g[3] += v.w;
-          u[0] += w.x; u[1] += w.y; u[2] += w.z; u[3] += w.w;
+          if constexpr (kTwice) {
+            const float4 w = ld_cluster<float4>(from + static_cast<uint32_t>(p.w) * 4);
+            u[0] += w.x; u[1] += w.y; u[2] += w.z; u[3] += w.w;
+          }
         }
       }
       if (n0 + c >= p.N) continue;
@@ -459,7 +474,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_tc(const __grid_constan
 #pragma unroll
         for (int e = 0; e < 4; ++e) g[e] = static_cast<float>(s[e]);
       }
-      lin_out<MODE, TO>(p, out, a_scale, b_scale, bias, mr0 + r, n0 + c, g, u, quad_vec);
+      lin_out<MODE, TO>(p, out, a_scale, b_scale, bias, a_most, mr0 + r, n0 + c, g, u, quad_vec);
     }
     cluster_sync_all();  // nobody leaves while another reads its sums
   }
@@ -753,8 +768,9 @@ int run_linear(LinOperands ops, void* out, int64_t M, int64_t N, int64_t K, int 
       if (plan.share == kSplit) return launch_linear<MODE, TO, kSplit>(plan.splits, tiles * plan.splits, st, map_a, map_b, o, p, status);
       return launch_linear<MODE, TO, kSingle>(1, resident, st, map_a, map_b, o, p, status);
     };
-    if (dtype_out == B200_BF16) return go(static_cast<__nv_bfloat16*>(out));
     if (dtype_out == B200_F16) return go(static_cast<__half*>(out));
+    if constexpr (MODE != kScaled)
+      if (dtype_out == B200_BF16) return go(static_cast<__nv_bfloat16*>(out));
     if constexpr (MODE == kInt8) return go(static_cast<float*>(out));
     return B200_EDTYPE;
   };
@@ -805,6 +821,22 @@ extern "C" int b200_gated_linear(const void* x, const void* w, void* out, float*
   p.act = activation;
   p.side = projections;
   return run_linear<kGated>(LinOperands(x, w, M, N, K, sxm, sxk, swn, swk, 2, 2), out, M, N, K, dtype, dtype == B200_BF16, p, scratch, scratch_bytes, status, st);
+}
+
+extern "C" int64_t b200_linear_scaled_scratch_bytes(const void* A, const void* B, int64_t M, int64_t N, int64_t K, int64_t sAm, int64_t sAk, int64_t sBk, int64_t sBn) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  const int64_t need = LinOperands(A, B, M, N, K, sAm, sAk, sBn, sBk, 1, 2).packed_bytes();
+  return need ? need + 256 : 0;
+}
+
+extern "C" int b200_linear_scaled(const void* A, const uint32_t* a_most, const void* B, void* out, int64_t M, int64_t N, int64_t K, int64_t sAm, int64_t sAk, int64_t sBk, int64_t sBn, void* scratch,
+                                  int64_t scratch_bytes, uint32_t* status, void* stream) {
+  if (M < 0 || N < 0 || K < 1) return B200_EINVAL;
+  if (M == 0 || N == 0) return B200_OK;
+  if (!A || !a_most || !B || !out || M > kMostExtent || N > kMostExtent || K > kMostExtent) return B200_EINVAL;
+  LinParams p{};
+  p.a_most = a_most;
+  return run_linear<kScaled>(LinOperands(A, B, M, N, K, sAm, sAk, sBn, sBk, 1, 2), out, M, N, K, B200_F16, false, p, scratch, scratch_bytes, status, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int64_t b200_mm_int8_scratch_bytes(const void* A, const void* B, int64_t M, int64_t N, int64_t K, int64_t sAm, int64_t sAk, int64_t sBk, int64_t sBn) {

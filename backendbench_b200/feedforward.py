@@ -92,6 +92,23 @@ def _product(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _scaled_product(a: torch.Tensor, most: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    """a @ b in f16, of an `a` whose rows were scaled by powers of two that bring `most` to [2^14, 2^15): the fp32 sums take the factors back."""
+    (M, K), N = a.shape, b.shape[1]
+    out = ops._new((M, N), a.dtype, a.device)
+    if out.numel():
+        strides = (a.stride(0), a.stride(1), b.stride(0), b.stride(1))
+        need = int(lib().b200_linear_scaled_scratch_bytes(a.data_ptr(), b.data_ptr(), M, N, K, *strides))
+        scratch = ops._scratch(a.device, need) if need else None
+        check(
+            lib().b200_linear_scaled(
+                a.data_ptr(), most.data_ptr(), b.data_ptr(), out.data_ptr(), M, N, K, *strides, scratch.data_ptr() if need else None, need, ops._status(a.device).data_ptr(), ops._stream_handle()
+            ),
+            "b200_linear_scaled",
+        )
+    return out
+
+
 def _gated(input: torch.Tensor, weight: torch.Tensor, activation: str, keep: bool, what: str):
     ops._require_cuda(input, weight)
     act = _activation(activation)
@@ -151,8 +168,8 @@ def gated_linear_train(input: torch.Tensor, weight: torch.Tensor, activation: st
 def gated_linear_backward(grad_output: torch.Tensor, input: torch.Tensor, weight: torch.Tensor, projections: torch.Tensor, activation: str = "silu", output_mask=(True, True)):
     """(grad_input, grad_weight) of gated_linear, None where `output_mask` is False. With P = [g | u] the
     projections: dP = [grad u act'(g) | grad act(g)] (rounded to the type of the operands: it is one of the two
-    products that follow), grad_input = dP @ weight, grad_weight = dP^T @ input, in one launch where one product after the other
-    would leave SMs idle."""
+    products that follow; f16, whose range it need not keep to, holds it twice, scaled by a power of two to each row and to each column), grad_input = dP @ weight,
+    grad_weight = dP^T @ input, in one launch where one product after the other would leave SMs idle."""
     ops._require_cuda(grad_output, input, weight, projections)
     act = _activation(activation)
     F, K = _pair_args(input, weight, "gated_linear_backward")
@@ -168,8 +185,22 @@ def gated_linear_backward(grad_output: torch.Tensor, input: torch.Tensor, weight
     J = 2 * F
     # rows on lines of 128 bytes for the copy engine (fp32 ones are split into planes from anywhere)
     pitch = J if input.dtype == torch.float32 or J % 64 == 0 else (J + 63) // 64 * 64 if J > 64 else (J + 7) // 8 * 8
-    dp = ops._new((M, pitch), input.dtype, input.device)[:, :J]
-    if dp.numel():
+    scaled = input.dtype == torch.float16 and M * J > 0
+    dp = ops._new((M, pitch), input.dtype, input.device)[:, :J] if want_dx or not scaled else None
+    dp_columns = most = None
+    if scaled:
+        # (the gradient that nobody wants has no dP)
+        g, p = ops._contig(grad_output), ops._contig(projections)
+        dp_columns = ops._new((M, pitch), input.dtype, input.device)[:, :J] if want_dw else dp
+        dp = dp if want_dx else dp_columns
+        most = ops._new((M + J,), torch.int32, input.device)
+        check(
+            lib().b200_gate_backward_scaled(
+                g.data_ptr(), p.data_ptr(), dp.data_ptr() if want_dx else None, dp_columns.data_ptr() if want_dw else None, most.data_ptr(), pitch, M, F, act, ops._stream_handle()
+            ),
+            "b200_gate_backward_scaled",
+        )
+    elif dp.numel():
         g, p = ops._contig(grad_output), ops._contig(projections)
         check(lib().b200_gate_backward_rows(g.data_ptr(), p.data_ptr(), dp.data_ptr(), pitch, M, F, act, ops._dt(g.dtype), ops._stream_handle()), "b200_gate_backward_rows")
     x = _as_rows(input)
@@ -177,7 +208,8 @@ def gated_linear_backward(grad_output: torch.Tensor, input: torch.Tensor, weight
         fp32 = dp.dtype == torch.float32
         xs, ws = (x.stride(0), x.stride(1)), (weight.stride(0), weight.stride(1))
         operands = (dp.data_ptr(), x.data_ptr(), weight.data_ptr())
-        need = int(lib().b200_linear_f32_grads_scratch_bytes(M, J, K) if fp32 else lib().b200_linear_grads_scratch_bytes(*operands, M, J, K, pitch, *xs, *ws))
+        scratch_bytes = lib().b200_linear_grads_scaled_scratch_bytes if scaled else lib().b200_linear_grads_scratch_bytes
+        need = int(lib().b200_linear_f32_grads_scratch_bytes(M, J, K) if fp32 else scratch_bytes(*operands, M, J, K, pitch, *xs, *ws))
         if need >= 0:
             dx = ops._new(input.shape, input.dtype, input.device) if want_dx else None
             dw = ops._new((J, K), input.dtype, input.device) if want_dw else None
@@ -187,10 +219,14 @@ def gated_linear_backward(grad_output: torch.Tensor, input: torch.Tensor, weight
             if fp32:
                 rc = lib().b200_linear_f32_grads(*operands, *results, M, J, K, pitch, 1, *xs, *ws, *behind)
             else:
-                rc = lib().b200_linear_grads(*operands, *results, M, J, K, pitch, xs[0], ws[0], ops._dt(dp.dtype), *behind)
+                columns = (dp_columns.data_ptr(), most.data_ptr()) if scaled else (None, None)
+                rc = lib().b200_linear_grads(operands[0], *columns, *operands[1:], *results, M, J, K, pitch, xs[0], ws[0], ops._dt(dp.dtype), *behind)
             if rc != ELAUNCH:  # (a refused cluster launch: one product after the other)
                 check(rc, "b200_linear_grads")
                 return dx, dw
+    if scaled:
+        dx = _scaled_product(dp, most, weight).view(input.shape) if want_dx else None
+        return dx, _scaled_product(dp_columns.t(), most[M:], x) if want_dw else None
     dx = _product(dp, weight).view(input.shape) if want_dx else None
     dw = _product(dp.t(), x) if want_dw else None
     return dx, dw

@@ -378,18 +378,30 @@ int b200_gated_linear_f32(const float* x, const float* w, float* out, float* pro
                           void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream);
 
 /* Both gradients of y = x w^T in one launch (bf16, f16): dx [M, K] = g w and dw [J, K] = g^T x, contiguous, of g [M, J] with rows on the
- * 16-byte grid, x [M, K] and w [J, K] with rows along K; dx or dw may be NULL, and the other is the same then. b200_linear_grads_scratch_bytes is -1 where one product after the other is the
+ * 16-byte grid, x [M, K] and w [J, K] with rows along K; dx or dw may be NULL, and the other is the same then. f16: g comes as
+ * b200_gate_backward_scaled leaves it, `g` by rows (for dx), `g_columns` by columns (for dw), `most` with their magnitudes; bf16
+ * takes `g` for both and looks at neither. b200_linear_grads_scratch_bytes (f16: _scaled_) is -1 where one product after the other is the
  * better way (few tiles with a long contraction, or J up to 128 or K up to 64) or an operand lies otherwise. */
 int64_t b200_linear_grads_scratch_bytes(const void* g, const void* x, const void* w, int64_t M, int64_t J, int64_t K,
                                         int64_t sgm, int64_t sxm, int64_t sxk, int64_t swj, int64_t swk);
-int b200_linear_grads(const void* g, const void* x, const void* w, void* dx, void* dw, int64_t M, int64_t J,
-                      int64_t K, int64_t sgm, int64_t sxm, int64_t swj, int dtype, void* scratch,
+int64_t b200_linear_grads_scaled_scratch_bytes(const void* g, const void* x, const void* w, int64_t M, int64_t J, int64_t K,
+                                               int64_t sgm, int64_t sxm, int64_t sxk, int64_t swj, int64_t swk);
+int b200_linear_grads(const void* g, const void* g_columns, const uint32_t* most, const void* x, const void* w,
+                      void* dx, void* dw, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sxm, int64_t swj, int dtype, void* scratch,
                       int64_t scratch_bytes, uint32_t* status, void* stream);
 /* The same in fp32, by planes like b200_linear_f32, operands of any strides */
 int64_t b200_linear_f32_grads_scratch_bytes(int64_t M, int64_t J, int64_t K);
 int b200_linear_f32_grads(const float* g, const float* x, const float* w, float* dx, float* dw, int64_t M,
                           int64_t J, int64_t K, int64_t sgm, int64_t sgj, int64_t sxm, int64_t sxk, int64_t swj,
                           int64_t swk, void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream);
+
+/* out[m, n] = 2^e[m] * sum_k A[m, k] B[k, n] for f16 operands of any strides (as by b200_gated_linear), out [M, N] contiguous f16: fp32 sums, the
+ * factor, one rounding. A's rows have been scaled by 2^-e[m], which brings a_most[m] (fp32 bits) to [2^14, 2^15). */
+int64_t b200_linear_scaled_scratch_bytes(const void* A, const void* B, int64_t M, int64_t N, int64_t K, int64_t sAm,
+                                         int64_t sAk, int64_t sBk, int64_t sBn);
+int b200_linear_scaled(const void* A, const uint32_t* a_most, const void* B, void* out, int64_t M, int64_t N,
+                       int64_t K, int64_t sAm, int64_t sAk, int64_t sBk, int64_t sBn, void* scratch,
+                       int64_t scratch_bytes, uint32_t* status, void* stream);
 
 /* The gate by itself (fp32, whose products come in several launches), and its gradient, for contiguous fp32
  * projections [M, 2 N] = [g | u]: out = act(g) * u;  grad_projections = [grad * u * act'(g) | grad * act(g)], grad and
@@ -399,6 +411,11 @@ int b200_gate_backward(const void* grad, const float* projections, void* grad_pr
                        int64_t N, int activation, int dtype, void* stream);
 int b200_gate_backward_rows(const void* grad, const float* projections, void* grad_projections,
                             int64_t row_stride, int64_t M, int64_t N, int activation, int dtype, void* stream);
+/* f16, whose range grad_projections need not keep to: twice, rows (for a product with a weight) and columns (for one with the input) scaled by powers of
+ * two that bring their largest magnitudes to [2^14, 2^15); these go to most[M + 2 N] as fp32 bits, rows first.
+ * by_rows or by_columns may be NULL. */
+int b200_gate_backward_scaled(const void* grad, const float* projections, void* by_rows, void* by_columns, uint32_t* most,
+                              int64_t row_stride, int64_t M, int64_t N, int activation, void* stream);
 
 /* out[i] = residual[i] + (word(i) >= round(p 2^32) ? x[i] / (1 - p) : 0) for n contiguous elements (residual
  * may be NULL). word(i) is word i % 4 of Philox-4x32 with ten rounds for the counter (state[1] + i / 4, subsequence)
