@@ -6,8 +6,12 @@
 //   relu       g for g > 0, else 0; NaN stays NaN
 //   sigmoid    s(g)                        s (1 - s)
 //
-// `fast` goes with 16-bit results (the exponential and the quotient are good to a few units in the last place of fp32, 2^-20 or
-// better against the 2^-8 or 2^-11 of the rounding that follows), `exact` with fp32 ones. The normal cdf is CUDA's
+// s(z) is 1 / (1 + t) for z >= 0 and t / (1 + t) below, t = e^-|z|: a denominator of 1 to 2. (1 + e^-z overflows below -88.7, and the fast quotient
+// gives 0 for denominators above 2^126, below -87.3, where s is 2^-127 and g s times a large u is not small.) Below -87.3 t is subnormal, and resolved to
+// 2^-149; below -103.9 it is 0.
+//
+// `fast` goes with 16-bit results: its exponential is off by 2 + 1.173 |z| units in the last place of fp32 (2^-19 at |z| = 10, 2^-16.4 at 80), its quotient by
+// two, against the 2^-8 or 2^-11 of the rounding that follows. `exact` goes with fp32 ones. The normal cdf is CUDA's
 // own function, which does not cancel on the negative side as 1 + erf does.
 #pragma once
 
@@ -15,13 +19,16 @@
 
 namespace b200 {
 
-template <bool FAST> __device__ __forceinline__ float gate_sigmoid(float z) {
-  return FAST ? __fdividef(1.f, 1.f + __expf(-z)) : 1.f / (1.f + expf(-z));
+// v s(z)
+template <bool FAST> __device__ __forceinline__ float gate_times_sigmoid(float v, float z) {
+  const float t = FAST ? __expf(-fabsf(z)) : expf(-fabsf(z)), w = z < 0.f ? v * t : v;
+  return FAST ? __fdividef(w, 1.f + t) : w / (1.f + t);
 }
+template <bool FAST> __device__ __forceinline__ float gate_sigmoid(float z) { return gate_times_sigmoid<FAST>(1.f, z); }
 __device__ __forceinline__ float gelu_tanh_arg(float g) { return 1.5957691216057308f * (g + 0.044715f * g * g * g); }  // 2 z
 
 struct ActSilu {
-  template <bool FAST> static __device__ __forceinline__ float f(float g) { return FAST ? __fdividef(g, 1.f + __expf(-g)) : g / (1.f + expf(-g)); }
+  template <bool FAST> static __device__ __forceinline__ float f(float g) { return gate_times_sigmoid<FAST>(g, g); }
   template <bool FAST> static __device__ __forceinline__ void both(float g, float& a, float& d) {
     const float s = gate_sigmoid<FAST>(g);
     a = g * s;
@@ -41,10 +48,7 @@ struct ActGelu {
   __device__ __forceinline__ float exact(float g) const { return f<false>(g); }
 };
 struct ActGeluTanh {
-  template <bool FAST> static __device__ __forceinline__ float f(float g) {
-    const float y = gelu_tanh_arg(g);
-    return FAST ? __fdividef(g, 1.f + __expf(-y)) : g / (1.f + expf(-y));
-  }
+  template <bool FAST> static __device__ __forceinline__ float f(float g) { return gate_times_sigmoid<FAST>(g, gelu_tanh_arg(g)); }
   template <bool FAST> static __device__ __forceinline__ void both(float g, float& a, float& d) {
     const float s = gate_sigmoid<FAST>(gelu_tanh_arg(g));
     a = g * s;

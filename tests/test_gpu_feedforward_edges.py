@@ -96,3 +96,36 @@ def test_f16_gradients_captured_and_replayed():
         for g, out in graphs:
             g.replay()
             assert all(bits_equal(a, b) for a, b in zip(out, want)), step
+
+
+# ------------------------------------------------------------------ where the exponential of a gate leaves fp32
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("name", ["silu", "gelu_tanh", "sigmoid"])
+def test_gates_whose_exponential_is_at_the_end_of_fp32(name, dtype):
+    """e^-y between 2^116 and 2^148: 1 + e^-y passes 2^126 (where a fast quotient ends) and 2^128, the activation is 2^-148 or more all
+    the same, and an up projection of 2^100 brings it back. Beside the relative errors, e^y is off by two steps of the subnormals at
+    most, 2^-148, where it is one."""
+    g = torch.arange(-10.625, -9.5, 1 / 16) if name == "gelu_tanh" else torch.arange(-102.0, -80.0, 0.5)
+    n = g.numel()
+    up = 2.0**100
+    for M, k in ((2, 64), (300, 64), (128, 1024)):
+        F = 256
+        g64 = g.double().to(DEV).repeat((F + n - 1) // n)[:F]
+        x = torch.zeros(M, k, device=DEV, dtype=dtype)
+        x[:, 0] = 1
+        w = torch.zeros(2 * F, k, device=DEV, dtype=dtype)
+        w[:F, 0], w[F:, 0] = g64.to(dtype), up
+        want = ref.act(g64, name) * up
+        tol = (ref.U[dtype] + ref.act_error(g64, name, dtype)) * want.abs() + 2.0**-148 * (1 + g64.abs()) * up
+        assert want.abs().min() > 2.0**-48
+        for h in (K.gated_linear(x, w, name), K.gated_linear_train(x, w, name)[0]):
+            ref.assert_within(h, want.expand(M, F), 1.001 * tol.expand(M, F), f"{M} rows")
+    # the slope, by a weight that hands dP on as it is: dx = [dh u act'(g) | dh act(g)]
+    g64 = g.double().to(DEV)
+    p = torch.stack([g64, torch.ones_like(g64)], 1).float()
+    dh = torch.full((n, 1), up, device=DEV, dtype=dtype)
+    dx, _ = K.gated_linear_backward(dh, torch.zeros(n, 2, device=DEV, dtype=dtype), torch.eye(2, device=DEV, dtype=dtype), p, name)
+    for got, value in ((dx[:, 0], ref.slope(g64, name)), (dx[:, 1], ref.act(g64, name))):
+        # a slope has another factor of up to 1 + 1.6 |g| (1 + 0.14 g^2), of a dozen roundings
+        tol = (ref.U[dtype] + ref.act_error(g64, name, dtype) + 16 * 2.0**-24) * value.abs() + 2.0**-148 * (1 + 1.6 * g64.abs() * (1 + 0.14 * g64.square()))
+        ref.assert_within(got, value * up, 1.001 * tol * up, "dP")
