@@ -2,7 +2,7 @@
 //
 // A row of an operand (its K elements) is scaled by a power of two so that its largest magnitude lies in [2^14, 2^15), and every
 // element is split into two f16 values, y = h + l: h the nearest one, l the nearest to what is left. That resolves an element to
-// 2^-22 of itself, or to 2^-40 of the row's largest, whichever is more (l is subnormal below 2^-14). Three f16 products, h h + h l + l h,
+// 2^-22 of itself, or to 2^-39 of the row's largest, whichever is more (l is subnormal below 2^-14, where half a step is 2^-25). Three f16 products, h h + h l + l h,
 // exact in the tensor cores' fp32 sums, are then the fp32 product; what l l would add is below 2^-22 of it. Half the products
 // that three bf16 planes take, and as those have no exponents to spare, the scales come back with the result.
 //

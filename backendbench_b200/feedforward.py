@@ -152,7 +152,7 @@ def _gated(input: torch.Tensor, weight: torch.Tensor, activation: str, keep: boo
 @_on_device_of
 def gated_linear(input: torch.Tensor, weight: torch.Tensor, activation: str = "silu") -> torch.Tensor:
     """act(input @ weight[:F].T) * (input @ weight[F:].T), [..., K] x [2 F, K] -> [..., F]. One kernel on fp32 sums, with one
-    rounding; large fp32 operands are split into two f16 planes before it (2^-22 of an element, 2^-40 of its row's largest
+    rounding; large fp32 operands are split into two f16 planes before it (2^-22 of an element, 2^-39 of its row's largest
     magnitude), small ones take the package's fp32 product and a gate behind it. `activation`: silu, gelu (erf), gelu_tanh, relu or sigmoid."""
     return _gated(input, weight, activation, False, "gated_linear")[0]
 

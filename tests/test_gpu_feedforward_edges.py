@@ -4,8 +4,9 @@ import pytest
 import torch
 
 import feedforward_ref as ref
+from backendbench_b200 import _abi, feedforward, ops
 from conftest import bits_equal
-from test_gpu_feedforward import BF, DEV, F16, F32, K, _on_lines, _pair, _randn, _takes, bands, without_bands  # noqa: F401  (bands: every output between sentinels)
+from test_gpu_feedforward import BF, DEV, F16, F32, K, _pair, _randn, bands, without_bands  # noqa: F401  (bands: every output between sentinels)
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +130,97 @@ def test_gates_whose_exponential_is_at_the_end_of_fp32(name, dtype):
         # a slope has another factor of up to 1 + 1.6 |g| (1 + 0.14 g^2), of a dozen roundings
         tol = (ref.U[dtype] + ref.act_error(g64, name, dtype) + 16 * 2.0**-24) * value.abs() + 2.0**-148 * (1 + 1.6 * g64.abs() * (1 + 0.14 * g64.square()))
         ref.assert_within(got, value * up, 1.001 * tol * up, "dP")
+
+
+# ------------------------------------------------------------------ fp32: sizes and rules
+def _check_f32(M, k, F, name="silu"):
+    """Both passes elementwise and by the norm (see test_large_products_in_32_bits_are_as_exact_as_their_sums)."""
+    x, w = _pair(M, k, F, F32)
+    h, th, p, tp = ref.gated(x, w, name, F32)
+    out, projections = K.gated_linear_train(x, w, name)
+    ref.assert_within(projections, p, tp, "projections")
+    ref.assert_within(out, h, th, "h")
+    assert (projections.double() - p).norm() <= 1e-6 * p.norm() and (out.double() - h).norm() <= 2e-6 * h.norm()
+    dh = _randn(M, F, dtype=F32, seed=3) * _spread(M, -8, 8)  # (columns of dP, which are rows of a product, hold all magnitudes)
+    dx, tx, dw, tw = ref.gated_grads(dh, x, w, projections, name, F32)
+    gx, gw = K.gated_linear_backward(dh, x, w, projections, name)
+    ref.assert_within(gx, dx, tx, "dx")
+    ref.assert_within(gw, dw, tw, "dw")
+    assert (gx.double() - dx).norm() <= 1e-6 * dx.norm() and (gw.double() - dw).norm() <= 1e-6 * dw.norm()
+
+
+def _joint(M, k, F):
+    return feedforward.lib().b200_linear_f32_grads_scratch_bytes(M, 2 * F, k) >= 0
+
+
+@pytest.mark.parametrize("size", [(70, 97, 7003), (13401, 73, 71), (261, 2190, 6844), (13850, 2199, 129)], ids=str)
+def test_fp32_operands_that_lie_across_long_contractions(size):
+    """Contractions of more than 13,312 (eight CTAs' shared memory) are read twice where they lie across: the weight for dx, dP and x for dw; by
+    products of their own and in the joint launch."""
+    M, k, F = size
+    assert max(M, 2 * F) > 8 * 26 * 64 and _joint(M, k, F) == (k > 2000)
+    _check_f32(M, k, F)
+
+
+@pytest.mark.parametrize("size", [(33, 4096, 300), (40, 2048, 1001), (57, 1030, 701), (64, 4100, 257)], ids=str)
+def test_fp32_products_of_33_to_64_rows(size):
+    M, k, F = size
+    assert feedforward.lib().b200_linear_f32_scratch_bytes(M, 2 * F, k) > 0
+    _check_f32(M, k, F, "gelu")
+
+
+def test_fp32_products_take_planes_from_33_rows_and_enough_work():
+    planes = lambda *a: feedforward.lib().b200_linear_f32_scratch_bytes(*a)
+    assert planes(32, 4096, 4096) == planes(4096, 32, 4096) == planes(4096, 4096, 31) == planes(0, 1, 1) == 0
+    assert planes(33, 4096, 4096) > 0 and planes(4096, 33, 4096) > 0 and planes(4096, 4096, 32) > 0 and planes(64, 4096, 4096) > 0
+    assert planes(256, 512, 512) > 0 and planes(256, 512, 511) == 0  # 2^26 multiply-adds
+
+
+@pytest.mark.parametrize("size", [(300, 700, 333), (777, 520, 1003), (583, 477, 145), (856, 237, 219), (1049, 841, 84), (1475, 570, 647)], ids=str)
+def test_both_gradients_of_fp32_come_from_one_launch(size):
+    """Sizes that take it, the longer contraction on either side."""
+    M, k, F = size
+    assert _joint(M, k, F)
+    _check_f32(M, k, F)
+
+
+@pytest.mark.parametrize("size", [(200, 512, 300), (2752, 640, 400)], ids=str)
+def test_both_gradients_of_fp32_come_from_two_launches(size):
+    M, k, F = size
+    assert not _joint(M, k, F)
+    _check_f32(M, k, F)
+
+
+@pytest.mark.parametrize("M", [32, 33])
+def test_what_a_row_of_one_large_element_leaves_of_the_others_in_fp32(M):
+    """Planes (from 33 rows on) resolve an element to 2^-22 of itself or 2^-39 of its row's largest, which shows where the largest meets a
+    zero; the products below keep every element to 2^-22. (The largest is scaled to 2^14 at least, where both planes end in steps of 2^-24: half
+    a step is 2^-25 = 2^-39 * 2^14. Rows whose largest is a power of two, as here, are those that come to 2^14.)"""
+    k, F = 2048, 512
+    x, w = torch.zeros(M, k, device=DEV), torch.zeros(2 * F, k, device=DEV)
+    large = 2.0 ** torch.arange(M, device=DEV, dtype=torch.float64) * 2.0**10  # beside 1.2345..: 2^10 to 2^42
+    x[:, 0], x[:, 1] = large.float(), 1.2345678
+    w[:, 1] = 0.7654321
+    _, p = K.gated_linear_train(x, w, "relu")
+    want = (x.double() @ w.double().t())
+    tol = 2.0**-22 * want.abs() * 3  # both operands' elements and the sum
+    if M > 32:
+        tol = tol + 2.0**-39 * large.unsqueeze(1) * 0.7654321
+    ref.assert_within(p, want, tol, "projections")
+
+
+def test_the_gates_gradient_as_a_c_entry():
+    """b200_gate_backward is b200_gate_backward_rows without a gap between rows."""
+    lib = feedforward.lib()
+    for M, F in ((5, 24), (70, 129), (300, 1000)):
+        for dtype, code in ((BF, _abi.BF16), (F16, _abi.F16), (F32, _abi.F32)):
+            dh, p = _randn(M, F, dtype=dtype, seed=3), _randn(M, 2 * F, dtype=F32, seed=4)
+            wide, tight = ops._new((M, 2 * F + 8), dtype, p.device), ops._new((M, 2 * F), dtype, p.device)
+            assert lib.b200_gate_backward(dh.data_ptr(), p.data_ptr(), tight.data_ptr(), M, F, 1, code, ops._stream_handle()) == 0
+            assert lib.b200_gate_backward_rows(dh.data_ptr(), p.data_ptr(), wide.data_ptr(), 2 * F + 8, M, F, 1, code, ops._stream_handle()) == 0
+            d, g, u = dh.double(), p[:, :F].double(), p[:, F:].double()
+            want = torch.cat([d * u * ref.slope(g, "gelu"), d * ref.act(g, "gelu")], 1)
+            fn = 2.0**-18 if dtype != F32 else 2.0**-20
+            tol = ref.U[dtype] * want.abs() + torch.cat([fn * (d * u).abs() * (1 + g.abs()), ref.act_error(g, "gelu", dtype) * (d * ref.act(g, "gelu")).abs()], 1) + ref.TINY[dtype]
+            ref.assert_within(tight, want, 1.001 * tol, f"{M} x {F}")
+            assert bits_equal(wide[:, : 2 * F], tight)
