@@ -13,8 +13,8 @@ namespace {
 constexpr int kFfThreads = 256;
 
 // ------------------------------------------------------------------ the gate
-// h = act(g) * u of fp32 projections P = [g | u] (M x 2 N). fp32 products come in two steps (their sums are
-// put together from six plane products over several launches), so the gate has a kernel of its own there.
+// h = act(g) * u of fp32 projections P = [g | u] (M x 2 N). The tensor-core products form the gate on their sums; small fp32 ones (b200_linear_f32_scratch_bytes
+// gives 0) are the package's other fp32 products, which know no gate, so it has a kernel of its own for them.
 // Backward: dP = [dh * u * act'(g) | dh * act(g)], rounded to the type of the operands it is multiplied by next, in rows of any pitch.
 template <int N> __device__ __forceinline__ void load_f32(const float* p, float* v) {
 #pragma unroll

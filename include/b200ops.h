@@ -403,7 +403,7 @@ int b200_linear_scaled(const void* A, const uint32_t* a_most, const void* B, voi
                        int64_t K, int64_t sAm, int64_t sAk, int64_t sBk, int64_t sBn, void* scratch,
                        int64_t scratch_bytes, uint32_t* status, void* stream);
 
-/* The gate by itself (fp32, whose products come in several launches), and its gradient, for contiguous fp32
+/* The gate by itself (for fp32 products that b200_gated_linear_f32 would not pay for), and its gradient, for contiguous fp32
  * projections [M, 2 N] = [g | u]: out = act(g) * u;  grad_projections = [grad * u * act'(g) | grad * act(g)], grad and
  * grad_projections of any float dtype; the last form with rows of grad_projections row_stride elements apart. */
 int b200_gate(const float* projections, float* out, int64_t M, int64_t N, int activation, void* stream);
