@@ -460,13 +460,22 @@ struct F32Operand {
 // 2^-exponent as two factors (one cannot hold all of them)
 struct ToScale {
   float a, b;
-  __device__ __forceinline__ explicit ToScale(uint32_t most) {
+  bool finite;  // the whole row
+  __device__ __forceinline__ explicit ToScale(uint32_t most) : finite(most < 0x7f800000u) {
     const int e = -scale_exponent(most), h = e >> 1;
     a = __int_as_float((h + 127) << 23);
     b = __int_as_float((e - h + 127) << 23);
   }
 };
+// A row that holds an infinity or a NaN makes no finite output, so of its elements only signs count, and which are zero or not finite: h is 1, -1 or 0, l is
+// the infinity (or NaN) itself, else 0. In h h + h l + l h an infinity meets the other operand's h alone, as it would meet the element in fp32; with h infinite
+// it would meet l too, which is as often zero or of the other sign, and every output of its row would be NaN.
 __device__ __forceinline__ void planes_of(float x0, float x1, const ToScale& s, __half2& h, __half2& l) {
+  if (!s.finite) {
+    h = __floats2half2_rn(x0 == 0.f ? 0.f : copysignf(1.f, x0), x1 == 0.f ? 0.f : copysignf(1.f, x1));
+    l = __floats2half2_rn(isfinite(x0) ? 0.f : x0, isfinite(x1) ? 0.f : x1);
+    return;
+  }
   const float y0 = x0 * s.a * s.b, y1 = x1 * s.a * s.b;
   h = __floats2half2_rn(y0, y1);
   const float2 f = __half22float2(h);

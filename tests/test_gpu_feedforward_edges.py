@@ -224,3 +224,36 @@ def test_the_gates_gradient_as_a_c_entry():
             tol = ref.U[dtype] * want.abs() + torch.cat([fn * (d * u).abs() * (1 + g.abs()), ref.act_error(g, "gelu", dtype) * (d * ref.act(g, "gelu")).abs()], 1) + ref.TINY[dtype]
             ref.assert_within(tight, want, 1.001 * tol, f"{M} x {F}")
             assert bits_equal(wide[:, : 2 * F], tight)
+
+
+def _same_where_not_finite(got, want, what):
+    """Infinities of the same sign, NaN where NaN, nothing else that is not finite (want is in 64 bits, which holds every finite value here)."""
+    got = got.double()
+    bad = ~((got == want) | (got.isnan() & want.isnan()) | (got.isfinite() & want.isfinite()))
+    assert not bad.any(), f"{what}: {int(bad.sum())} differ, first {got[bad][0].item()} for {want[bad][0].item()}"
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("size", [(20, 64, 40), (300, 512, 300), (129, 1030, 1001), (64, 4100, 257), (1531, 1027, 205)], ids=str)
+def test_infinities_are_those_of_the_formula(size, dtype):
+    """One infinity in a row or column makes its products infinite with their signs; one that meets a zero, or another of the other sign, NaN."""
+    M, k, F = size
+    x, w = _pair(M, k, F, dtype)
+    inf = float("inf")
+    x[2, 3], x[5, 1], x[7, [4, 9]], w[7, 2], w[9, 3], w[F + 4, k - 1], w[11, 3] = inf, -inf, inf, inf, -inf, inf, 0.0
+    for what, xs, ws in (("rows", x, w), ("turned", x.t().contiguous().t(), w.t().contiguous().t())):
+        out, projections = K.gated_linear_train(xs, ws, "relu")
+        p = x.double() @ w.double().t()
+        _same_where_not_finite(projections, p, what + ": projections")
+        h = ref.act(p[:, :F], "relu") * p[:, F:]
+        _same_where_not_finite(out, h, what + ": h")
+    x, w = _pair(M, k, F, dtype)
+    dh = _randn(M, F, dtype=dtype, seed=3)
+    _, projections = K.gated_linear_train(x, w)
+    dh[3, 5], dh[6, 7], dh[6, 8], w[5, 2] = inf, -inf, inf, 0.0
+    p = projections.double()
+    dp = torch.cat([dh.double() * p[:, F:] * ref.slope(p[:, :F], "silu"), dh.double() * ref.act(p[:, :F], "silu")], 1)
+    for what, xs, ws in (("rows", x, w), ("turned", x.t().contiguous().t(), w.t().contiguous().t())):
+        gx, gw = K.gated_linear_backward(dh, xs, ws, projections)
+        _same_where_not_finite(gx, dp @ w.double(), what + ": dx")
+        _same_where_not_finite(gw, dp.t() @ x.double(), what + ": dw")
