@@ -90,7 +90,8 @@ SIGNATURES = {
     "b200_gated_linear_f32": (c_int, [c_void_p] * 4 + [c_int64] * 7 + [c_int, c_void_p, c_int64, c_void_p, c_void_p]),
     "b200_linear_grads_scratch_bytes": (c_int64, [c_void_p] * 3 + [c_int64] * 8),
     "b200_linear_grads_scaled_scratch_bytes": (c_int64, [c_void_p] * 3 + [c_int64] * 8),
-    "b200_linear_grads": (c_int, [c_void_p] * 7 + [c_int64] * 6 + [c_int, c_void_p, c_int64, c_void_p, c_void_p]),
+    "b200_linear_grads": (c_int, [c_void_p] * 5 + [c_int64] * 6 + [c_int, c_void_p, c_int64, c_void_p, c_void_p]),
+    "b200_linear_grads_scaled": (c_int, [c_void_p] * 7 + [c_int64] * 6 + [c_void_p, c_int64, c_void_p, c_void_p]),
     "b200_linear_f32_grads_scratch_bytes": (c_int64, [c_int64] * 3),
     "b200_linear_f32_grads": (c_int, [c_void_p] * 5 + [c_int64] * 9 + [c_void_p, c_int64, c_void_p, c_void_p]),
     "b200_gate": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p]),

@@ -40,7 +40,7 @@ namespace {
   F(b200_scatter_add_scratch_bytes) F(b200_scatter_add) F(b200_embedding_backward_scratch_bytes) F(b200_embedding_backward) F(b200_copy_pitched) F(b200_gemm)                        \
   F(b200_gemm_takes_as_is) F(b200_gemm_f32_scratch_bytes) F(b200_gemm_f32) F(b200_gemm_splitk_scratch_bytes) F(b200_gemm_splitk) F(b200_allclose)                   \
   F(b200_gated_linear_scratch_bytes) F(b200_gated_linear) F(b200_linear_f32_scratch_bytes) F(b200_linear_f32) F(b200_gated_linear_f32) F(b200_gate)     \
-  F(b200_linear_grads_scratch_bytes) F(b200_linear_grads_scaled_scratch_bytes) F(b200_linear_grads) F(b200_linear_f32_grads_scratch_bytes) F(b200_linear_f32_grads)     \
+  F(b200_linear_grads_scratch_bytes) F(b200_linear_grads_scaled_scratch_bytes) F(b200_linear_grads) F(b200_linear_grads_scaled) F(b200_linear_f32_grads_scratch_bytes) F(b200_linear_f32_grads)     \
   F(b200_gate_backward_rows) F(b200_gate_backward_scaled) F(b200_linear_scaled_scratch_bytes) F(b200_linear_scaled) F(b200_dropout) F(b200_quantize_rows) F(b200_mm_int8_scratch_bytes) F(b200_mm_int8)
 struct Api {
 #define F(name) decltype(&::name) name;

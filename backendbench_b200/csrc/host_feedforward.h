@@ -248,7 +248,9 @@ std::tuple<TensorOpt, TensorOpt> ff_gated_linear_backward(const Tensor& g, const
         const Tensor s = ff_scratch(x, need);
         auto f = [](const Tensor& t) { return static_cast<float*>(ptr(t)); };
         const int rc = fp32 ? api.b200_linear_f32_grads(f(dp), f(x), f(w), f(dx), f(dw), r.M, 2 * F, r.K, pitch, 1, r.s_m, r.s_k, ws0, ws1, ptr(s), need, ff_status(x), stream())
-                            : api.b200_linear_grads(ptr(dp), ptr(dp_columns), static_cast<const uint32_t*>(ptr(most)), ptr(x), ptr(w), ptr(dx), ptr(dw), r.M, 2 * F, r.K, pitch, r.s_m, ws0, dt(x), ptr(s), need, ff_status(x), stream());
+                       : scaled ? api.b200_linear_grads_scaled(ptr(dp), ptr(dp_columns), static_cast<const uint32_t*>(ptr(most)), ptr(x), ptr(w), ptr(dx), ptr(dw), r.M, 2 * F, r.K, pitch, r.s_m, ws0, ptr(s),
+                                                               need, ff_status(x), stream())
+                                : api.b200_linear_grads(ptr(dp), ptr(x), ptr(w), ptr(dx), ptr(dw), r.M, 2 * F, r.K, pitch, r.s_m, ws0, dt(x), ptr(s), need, ff_status(x), stream());
         if (rc != B200_ELAUNCH) {  // (a refused cluster launch: one product after the other)
           ff_check(rc, "b200_linear_grads");
           if (mask[0]) std::get<0>(out) = dx;

@@ -34,7 +34,7 @@ struct GradParams {
   int64_t M, J, K;
   int nt;                       // tiles across
   TwoParts two;                 // 0 is dx, 1 is dw
-  const uint32_t* most[2];      // f16: largest magnitudes of g's rows and columns before they were scaled, as fp32 bits
+  const uint32_t* most[2];      // f16: largest magnitudes of g's rows and columns before they were scaled, as fp32 bits, or NULL
   int group_m;
 };
 
@@ -203,7 +203,8 @@ linear_grads(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ 
       const int64_t r0 = static_cast<int64_t>(mb) * 256 + static_cast<int64_t>(rank) * 128 + q * 32, n0 = static_cast<int64_t>(nb) * 256 + half * 128, rows = part ? p.J : p.M;
       const int left = p.K - n0 < 128 ? static_cast<int>(p.K - n0) : 128, nrows = rows - r0 < 32 ? static_cast<int>(rows - r0) : 32;  // (0 or less: none)
       const int count = (left + 63) / 64;
-      const float factor = kScaledRows && lane < nrows ? row_factor((part ? most_dw : most_dx)[r0 + lane]) : 0.f;
+      float factor = 1.f;
+      if (kScaledRows && most_dx && lane < nrows) factor = row_factor((part ? most_dw : most_dx)[r0 + lane]);
       int got = 0;
       if (lane == 0) got = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, kLinWaitNs) ? 1 : 0;
       got = __shfl_sync(0xffffffffu, got, 0);
@@ -366,15 +367,14 @@ extern "C" int64_t b200_linear_grads_scaled_scratch_bytes(const void* g, const v
   return grads_need(g, x, w, M, J, K, sgm, sxm, sxk, swj, swk, true);
 }
 
-extern "C" int b200_linear_grads(const void* g, const void* g_columns, const uint32_t* most, const void* x, const void* w, void* dx, void* dw, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sxm,
-                                 int64_t swj, int dtype, void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream) {
-  if (dtype != B200_BF16 && dtype != B200_F16) return B200_EDTYPE;
-  if (dtype == B200_BF16) g_columns = g;
-  else if (!most) return B200_EINVAL;
+namespace {
+// g by rows (for dx) and by columns (for dw), the same where neither is scaled (`most` is NULL)
+int run_linear_grads(const void* g, const void* g_columns, const uint32_t* most, const void* x, const void* w, void* dx, void* dw, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sxm, int64_t swj,
+                     int dtype, void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream) {
   if (!dx) g = g_columns;  // (the one that nobody wants need not be there)
   if (!dw) g_columns = g;
   if (!g || !g_columns || !aligned16(g_columns) || !x || !w || (!dx && !dw)) return B200_EINVAL;
-  const int64_t need = grads_need(g, x, w, M, J, K, sgm, sxm, 1, swj, 1, dtype == B200_F16);
+  const int64_t need = grads_need(g, x, w, M, J, K, sgm, sxm, 1, swj, 1, most != nullptr);
   if (need < 0) return B200_EINVAL;
   if (need && (!scratch || scratch_bytes < need)) return B200_ESCRATCH;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -402,4 +402,16 @@ extern "C" int b200_linear_grads(const void* g, const void* g_columns, const uin
   const GradTimes t(M, J, K);
   p.two = two_parts(t.first, dx ? t.tiles[0] : 0, dw ? t.tiles[1] : 0, t.tile);
   return bf16 ? launch_grads<__nv_bfloat16>(maps, dx, dw, p, launches, status, st) : launch_grads<__half>(maps, dx, dw, p, launches, status, st);
+}
+}  // namespace
+
+extern "C" int b200_linear_grads(const void* g, const void* x, const void* w, void* dx, void* dw, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sxm, int64_t swj, int dtype, void* scratch,
+                                 int64_t scratch_bytes, uint32_t* status, void* stream) {
+  if (dtype != B200_BF16 && dtype != B200_F16) return B200_EDTYPE;
+  return run_linear_grads(g, g, nullptr, x, w, dx, dw, M, J, K, sgm, sxm, swj, dtype, scratch, scratch_bytes, status, stream);
+}
+extern "C" int b200_linear_grads_scaled(const void* g, const void* g_columns, const uint32_t* most, const void* x, const void* w, void* dx, void* dw, int64_t M, int64_t J, int64_t K, int64_t sgm,
+                                        int64_t sxm, int64_t swj, void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream) {
+  if (!most) return B200_EINVAL;
+  return run_linear_grads(g, g_columns, most, x, w, dx, dw, M, J, K, sgm, sxm, swj, B200_F16, scratch, scratch_bytes, status, stream);
 }

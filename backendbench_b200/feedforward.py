@@ -218,9 +218,10 @@ def gated_linear_backward(grad_output: torch.Tensor, input: torch.Tensor, weight
             behind = (scratch.data_ptr() if need else None, need, ops._status(dp.device).data_ptr(), ops._stream_handle())
             if fp32:
                 rc = lib().b200_linear_f32_grads(*operands, *results, M, J, K, pitch, 1, *xs, *ws, *behind)
+            elif scaled:
+                rc = lib().b200_linear_grads_scaled(operands[0], dp_columns.data_ptr(), most.data_ptr(), *operands[1:], *results, M, J, K, pitch, xs[0], ws[0], *behind)
             else:
-                columns = (dp_columns.data_ptr(), most.data_ptr()) if scaled else (None, None)
-                rc = lib().b200_linear_grads(operands[0], *columns, *operands[1:], *results, M, J, K, pitch, xs[0], ws[0], ops._dt(dp.dtype), *behind)
+                rc = lib().b200_linear_grads(*operands, *results, M, J, K, pitch, xs[0], ws[0], ops._dt(dp.dtype), *behind)
             if rc != ELAUNCH:  # (a refused cluster launch: one product after the other)
                 check(rc, "b200_linear_grads")
                 return dx, dw

@@ -378,17 +378,20 @@ int b200_gated_linear_f32(const float* x, const float* w, float* out, float* pro
                           void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream);
 
 /* Both gradients of y = x w^T in one launch (bf16, f16): dx [M, K] = g w and dw [J, K] = g^T x, contiguous, of g [M, J] with rows on the
- * 16-byte grid, x [M, K] and w [J, K] with rows along K; dx or dw may be NULL, and the other is the same then. f16: g comes as
- * b200_gate_backward_scaled leaves it, `g` by rows (for dx), `g_columns` by columns (for dw), `most` with their magnitudes; bf16
- * takes `g` for both and looks at neither. b200_linear_grads_scratch_bytes (f16: _scaled_) is -1 where one product after the other is the
+ * 16-byte grid, x [M, K] and w [J, K] with rows along K; dx or dw may be NULL, and the other is the same then. The scaled form is for f16, with g as
+ * b200_gate_backward_scaled leaves it: `g` by rows (for dx; not read where that is NULL), `g_columns` by columns (for dw, likewise), `most` with their magnitudes.
+ * The two scratch_bytes are -1 where one product after the other is the
  * better way (few tiles with a long contraction, or J up to 128 or K up to 64) or an operand lies otherwise. */
 int64_t b200_linear_grads_scratch_bytes(const void* g, const void* x, const void* w, int64_t M, int64_t J, int64_t K,
                                         int64_t sgm, int64_t sxm, int64_t sxk, int64_t swj, int64_t swk);
+int b200_linear_grads(const void* g, const void* x, const void* w, void* dx, void* dw, int64_t M, int64_t J,
+                      int64_t K, int64_t sgm, int64_t sxm, int64_t swj, int dtype, void* scratch,
+                      int64_t scratch_bytes, uint32_t* status, void* stream);
 int64_t b200_linear_grads_scaled_scratch_bytes(const void* g, const void* x, const void* w, int64_t M, int64_t J, int64_t K,
                                                int64_t sgm, int64_t sxm, int64_t sxk, int64_t swj, int64_t swk);
-int b200_linear_grads(const void* g, const void* g_columns, const uint32_t* most, const void* x, const void* w,
-                      void* dx, void* dw, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sxm, int64_t swj, int dtype, void* scratch,
-                      int64_t scratch_bytes, uint32_t* status, void* stream);
+int b200_linear_grads_scaled(const void* g, const void* g_columns, const uint32_t* most, const void* x, const void* w,
+                             void* dx, void* dw, int64_t M, int64_t J, int64_t K, int64_t sgm, int64_t sxm, int64_t swj,
+                             void* scratch, int64_t scratch_bytes, uint32_t* status, void* stream);
 /* The same in fp32, by planes like b200_linear_f32, operands of any strides */
 int64_t b200_linear_f32_grads_scratch_bytes(int64_t M, int64_t J, int64_t K);
 int b200_linear_f32_grads(const float* g, const float* x, const float* w, float* dx, float* dw, int64_t M,

@@ -18,8 +18,9 @@ def test_entries_for_f16_gradients_refuse_bad_arguments():
     assert product(None, None, None, None, 0, 8, 64, 64, 1, 1, 64) == 0
     assert lib.b200_linear_scaled_scratch_bytes(BASE, BASE, 4, 8, 64, 64, 1, 1, 64) == 0  # B as the transpose of rows along K
     assert lib.b200_linear_scaled_scratch_bytes(BASE, BASE, 4, 8, 64, 64, 1, 8, 1) >= 8 * 64 * 2
-    grads = lambda g, c, most, x, w, dx, dw, dtype: lib.b200_linear_grads(g, c, most, x, w, dx, dw, 256, 256, 256, 256, 256, 256, dtype, None, 0, None, None)
-    assert grads(BASE, BASE, None, BASE, BASE, BASE, BASE, F16) == -1  # f16 without its magnitudes
-    assert grads(BASE, None, BASE, BASE, BASE, BASE, BASE, F16) == -1 and grads(None, BASE, BASE, BASE, BASE, BASE, BASE, F16) == -1
-    assert grads(BASE, BASE, BASE, BASE, BASE, None, None, F16) == -1 and grads(None, None, None, BASE, BASE, BASE, BASE, BF) == -1
-    assert grads(BASE, BASE, BASE, BASE, BASE, BASE, BASE, _abi.F32) == -2
+    grads = lambda *operands: lib.b200_linear_grads_scaled(*operands, 256, 256, 256, 256, 256, 256, None, 0, None, None)
+    assert grads(BASE, BASE, None, BASE, BASE, BASE, BASE) == -1  # without the magnitudes
+    assert grads(BASE, None, BASE, BASE, BASE, BASE, BASE) == -1 and grads(None, BASE, BASE, BASE, BASE, BASE, BASE) == -1
+    assert grads(BASE, BASE, BASE, BASE, BASE, None, None) == -1 and grads(BASE, BASE, BASE, None, BASE, BASE, BASE) == -1
+    plain = lambda g, dx, dw, dtype: lib.b200_linear_grads(g, BASE, BASE, dx, dw, 256, 256, 256, 256, 256, 256, dtype, None, 0, None, None)
+    assert plain(None, BASE, BASE, BF) == -1 and plain(BASE, None, None, F16) == -1 and plain(BASE, BASE, BASE, _abi.F32) == -2

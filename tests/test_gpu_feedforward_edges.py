@@ -257,3 +257,25 @@ def test_infinities_are_those_of_the_formula(size, dtype):
         gx, gw = K.gated_linear_backward(dh, xs, ws, projections)
         _same_where_not_finite(gx, dp @ w.double(), what + ": dx")
         _same_where_not_finite(gw, dp.t() @ x.double(), what + ": dw")
+
+
+@pytest.mark.parametrize("dtype", [BF, F16], ids=["bf16", "f16"])
+def test_both_gradients_of_a_linear_layer_as_a_c_entry(dtype):
+    """dx = g w and dw = g^T x of a 16-bit g as it is, both and each by itself."""
+    lib, (M, J, k) = feedforward.lib(), (300, 664, 520)
+    g, x, w = _randn(M, J, dtype=dtype, seed=1), _randn(M, k, dtype=dtype, seed=2), _randn(J, k, dtype=dtype, seed=3)
+    need = lib.b200_linear_grads_scratch_bytes(g.data_ptr(), x.data_ptr(), w.data_ptr(), M, J, k, J, k, 1, k, 1)
+    assert need >= 0
+    scratch = ops._scratch(g.device, max(need, 1))
+    g64, x64, w64 = g.double(), x.double(), w.double()
+    want = g64 @ w64, g64.t() @ x64
+    tol = [ref.U[dtype] * v.abs() + ref.sum_error(n, dtype) * m + ref.TINY[dtype] for v, n, m in zip(want, (J, M), (g64.abs() @ w64.abs(), g64.abs().t() @ x64.abs()))]
+    for wanted in ((0, 1), (0,), (1,)):
+        out = [ops._new(v.shape, dtype, g.device) if i in wanted else None for i, v in enumerate(want)]
+        rc = lib.b200_linear_grads(
+            g.data_ptr(), x.data_ptr(), w.data_ptr(), *(o.data_ptr() if o is not None else None for o in out), M, J, k, J, k, k, ops._dt(dtype),
+            scratch.data_ptr(), need, ops._status(g.device).data_ptr(), ops._stream_handle(),
+        )
+        assert rc == 0
+        for i in wanted:
+            ref.assert_within(out[i], want[i], 1.001 * tol[i], ("dx", "dw")[i])
