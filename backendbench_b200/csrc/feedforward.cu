@@ -146,6 +146,7 @@ template <typename ACT, bool WRITE, bool VECTOR>
 __global__ void __launch_bounds__(kFfThreads)
 gate_backward_scaled(const __half* dh, const float* p, __half* __restrict__ by_rows, __half* __restrict__ by_cols, uint32_t* row_most, uint32_t* col_most, int64_t M, int64_t N, int64_t pitch) {
   __shared__ uint32_t part[WRITE ? 1 : 8][2 * kScaledCols];
+  next_grid_may_start();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t across = (N + kScaledCols - 1) / kScaledCols, tiles = (M + kScaledRows - 1) / kScaledRows * across;
   for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
@@ -177,6 +178,9 @@ gate_backward_scaled(const __half* dh, const float* p, __half* __restrict__ by_r
     }
     float col[4][2];
     if constexpr (WRITE) {
+      after_grids_before();  // (dh and P were complete before the first pass, which is launched the ordinary way)
+      row_most = waited(row_most);
+      col_most = waited(col_most);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const bool in = n0 + kStep * c < N;
@@ -281,18 +285,17 @@ int launch_gate_backward_scaled(const __half* dh, const float* p, __half* by_row
   const bool vec = N % 4 == 0 && pitch % 4 == 0 && aligned16(p) && ((reinterpret_cast<uintptr_t>(dh) | reinterpret_cast<uintptr_t>(by_rows) | reinterpret_cast<uintptr_t>(by_cols)) & 7u) == 0;
   const int64_t tiles = (M + kScaledRows - 1) / kScaledRows * ((N + kScaledCols - 1) / kScaledCols), room = kNumSMs * 16LL;
   const int grid = static_cast<int>(tiles < room ? tiles : room);
-  const cudaError_t e = cudaMemsetAsync(most, 0, static_cast<size_t>(M + 2 * N) * 4, st);
+  cudaError_t e = cudaMemsetAsync(most, 0, static_cast<size_t>(M + 2 * N) * 4, st);
   if (e != cudaSuccess) { set_last_cuda_error(e); return B200_ELAUNCH; }
   gate_act_each(act, [&](auto a) {
-    auto go = [&](auto kernel) { kernel<<<grid, kFfThreads, 0, st>>>(dh, p, by_rows, by_cols, most, most + M, M, N, pitch); };
-    if (vec) {
-      go(gate_backward_scaled<decltype(a), false, true>);
-      go(gate_backward_scaled<decltype(a), true, true>);
-    } else {
-      go(gate_backward_scaled<decltype(a), false, false>);
-      go(gate_backward_scaled<decltype(a), true, false>);
-    }
+    auto go = [&](auto look, auto write) {
+      look<<<grid, kFfThreads, 0, st>>>(dh, p, by_rows, by_cols, most, most + M, M, N, pitch);
+      e = launch_after(write, grid, kFfThreads, 0, st, dh, p, by_rows, by_cols, most, most + M, M, N, pitch);
+    };
+    if (vec) go(gate_backward_scaled<decltype(a), false, true>, gate_backward_scaled<decltype(a), true, true>);
+    else go(gate_backward_scaled<decltype(a), false, false>, gate_backward_scaled<decltype(a), true, false>);
   });
+  if (e != cudaSuccess) { set_last_cuda_error(e); return B200_ELAUNCH; }
   return check_launch(2);
 }
 
