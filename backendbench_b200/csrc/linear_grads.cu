@@ -351,7 +351,7 @@ int64_t grads_need(const void* g, const void* x, const void* w, int64_t M, int64
   // rows that this lets through: 19 % faster than one product after the other on average, slower by more than 3 % for 38; up to 128 rows, which are half a
   // tile, 27 to 39 % faster for J up to 1400, even at 2048.
   // f16 has other products to weigh against (b200_linear_scaled), which turn dP, x and w first, 2.6e-6 us an element: 17 x 22016 x 4096 363 us with
-  // them, 135 here; 1024 x 4096 x 1024 95 and 53.
+  // them, 134 here; 1024 x 4096 x 1024 95 and 50.
   const double turned = 2.6e-6 * (static_cast<double>(J) * static_cast<double>(K) + static_cast<double>(M) * static_cast<double>(J + K));
   const double most = f16 ? 20. + turned : M <= 128 ? 10. : 20.;
   if (t.longest >= most && ((M <= 128 && !f16) || t.longest > 1.75 * t.even)) return -1;
