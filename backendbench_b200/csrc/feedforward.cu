@@ -179,8 +179,6 @@ gate_backward_scaled(const __half* dh, const float* p, __half* __restrict__ by_r
     float col[4][2];
     if constexpr (WRITE) {
       after_grids_before();  // (dh and P were complete before the first pass, which is launched the ordinary way)
-      row_most = waited(row_most);
-      col_most = waited(col_most);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const bool in = n0 + kStep * c < N;
